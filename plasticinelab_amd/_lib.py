@@ -1,4 +1,5 @@
-"""ctypes binding of libplmpm.so (include/plmpm.h; the tools of include/plmpm_tools.h for bench.py / profiles / tests).
+"""ctypes binding of libplmpm.so (include/plmpm.h; the tools of include/plmpm_tools.h for bench.py / profiles / tests; the policy-training
+operators of include/plmpm_policy.h).
 
 There is no fallback: if the HIP library is missing or fails to load, importing
 the engine raises.  Build it with ``python -c "import __graft_entry__ as g; g.build()"``
@@ -144,7 +145,45 @@ SYMBOLS = {
     "plmpm_profile_read": (_I, [_P, _P, _P]),
 }
 
+# ---- include/plmpm_policy.h: the policy-training operators (policy.py, optimizer/adamw.py); bound when first used
+class Scan(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("reserved", C.c_int32), ("batch", C.c_int64), ("steps", C.c_int64), ("width", C.c_int64),
+                ("stride_b", C.c_int64 * 3), ("stride_t", C.c_int64 * 3), ("c", _D), ("x", _P), ("r", _P), ("i", _P), ("decay", _P), ("h0", _P),
+                ("reset", _P), ("h", _P), ("h_last", _P), ("checkpoint", _P), ("dh", _P), ("dlast", _P), ("dx", _P), ("dr", _P), ("di", _P),
+                ("ddecay", _P), ("dh0", _P), ("workspace", _P), ("workspace_bytes", C.c_size_t)]
+
+
+class Norm(C.Structure):
+    _fields_ = [("x_dtype", C.c_int32), ("u_dtype", C.c_int32), ("w_dtype", C.c_int32), ("gate_fn", C.c_int32), ("rows", C.c_int64), ("width", C.c_int64),
+                ("stride_x", C.c_int64), ("stride_u", C.c_int64), ("stride_gate", C.c_int64), ("stride_dy", C.c_int64), ("stride_dz", C.c_int64),
+                ("eps", _D), ("x", _P), ("u", _P), ("gate", _P), ("scale", _P), ("post", _P), ("pre", _P), ("y", _P), ("z", _P), ("dy", _P), ("dz", _P),
+                ("dx", _P), ("du", _P), ("dgate", _P), ("dscale", _P), ("dpost", _P), ("dpre", _P), ("workspace", _P), ("workspace_bytes", C.c_size_t)]
+
+
+class AdamWTensor(C.Structure):
+    _fields_ = [("p", _P), ("g", _P), ("m", _P), ("v", _P), ("m_scale", _P), ("v_scale", _P), ("master", _P), ("n", C.c_int64),
+                ("dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
+class AdamWStep(C.Structure):
+    _fields_ = [("state_bits", C.c_int32), ("reserved", C.c_int32), ("lr", _D), ("beta_1", _D), ("beta_2", _D), ("epsilon", _D), ("weight_decay", _D),
+                ("max_norm", _D), ("lo", _D), ("hi", _D), ("step", _P), ("grad_norm", _P), ("workspace", _P), ("workspace_bytes", C.c_size_t)]
+
+
+POLICY_SYMBOLS = {
+    "plmpm_scan_workspace": (_I, [C.POINTER(Scan), _I, C.POINTER(C.c_size_t)]),
+    "plmpm_scan_forward": (_I, [C.POINTER(Scan), _P]),
+    "plmpm_scan_backward": (_I, [C.POINTER(Scan), _P]),
+    "plmpm_norm_workspace": (_I, [C.POINTER(Norm), C.POINTER(C.c_size_t)]),
+    "plmpm_norm_forward": (_I, [C.POINTER(Norm), _P]),
+    "plmpm_norm_backward": (_I, [C.POINTER(Norm), _P]),
+    "plmpm_adamw_workspace": (_I, [C.POINTER(AdamWStep), _P, _I, C.POINTER(C.c_size_t)]),
+    "plmpm_adamw_step": (_I, [C.POINTER(AdamWStep), _P, _I, _P]),
+    "plmpm_adamw_values": (_I, [_P, _P, _P, _P, _P, _I, _P]),
+}
+
 _lib = None
+_policy = None
 
 
 class EngineError(RuntimeError):
@@ -164,10 +203,18 @@ def load():
     return _lib
 
 
-def bind(lib):
+def load_policy():
+    """The same library with the entry points of include/plmpm_policy.h bound (a build made before they were there still loads)."""
+    global _policy
+    if _policy is None:
+        _policy = bind(load(), POLICY_SYMBOLS)
+    return _policy
+
+
+def bind(lib, symbols=SYMBOLS):
     """Give every entry point of a loaded build of the library its ctypes signature (load() for the product build; the tests'
     CPU interpreter of the device source, tests/emul_engine.py, binds its own build of the same sources)."""
-    for name, (res, args) in SYMBOLS.items():
+    for name, (res, args) in symbols.items():
         fn = getattr(lib, name)          # AttributeError if the library lacks a declared symbol
         fn.restype, fn.argtypes = res, args
     return lib

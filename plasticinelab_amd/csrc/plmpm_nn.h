@@ -1,0 +1,124 @@
+// Shared by the policy-training operators (plmpm_scan.hip, plmpm_norm.hip, plmpm_adamw.hip): element types and their conversions, vector
+// loads and stores of VW neighbouring elements, sums over a wave and over the waves of a row.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+#include <cstring>
+
+#include "../../include/plmpm_policy.h"
+
+int plmpm_fail(const char* fmt, ...);          // plmpm_capi.hip: sets the text of plmpm_last_error, returns -1
+#define NN_REQUIRE(cond, ...) do { if (!(cond)) return plmpm_fail(__VA_ARGS__); } while (0)
+#define NN_LAUNCHED(what)                                                                                           \
+    do {                                                                                                            \
+        hipError_t e_ = hipGetLastError();                                                                          \
+        if (e_ != hipSuccess) return plmpm_fail("%s: launch failed: %s", what, hipGetErrorString(e_));              \
+    } while (0)
+
+namespace plbnn {
+
+struct bf16 { uint16_t v; };
+struct f16 { uint16_t v; };
+
+__device__ __forceinline__ float as_f(uint32_t u) { float f; memcpy(&f, &u, 4); return f; }
+__device__ __forceinline__ uint32_t as_u(float f) { uint32_t u; memcpy(&u, &f, 4); return u; }
+
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(bf16 x) { return as_f((uint32_t)x.v << 16); }
+#if defined(PLB_HOST_EMUL)
+inline float to_f(f16 x) {
+    const uint32_t s = (uint32_t)(x.v & 0x8000) << 16, e = (x.v >> 10) & 31, m = x.v & 1023;
+    if (e == 31) return as_f(s | 0x7f800000u | (m << 13));
+    if (e) return as_f(s | ((e + 112) << 23) | (m << 13));
+    const float f = (float)m * 5.9604644775390625e-8f;         // subnormal: m 2^-24
+    return s ? -f : f;
+}
+inline void from_f(float f, bf16& o) {
+    const uint32_t u = as_u(f);
+    o.v = f != f ? 0x7fc0 : (uint16_t)((u + 0x7fffu + ((u >> 16) & 1)) >> 16);
+}
+inline void from_f(float f, f16& o) {
+    const uint32_t u = as_u(f), s = (u >> 16) & 0x8000;
+    const float a = std::fabs(f);
+    if (f != f) { o.v = 0x7e00; return; }
+    if (a >= 65520.0f) { o.v = (uint16_t)(s | 0x7c00); return; }
+    if (a < 6.103515625e-5f) { o.v = (uint16_t)(s | (uint32_t)std::nearbyint(a * 16777216.0f)); return; }
+    const uint32_t b = as_u(a), r = b + 0xfffu + ((b >> 13) & 1);
+    o.v = (uint16_t)(s | ((r - (112u << 23)) >> 13));
+}
+inline float exp2_fast(float x) { return exp2f(x); }
+inline void sleep_a_little() { __builtin_amdgcn_s_sleep(1); }
+#else
+__device__ __forceinline__ float to_f(f16 x) { _Float16 h; memcpy(&h, &x, 2); return (float)h; }
+// round to nearest even, one conversion instruction each
+__device__ __forceinline__ void from_f(float f, bf16& o) { const __bf16 h = (__bf16)f; memcpy(&o, &h, 2); }
+__device__ __forceinline__ void from_f(float f, f16& o) { const _Float16 h = (_Float16)f; memcpy(&o, &h, 2); }
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }       // v_exp_f32: within 1 ulp; exponents below -126 give 0
+__device__ __forceinline__ void sleep_a_little() { __builtin_amdgcn_s_sleep(1); }
+#endif
+__device__ __forceinline__ void from_f(float f, float& o) { o = f; }
+
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+// 1 / (1 + e^-x): both ends come out right by themselves (e^-x = inf -> 0, 0 -> 1)
+__device__ __forceinline__ float sigmoid_fast(float x) { return __builtin_amdgcn_rcpf(1.0f + exp2_fast(-kLog2e * x)); }
+
+// N neighbouring elements as one access of the widest type their bytes allow (up to 16; more: several)
+template <int BYTES> struct Wide;
+template <> struct Wide<2> { typedef uint16_t type; };
+template <> struct Wide<4> { typedef uint32_t type; };
+template <> struct Wide<8> { struct alignas(8) type { uint32_t w[2]; }; };
+template <> struct Wide<16> { struct alignas(16) type { uint32_t w[4]; }; };
+template <class T, int N> struct Vec {
+    static constexpr int bytes = N * (int)sizeof(T), part = bytes > 16 ? 16 : bytes, parts = bytes / part;
+    typedef typename Wide<part>::type W;
+    W w[parts];
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int k = 0; k < parts; ++k) w[k] = reinterpret_cast<const W*>(p)[k];
+    }
+    __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+        for (int k = 0; k < parts; ++k) reinterpret_cast<W*>(p)[k] = w[k];
+    }
+    __device__ __forceinline__ void zero() { memset(w, 0, sizeof(w)); }
+    __device__ __forceinline__ void get(float* f) const {
+        T e[N];
+        memcpy(e, w, sizeof(w));
+#pragma unroll
+        for (int k = 0; k < N; ++k) f[k] = to_f(e[k]);
+    }
+    __device__ __forceinline__ void set(const float* f) {
+        T e[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) from_f(f[k], e[k]);
+        memcpy(w, e, sizeof(w));
+    }
+};
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+    return v;
+}
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+    return v;
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) { const uint32_t o = (uint32_t)__shfl_xor((int)v, m); v = o > v ? o : v; }
+    return v;
+}
+
+// host side: bytes that a pointer and a stride (in elements) both keep to
+inline int aligned_to(const void* p, int64_t stride, int size) {
+    const uint64_t a = (uint64_t)(uintptr_t)p | ((uint64_t)stride * (uint64_t)size);
+    return (a & 15) == 0 ? 16 : (a & 7) == 0 ? 8 : (a & 3) == 0 ? 4 : (a & 1) == 0 ? 2 : 1;
+}
+inline int dtype_size(int dtype) { return dtype == PLMPM_NN_F32 ? 4 : 2; }
+inline size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
+
+}  // namespace plbnn

@@ -1,0 +1,94 @@
+"""CPU tier: the policy-training operators' device source on the CPU interpreter (tests/host_emul/hipemu), against their 64-bit forms, and the
+refusals of their Python and C surfaces.  tests/test_gpu_policy_ops.py runs the same checks, and larger ones, on a GPU."""
+import ctypes as C
+import os
+import re
+import subprocess
+
+import pytest
+import torch
+
+from plasticinelab_amd import _lib
+from plasticinelab_amd import policy as P
+from plasticinelab_amd.optimizer import AdamW, adamw_step, adamw_values
+from tests import policy_cases as cases
+from tests.util import ROOT
+
+HERE = os.path.join(ROOT, "tests", "host_emul")
+SOURCES = "plmpm_capi.hip plmpm_kinematics.hip plmpm_loss.hip plmpm_migrate.hip plmpm_peer.hip plmpm_scan.hip plmpm_norm.hip plmpm_adamw.hip"
+
+
+@pytest.fixture(scope="module")
+def interpreter():
+    """The operators' library compiled by g++ for the interpreter; tensors on the CPU stand for device memory.  (PLMPM_EMUL_VARIANT=asan: under
+    AddressSanitizer, with the LD_PRELOAD of tests/test_emul_tier.py.)"""
+    tag = "_asan" if os.environ.get("PLMPM_EMUL_VARIANT") == "asan" else ""
+    out = f"libplmpm_policy_emul{tag}.so"
+    subprocess.check_call(["make", "-s", "-j", "6", "-C", HERE, f"OBJDIR=build_emul_policy{tag}", f"OUT={out}", f"SAN={1 if tag else 0}",
+                           "HDRS=" + " ".join(os.path.join("../../plasticinelab_amd/csrc", h) for h in ("plmpm_nn.h", "plmpm_kernels.h")) + " ../../include/plmpm_policy.h",
+                           "SRCS=" + SOURCES, out])
+    lib = _lib.bind(C.CDLL(os.path.join(HERE, out)), {**_lib.POLICY_SYMBOLS, "plmpm_last_error": _lib.SYMBOLS["plmpm_last_error"]})
+    import contextlib
+    patch = pytest.MonkeyPatch()
+    patch.setattr(P, "_library", lambda: lib)
+    patch.setattr(P, "_site", lambda t: (0, contextlib.nullcontext()))
+    yield "cpu"
+    patch.undo()
+
+
+def test_policy_header_and_binding_agree():
+    text = re.sub(r"/\*.*?\*/", "", open(os.path.join(ROOT, "include", "plmpm_policy.h")).read(), flags=re.S)
+    assert sorted(set(re.findall(r"\b(plmpm_[a-z_0-9]+)\s*\(", text))) == sorted(_lib.POLICY_SYMBOLS)
+    lib = _lib.load_policy()
+    for name in _lib.POLICY_SYMBOLS:
+        assert hasattr(lib, name)
+    assert C.sizeof(_lib.Scan) == 4 * 8 + 6 * 8 + 8 + 18 * 8 and C.sizeof(_lib.Norm) == 16 + 7 * 8 + 8 + 18 * 8
+    assert C.sizeof(_lib.AdamWTensor) == 72 and C.sizeof(_lib.AdamWStep) == 8 + 8 * 8 + 4 * 8
+
+
+@pytest.mark.parametrize("B,T,D,dtype,layout,resets", [
+    (1, 1, 1, "f32", "plain", 0.0), (2, 7, 64, "bf16", "plain", 0.3), (1, 64, 65, "f32", "packed", 0.0), (2, 65, 130, "f16", "packed", 0.1),
+    (1, 129, 128, "f32", "time_major", 0.05), (3, 20, 33, "bf16", "odd", 0.0), (1, 200, 6, "f32", "plain", 0.0)])
+def test_scan(interpreter, B, T, D, dtype, layout, resets):
+    cases.run_scan(interpreter, 11, B, T, D, dtype, layout, resets=resets, with_h0=T != 20)
+
+
+@pytest.mark.parametrize("use", [("h",), ("last",)])
+def test_scan_with_one_gradient(interpreter, use):
+    cases.run_scan(interpreter, 5, 2, 70, 16, "f32", use=use)
+
+
+def test_scan_step(interpreter):
+    cases.run_step(interpreter, 3, 5, 66, "bf16")
+
+
+@pytest.mark.parametrize("shape,tx,tu,fn,strided", [
+    ((3, 8), "f32", "f32", "sigmoid", False), ((2, 5, 33), "bf16", "bf16", "silu", False), ((9, 130), "f32", "f16", "identity", True),
+    ((5, 520), "f16", "f16", "sigmoid", True), ((2, 2050), "f32", "bf16", "silu", False), ((70, 1), "f32", "f32", "sigmoid", False)])
+def test_norm(interpreter, shape, tx, tu, fn, strided):
+    cases.run_norm(interpreter, 21, shape, tx, tu, fn, strided=strided)
+
+
+@pytest.mark.parametrize("use,grads", [(("pre",), ("dz",)), (("u",), ("dy",)), (("u", "pre"), ("dz",)), (("u", "gate", "post"), ("dy",)), (("u", "gate", "pre"), ("dy",))])
+def test_norm_parts(interpreter, use, grads):
+    cases.run_norm(interpreter, 22, (6, 72), "f32", "f32", use=use, grads=grads)
+    cases.run_norm(interpreter, 23, (3, 600), "bf16", "bf16", use=use, grads=grads, weights=torch.bfloat16)
+
+
+def test_norm_first_of_a_16_bit_block_next_to_a_float_stream(interpreter):
+    cases.run_norm(interpreter, 24, (4, 40), "f32", "bf16", use=("pre",), grads=("dz",), dtype=torch.bfloat16)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("sizes,dtypes,offset", [((1, 5, 300, 4096), ("f32",), 0), ((4097, 255), ("bf16", "f32", "f16"), 0), ((700, 4100), ("f32", "bf16"), 1)])
+def test_adamw(interpreter, bits, sizes, dtypes, offset):
+    cases.run_adamw(interpreter, 31, sizes, dtypes, bits, lr=1e-2, offset=offset, max_norm=0.05)
+
+
+def test_adamw_without_masters_or_a_gradient_and_with_bounds(interpreter):
+    cases.run_adamw(interpreter, 32, (40, 33), ("bf16",), 32, lr=0.1, masters=False)
+    cases.run_adamw(interpreter, 33, (40, 33, 7), ("f32",), 8, lr=0.5, missing=(1,), bounds=(-0.3, 0.2), max_norm=1e3)
+
+
+def test_adamw_more_tensors_than_one_launch_takes(interpreter):
+    cases.run_adamw(interpreter, 34, tuple(range(1, 102)), ("f32",), 32, steps=2, max_norm=0.1)
