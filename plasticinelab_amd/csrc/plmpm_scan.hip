@@ -2,10 +2,19 @@
 //
 //   a_t = exp(la_t), la_t = -c softplus(decay) sigmoid(r_t);   h_t = a_t h_{t-1} + m_t sigmoid(i_t) x_t,  m_t = sqrt(1 - a_t^2)
 //
-// A run of steps acts on the state as h -> A h + H (A the product of its a, H what it ends with from zero), and runs compose, so a
-// tile of 64 steps is cut into sub-runs of S steps, one a wave: every wave reduces its sub-run from registers to (A, H), the
-// channels' owners chain the sub-runs through LDS from the tile's state, and every wave replays its sub-run from the state it
-// starts with.  Inputs are read once and stay in registers between the two walks.
+// A run of steps acts on the state as h -> A h + H (A the product of its a, H what it ends with from zero), and runs compose.  A workgroup
+// takes a tile (S steps a wave, W waves) of 64 VEC channels: every wave reduces its sub-run from registers to (A, H), the channels'
+// owners chain the sub-runs through LDS from the state the tile starts with, and every wave replays its sub-run from the state it starts with.
+// Inputs are read once and stay in registers between the two walks.
+//
+// The state a tile starts with comes from the tiles before it while all of them are under way: a tile first publishes its own (A, H) for each
+// channel, then walks back over its predecessors' until it meets one that already knows the state it ends with, and publishes
+// its own end.  A word of 64 bits holds what is published and says what it is, so one relaxed store and load (agent scope: past the caches of the
+// compute units and of the eight dies) carry both, and nothing else has to be ordered.  Tiles are handed out by a ticket in the order of time, all
+// channels of a tile before the next tile: whoever waits, waits for tickets below its own, which are held by workgroups that run already
+// and publish before they wait -- the lowest unfinished ticket waits for nobody, so every wait ends.
+// The words and the ticket are cleared by a small kernel before each launch (not a memset node: calls may be captured).
+//
 // A reset makes the run forget what came before, also a NaN: its A is then -0 (every genuine A is +0 or above), and whoever
 // composes runs takes H alone where the sign is set.
 #include "plmpm_nn.h"
@@ -14,8 +23,8 @@ using namespace plbnn;
 
 namespace {
 
-constexpr int kTile = 64;               // steps of a tile, forward and backward: the checkpoints' spacing
-constexpr int kMaxWaves = 8;
+constexpr int kCheckpoint = 64;         // steps between the states kept for the backward pass
+typedef unsigned long long Word;
 
 struct ScanArgs {
     const void* in[3];
@@ -28,6 +37,8 @@ struct ScanArgs {
     const float* dlast;
     void* out[3];                       // dx, dr, di
     float *part, *dh0;                  // part: [tiles][batch][width] sums of dla sigmoid(r)
+    unsigned* ticket;
+    Word* words;                        // [tiles][batch][width], in the order the tiles are handed out
     int64_t B, T;
     int D, cblks, tiles;
     float c;
@@ -58,237 +69,315 @@ template <int S> __device__ __forceinline__ unsigned reset_bits(const ScanArgs& 
     return (unsigned)__ballot(hit);
 }
 
-template <class T, int VEC, int S, bool RESET>
-__global__ __launch_bounds__(kTile / S * 64) void k_scan_forward(ScanArgs A) {
+// What a tile publishes for a channel: the state behind it in the high half; in the low half 0 (nothing yet), the bits of its A plus one (A and
+// H of the tile alone), or all ones (the high half is the state itself).
+constexpr unsigned kState = 0xffffffffu;
+__device__ __forceinline__ Word word_of(float A, float H) {
+    const unsigned a = A != A ? 0x7fc00000u : as_u(A);
+    return ((Word)as_u(H) << 32) | (a + 1u);
+}
+__device__ __forceinline__ Word state_word(float h) { return ((Word)as_u(h) << 32) | kState; }
+__device__ __forceinline__ void publish(Word* p, Word w) { __hip_atomic_store(p, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ Word look(const Word* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// the state that position `pos` starts with: back over the positions before it (`p`: this channel's word at position 0, `stride` words
+// apart), four at a time.  Position 0 publishes its state, so the walk ends there at the latest.
+__device__ __forceinline__ float state_before(const Word* p, int64_t stride, int pos) {
+    float A = 1.0f, H = 0.0f;
+    int j = pos - 1;
+    for (;;) {
+        Word w[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) w[q] = look(p + (j > q ? j - q : 0) * stride);
+        bool waits = false;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (waits || j < 0) continue;
+            const unsigned low = (unsigned)w[q];
+            const float h = as_f((unsigned)(w[q] >> 32));
+            if (low == 0) { waits = true; continue; }
+            H = fmaf(A, h, H);
+            if (low == kState) return H;
+            A *= as_f(low - 1u);
+            if (forgets(as_f(low - 1u))) return H;
+            --j;
+        }
+        if (waits) sleep_a_little();
+    }
+}
+
+// which tile and which channels this workgroup takes: in the order of a ticket where there is more than one tile
+struct Place { int64_t b; int pos, first; };
+template <int NCH> __device__ __forceinline__ Place place(const ScanArgs& A, unsigned* shared) {
+    unsigned id = blockIdx.x;
+    if (A.tiles > 1) {
+        if (threadIdx.x == 0) *shared = atomicAdd(A.ticket, 1u);
+        __syncthreads();
+        id = (unsigned)__builtin_amdgcn_readfirstlane((int)*shared);
+    }
+    const unsigned blocks = (unsigned)(A.B * A.cblks), rest = id % blocks;
+    return {(int64_t)(rest / (unsigned)A.cblks), (int)(id / blocks), (int)(rest % (unsigned)A.cblks) * NCH};
+}
+
+template <class T, int VEC, int S, int W, bool RESET>
+__global__ __launch_bounds__(W * 64) void k_scan_forward(ScanArgs A) {
     constexpr int NCH = 64 * VEC;
-    __shared__ float sA[kTile / S][NCH], sH[kTile / S][NCH], carry[NCH];
+    __shared__ float sA[W][NCH], sH[W][NCH];
+    __shared__ unsigned ticket;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int64_t b = blockIdx.x / A.cblks;
-    const int first = (int)(blockIdx.x % A.cblks) * NCH, d0 = first + lane * VEC;
+    const Place at = place<NCH>(A, &ticket);
+    const int64_t b = at.b;
+    const int first = at.first, d0 = first + lane * VEC;
     const bool live = d0 < A.D;                          // VEC divides the width: a lane's channels are all there or none is
     const int dl = live ? d0 : 0;
-    float k2[VEC];
+    const int64_t t0 = (int64_t)at.pos * (S * W) + wave * S;
+    Vec<T, VEC> raw[3][S];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) k2[v] = -A.c * kLog2e * softplus(A.decay[dl + v]);
-    for (int ch = threadIdx.x; ch < NCH; ch += blockDim.x)
-        carry[ch] = A.h0 && first + ch < A.D ? A.h0[b * A.D + first + ch] : 0.0f;
-    __syncthreads();
-    for (int tile = 0; tile < A.tiles; ++tile) {
-        const int64_t t0 = (int64_t)tile * kTile + wave * S;
-        Vec<T, VEC> raw[3][S];
+    for (int k = 0; k < 3; ++k) {
+        const T* p = (const T*)A.in[k] + b * A.sb[k];
 #pragma unroll
-        for (int k = 0; k < 3; ++k) {
-            const T* p = (const T*)A.in[k] + b * A.sb[k];
+        for (int s = 0; s < S; ++s) raw[k][s].load(p + (t0 + s < A.T ? t0 + s : A.T - 1) * A.st[k] + dl);
+    }
+    const unsigned cut = RESET ? reset_bits<S>(A, b, t0) : 0u;
+    float k2[VEC], a[S][VEC], u[S][VEC], PA[VEC], PH[VEC];
 #pragma unroll
-            for (int s = 0; s < S; ++s) raw[k][s].load(p + (t0 + s < A.T ? t0 + s : A.T - 1) * A.st[k] + dl);
-        }
-        const unsigned cut = RESET ? reset_bits<S>(A, b, t0) : 0u;
-        float a[S][VEC], u[S][VEC], PA[VEC], PH[VEC];
+    for (int v = 0; v < VEC; ++v) {
+        k2[v] = -A.c * kLog2e * softplus(A.decay[dl + v]);
+        PA[v] = 1.0f;
+        PH[v] = 0.0f;
+    }
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) { PA[v] = 1.0f; PH[v] = 0.0f; }
+    for (int s = 0; s < S; ++s) {
+        float x[VEC], r[VEC], i[VEC];
+        raw[0][s].get(x);
+        raw[1][s].get(r);
+        raw[2][s].get(i);
+        const bool there = t0 + s < A.T;                 // a step behind the end leaves the state as it is
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            float x[VEC], r[VEC], i[VEC];
-            raw[0][s].get(x);
-            raw[1][s].get(r);
-            raw[2][s].get(i);
-            const bool there = t0 + s < A.T;             // a step behind the end leaves the state as it is
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const Gates g = gates(r[v], i[v], k2[v]);
-                a[s][v] = there ? g.a : 1.0f;
-                u[s][v] = there ? __builtin_amdgcn_sqrtf(g.m2) * g.si * x[v] : 0.0f;
-                if (RESET && (cut >> s & 1)) {
-                    u[s][v] = g.si * x[v];
-                    PA[v] = -0.0f;
-                    PH[v] = u[s][v];
-                } else {
-                    PA[v] *= a[s][v];
-                    PH[v] = fmaf(a[s][v], PH[v], u[s][v]);
-                }
+        for (int v = 0; v < VEC; ++v) {
+            const Gates g = gates(r[v], i[v], k2[v]);
+            a[s][v] = there ? g.a : 1.0f;
+            u[s][v] = there ? __builtin_amdgcn_sqrtf(g.m2) * g.si * x[v] : 0.0f;
+            if (RESET && (cut >> s & 1)) {
+                u[s][v] = g.si * x[v];
+                PA[v] = -0.0f;
+                PH[v] = u[s][v];
+            } else {
+                PA[v] *= a[s][v];
+                PH[v] = fmaf(a[s][v], PH[v], u[s][v]);
             }
         }
+    }
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) { sA[wave][lane * VEC + v] = PA[v]; sH[wave][lane * VEC + v] = PH[v]; }
-        __syncthreads();
-        for (int ch = threadIdx.x; ch < NCH; ch += blockDim.x) {
-            float c = carry[ch];
-            if (A.ckpt && first + ch < A.D) A.ckpt[((int64_t)tile * A.B + b) * A.D + first + ch] = c;
+    for (int v = 0; v < VEC; ++v) { sA[wave][lane * VEC + v] = PA[v]; sH[wave][lane * VEC + v] = PH[v]; }
+    __syncthreads();
+    for (int ch = threadIdx.x; ch < NCH; ch += blockDim.x) {
+        if (first + ch >= A.D) continue;
+        const int64_t col = b * A.D + first + ch, stride = A.B * A.D;
+        float c;
+        if (at.pos == 0) c = A.h0 ? A.h0[col] : 0.0f;
+        else {
+            float ta = 1.0f, th = 0.0f;
             for (int w = 0; w < waves; ++w) {
                 const float pa = sA[w][ch], ph = sH[w][ch];
-                sA[w][ch] = c;
-                c = forgets(pa) ? ph : fmaf(pa, c, ph);
+                th = forgets(pa) ? ph : fmaf(pa, th, ph);
+                ta = forgets(pa) ? -0.0f : ta * pa;
             }
-            carry[ch] = c;
-            if (A.h_last && tile == A.tiles - 1 && first + ch < A.D) A.h_last[b * A.D + first + ch] = c;
+            if (at.pos < A.tiles - 1) publish(A.words + (int64_t)at.pos * stride + col, word_of(ta, th));
+            c = state_before(A.words + col, stride, at.pos);
         }
-        __syncthreads();
-        float now[VEC];
+        for (int w = 0; w < waves; ++w) {
+            const float pa = sA[w][ch], ph = sH[w][ch];
+            const int64_t t = (int64_t)at.pos * (S * W) + w * S;
+            if (A.ckpt && t % kCheckpoint == 0 && t < A.T) A.ckpt[(t / kCheckpoint) * stride + col] = c;
+            sA[w][ch] = c;
+            c = forgets(pa) ? ph : fmaf(pa, c, ph);
+        }
+        if (at.pos < A.tiles - 1) publish(A.words + (int64_t)at.pos * stride + col, state_word(c));
+        else if (A.h_last) A.h_last[col] = c;
+    }
+    __syncthreads();
+    float now[VEC];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) now[v] = sA[wave][lane * VEC + v];
-        T* out = (T*)A.h + (b * A.T + t0) * A.D + d0;
+    for (int v = 0; v < VEC; ++v) now[v] = sA[wave][lane * VEC + v];
+    T* out = (T*)A.h + (b * A.T + t0) * A.D + d0;
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
+    for (int s = 0; s < S; ++s) {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) now[v] = RESET && (cut >> s & 1) ? u[s][v] : fmaf(a[s][v], now[v], u[s][v]);
-            if (live && t0 + s < A.T) {
-                Vec<T, VEC> o;
-                o.set(now);
-                o.store(out + (int64_t)s * A.D);
-            }
+        for (int v = 0; v < VEC; ++v) now[v] = RESET && (cut >> s & 1) ? u[s][v] : fmaf(a[s][v], now[v], u[s][v]);
+        if (live && t0 + s < A.T) {
+            Vec<T, VEC> o;
+            o.set(now);
+            o.store(out + (int64_t)s * A.D);
         }
     }
 }
 
 // Backward: g_t = dh_t + a_{t+1} g_{t+1}, walked from the end.  With e_t = a_t g_t as what a step hands to the one before it, a run acts
 // on what comes in from behind as e -> A e + E with the same A, so both walks (forward again from the tile's checkpoint, which gives
-// h_{t-1} in 32 bits, and backward) go through one exchange.
+// h_{t-1} in 32 bits, and backward) go through one exchange; tiles are handed out from the last to the first.
 //   dx = g m s_i   di = g m x s_i (1 - s_i)   dla = g (a h_{t-1} - s_i x a^2 / m)   dr = dla la (1 - s_r)
 // For la -> 0 the product la a^2 / m goes to 0 (m ~ sqrt(-2 la)): where m is 0 that term is left out.
-template <class T, int VEC, int S, bool RESET>
-__global__ __launch_bounds__(kTile / S * 64) void k_scan_backward(ScanArgs A) {
+template <class T, int VEC, int S, int W, bool RESET>
+__global__ __launch_bounds__(W * 64) void k_scan_backward(ScanArgs A) {
+    static_assert(S * W % kCheckpoint == 0, "a tile starts at a checkpoint");
     constexpr int NCH = 64 * VEC;
-    __shared__ float sA[kTile / S][NCH], sH[kTile / S][NCH], sE[kTile / S][NCH], carry[NCH];
+    __shared__ float sA[W][NCH], sH[W][NCH], sE[W][NCH];
+    __shared__ unsigned ticket;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int64_t b = blockIdx.x / A.cblks;
-    const int first = (int)(blockIdx.x % A.cblks) * NCH, d0 = first + lane * VEC;
+    const Place at = place<NCH>(A, &ticket);
+    const int tile = A.tiles - 1 - at.pos;
+    const int64_t b = at.b;
+    const int first = at.first, d0 = first + lane * VEC;
     const bool live = d0 < A.D;
     const int dl = live ? d0 : 0;
-    float k2[VEC];
+    const int64_t t0 = (int64_t)tile * (S * W) + wave * S;
+    Vec<T, VEC> raw[3][S], rawg[S];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) k2[v] = -A.c * kLog2e * softplus(A.decay[dl + v]);
-    for (int ch = threadIdx.x; ch < NCH; ch += blockDim.x)
-        carry[ch] = A.dlast && first + ch < A.D ? A.dlast[b * A.D + first + ch] : 0.0f;
-    __syncthreads();
-    for (int tile = A.tiles - 1; tile >= 0; --tile) {
-        const int64_t t0 = (int64_t)tile * kTile + wave * S;
-        Vec<T, VEC> raw[3][S], rawg[S];
+    for (int s = 0; s < S; ++s) {
+        const int64_t t = t0 + s < A.T ? t0 + s : A.T - 1;
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const int64_t t = t0 + s < A.T ? t0 + s : A.T - 1;
+        for (int k = 0; k < 3; ++k) raw[k][s].load((const T*)A.in[k] + b * A.sb[k] + t * A.st[k] + dl);
+        if (A.dh) rawg[s].load((const T*)A.dh + (b * A.T + t) * A.D + dl);
+        else rawg[s].zero();
+    }
+    const unsigned cut = RESET ? reset_bits<S>(A, b, t0) : 0u;
+    float k2[VEC], a[S][VEC], m2[S][VEC], sr[S][VEC], si[S][VEC], PA[VEC], PH[VEC], PE[VEC];
 #pragma unroll
-            for (int k = 0; k < 3; ++k) raw[k][s].load((const T*)A.in[k] + b * A.sb[k] + t * A.st[k] + dl);
-            if (A.dh) rawg[s].load((const T*)A.dh + (b * A.T + t) * A.D + dl);
-            else rawg[s].zero();
-        }
-        const unsigned cut = RESET ? reset_bits<S>(A, b, t0) : 0u;
-        float a[S][VEC], m2[S][VEC], sr[S][VEC], si[S][VEC], PA[VEC], PH[VEC], PE[VEC];
+    for (int v = 0; v < VEC; ++v) {
+        k2[v] = -A.c * kLog2e * softplus(A.decay[dl + v]);
+        PA[v] = 1.0f;
+        PH[v] = PE[v] = 0.0f;
+    }
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) { PA[v] = 1.0f; PH[v] = PE[v] = 0.0f; }
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            float x[VEC], r[VEC], i[VEC];
-            raw[0][s].get(x);
-            raw[1][s].get(r);
-            raw[2][s].get(i);
-            const bool there = t0 + s < A.T;
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const Gates g = gates(r[v], i[v], k2[v]);
-                a[s][v] = there ? g.a : 1.0f;
-                m2[s][v] = there ? g.m2 : 0.0f;
-                sr[s][v] = g.sr;
-                si[s][v] = g.si;
-                const float u = there ? __builtin_amdgcn_sqrtf(g.m2) * g.si * x[v] : 0.0f;
-                if (RESET && (cut >> s & 1)) {
-                    a[s][v] = 0.0f;
-                    m2[s][v] = 1.0f;
-                    PA[v] = -0.0f;
-                    PH[v] = g.si * x[v];
-                } else {
-                    PA[v] *= a[s][v];
-                    PH[v] = fmaf(a[s][v], PH[v], u);
-                }
-            }
-        }
-#pragma unroll
-        for (int s = S - 1; s >= 0; --s) {
-            float g[VEC];
-            rawg[s].get(g);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v)
-                PE[v] = RESET && (cut >> s & 1) ? 0.0f : t0 + s < A.T ? a[s][v] * (g[v] + PE[v]) : PE[v];
-        }
+    for (int s = 0; s < S; ++s) {
+        float x[VEC], r[VEC], i[VEC];
+        raw[0][s].get(x);
+        raw[1][s].get(r);
+        raw[2][s].get(i);
+        const bool there = t0 + s < A.T;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            sA[wave][lane * VEC + v] = PA[v];
-            sH[wave][lane * VEC + v] = PH[v];
-            sE[wave][lane * VEC + v] = PE[v];
+            const Gates g = gates(r[v], i[v], k2[v]);
+            a[s][v] = there ? g.a : 1.0f;
+            m2[s][v] = there ? g.m2 : 0.0f;
+            sr[s][v] = g.sr;
+            si[s][v] = g.si;
+            const float u = there ? __builtin_amdgcn_sqrtf(g.m2) * g.si * x[v] : 0.0f;
+            if (RESET && (cut >> s & 1)) {
+                a[s][v] = 0.0f;
+                m2[s][v] = 1.0f;
+                PA[v] = -0.0f;
+                PH[v] = g.si * x[v];
+            } else {
+                PA[v] *= a[s][v];
+                PH[v] = fmaf(a[s][v], PH[v], u);
+            }
         }
-        __syncthreads();
-        for (int ch = threadIdx.x; ch < NCH; ch += blockDim.x) {
-            float e = carry[ch], c = first + ch < A.D ? A.ckpt[((int64_t)tile * A.B + b) * A.D + first + ch] : 0.0f;
+    }
+#pragma unroll
+    for (int s = S - 1; s >= 0; --s) {
+        float g[VEC];
+        rawg[s].get(g);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v)
+            PE[v] = RESET && (cut >> s & 1) ? 0.0f : t0 + s < A.T ? a[s][v] * (g[v] + PE[v]) : PE[v];
+    }
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        sA[wave][lane * VEC + v] = PA[v];
+        sH[wave][lane * VEC + v] = PH[v];
+        sE[wave][lane * VEC + v] = PE[v];
+    }
+    __syncthreads();
+    for (int ch = threadIdx.x; ch < NCH; ch += blockDim.x) {
+        if (first + ch >= A.D) continue;
+        const int64_t col = b * A.D + first + ch, stride = A.B * A.D;
+        float c = A.ckpt[(int64_t)tile * (S * W / kCheckpoint) * stride + col], e;
+        if (at.pos == 0) e = A.dlast ? A.dlast[col] : 0.0f;
+        else {
+            float ta = 1.0f, te = 0.0f;
             for (int w = waves - 1; w >= 0; --w) {
                 const float pa = sA[w][ch], pe = sE[w][ch];
-                sE[w][ch] = e;
-                e = forgets(pa) ? pe : fmaf(pa, e, pe);
+                te = forgets(pa) ? pe : fmaf(pa, te, pe);
+                ta = forgets(pa) ? -0.0f : ta * pa;
             }
-            for (int w = 0; w < waves; ++w) {
-                const float pa = sA[w][ch], ph = sH[w][ch];
-                sA[w][ch] = c;
-                c = forgets(pa) ? ph : fmaf(pa, c, ph);
-            }
-            carry[ch] = e;
-            if (A.dh0 && tile == 0 && first + ch < A.D) A.dh0[b * A.D + first + ch] = e;
+            if (at.pos < A.tiles - 1) publish(A.words + (int64_t)at.pos * stride + col, word_of(ta, te));
+            e = state_before(A.words + col, stride, at.pos);
         }
-        __syncthreads();
-        float now[VEC], e[VEC], hp[S][VEC], sum[VEC];
+        for (int w = waves - 1; w >= 0; --w) {
+            const float pa = sA[w][ch], pe = sE[w][ch];
+            sE[w][ch] = e;
+            e = forgets(pa) ? pe : fmaf(pa, e, pe);
+        }
+        if (at.pos < A.tiles - 1) publish(A.words + (int64_t)at.pos * stride + col, state_word(e));
+        else if (A.dh0) A.dh0[col] = e;
+        for (int w = 0; w < waves; ++w) {
+            const float pa = sA[w][ch], ph = sH[w][ch];
+            sA[w][ch] = c;
+            c = forgets(pa) ? ph : fmaf(pa, c, ph);
+        }
+    }
+    __syncthreads();
+    float now[VEC], e[VEC], hp[S][VEC], sum[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        now[v] = sA[wave][lane * VEC + v];
+        e[v] = sE[wave][lane * VEC + v];
+        sum[v] = 0.0f;
+    }
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        float x[VEC];
+        raw[0][s].get(x);
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            now[v] = sA[wave][lane * VEC + v];
-            e[v] = sE[wave][lane * VEC + v];
-            sum[v] = 0.0f;
+            hp[s][v] = now[v];
+            const float u = __builtin_amdgcn_sqrtf(m2[s][v]) * si[s][v] * x[v];
+            now[v] = RESET && (cut >> s & 1) ? u : fmaf(a[s][v], now[v], u);
         }
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            float x[VEC];
-            raw[0][s].get(x);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                hp[s][v] = now[v];
-                const float u = __builtin_amdgcn_sqrtf(m2[s][v]) * si[s][v] * x[v];
-                now[v] = RESET && (cut >> s & 1) ? u : fmaf(a[s][v], now[v], u);
-            }
-        }
-#pragma unroll
-        for (int s = S - 1; s >= 0; --s) {
-            float x[VEC], g[VEC], dx[VEC], dr[VEC], di[VEC];
-            raw[0][s].get(x);
-            rawg[s].get(g);
-            const bool there = t0 + s < A.T;
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                g[v] = (there ? g[v] : 0.0f) + e[v];
-                const bool reset = RESET && (cut >> s & 1);
-                e[v] = reset ? 0.0f : a[s][v] * g[v];
-                const float inv = m2[s][v] > 0.0f ? __builtin_amdgcn_rsqf(m2[s][v]) : 0.0f;
-                const float sx = si[s][v] * x[v], m = m2[s][v] * inv, gm = g[v] * m;
-                dx[v] = gm * si[s][v];
-                di[v] = gm * sx * (1.0f - si[s][v]);
-                const float dla = reset || !there ? 0.0f : g[v] * (a[s][v] * hp[s][v] - sx * (a[s][v] * a[s][v] * inv));
-                dr[v] = dla * (k2[v] * kLn2 * sr[s][v]) * (1.0f - sr[s][v]);
-                sum[v] += dla * sr[s][v];
-            }
-            if (live && there) {
-                const int64_t at = (b * A.T + t0 + s) * A.D + d0;
-                Vec<T, VEC> o;
-                o.set(dx); o.store((T*)A.out[0] + at);
-                o.set(dr); o.store((T*)A.out[1] + at);
-                o.set(di); o.store((T*)A.out[2] + at);
-            }
-        }
-        // the tile's share of d decay: one row of `part`, summed over the waves (sH is free: its last reader is behind the barrier)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) sH[wave][lane * VEC + v] = sum[v];
-        __syncthreads();
-        for (int ch = threadIdx.x; ch < NCH; ch += blockDim.x)
-            if (first + ch < A.D) {
-                float p = 0.0f;
-                for (int w = 0; w < waves; ++w) p += sH[w][ch];
-                A.part[((int64_t)tile * A.B + b) * A.D + first + ch] = p;
-            }
-        __syncthreads();
     }
+#pragma unroll
+    for (int s = S - 1; s >= 0; --s) {
+        float x[VEC], g[VEC], dx[VEC], dr[VEC], di[VEC];
+        raw[0][s].get(x);
+        rawg[s].get(g);
+        const bool there = t0 + s < A.T;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            g[v] = (there ? g[v] : 0.0f) + e[v];
+            const bool reset = RESET && (cut >> s & 1);
+            e[v] = reset ? 0.0f : a[s][v] * g[v];
+            const float inv = m2[s][v] > 0.0f ? __builtin_amdgcn_rsqf(m2[s][v]) : 0.0f;
+            const float sx = si[s][v] * x[v], m = m2[s][v] * inv, gm = g[v] * m;
+            dx[v] = gm * si[s][v];
+            di[v] = gm * sx * (1.0f - si[s][v]);
+            const float dla = reset || !there ? 0.0f : g[v] * (a[s][v] * hp[s][v] - sx * (a[s][v] * a[s][v] * inv));
+            dr[v] = dla * (k2[v] * kLn2 * sr[s][v]) * (1.0f - sr[s][v]);
+            sum[v] += dla * sr[s][v];
+        }
+        if (live && there) {
+            const int64_t to = (b * A.T + t0 + s) * A.D + d0;
+            Vec<T, VEC> o;
+            o.set(dx); o.store((T*)A.out[0] + to);
+            o.set(dr); o.store((T*)A.out[1] + to);
+            o.set(di); o.store((T*)A.out[2] + to);
+        }
+    }
+    // the tile's share of d decay: one row of `part`, summed over the waves (sH is free: its last reader is behind the barrier)
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) sH[wave][lane * VEC + v] = sum[v];
+    __syncthreads();
+    for (int ch = threadIdx.x; ch < NCH; ch += blockDim.x)
+        if (first + ch < A.D) {
+            float p = 0.0f;
+            for (int w = 0; w < waves; ++w) p += sH[w][ch];
+            A.part[((int64_t)tile * A.B + b) * A.D + first + ch] = p;
+        }
+}
+
+__global__ __launch_bounds__(256) void k_clear(Word* p, int64_t n) {
+    for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < n; k += (int64_t)gridDim.x * 256) p[k] = 0;
 }
 
 // d decay[d] = -c sigmoid(decay[d]) * (sum of column d of part[rows][D]): 64 columns and 16 strips of rows a workgroup, strips joined in a
@@ -307,16 +396,29 @@ __global__ __launch_bounds__(1024) void k_decay_grad(const float* part, const fl
     }
 }
 
-template <class T, int VEC, int S, bool RESET> void launch(const ScanArgs& A, bool backward, hipStream_t st) {
+// Steps a wave and waves a workgroup of the two kernels.  Measured at 65537 steps x 1024 channels (forward) and 8 x 2047 x 2048 (both), bf16, us:
+// forward 16 x 8 141 / 83, 8 x 8 186 / 84, 8 x 16 181 / 104, 16 x 16 168 / 99, 4 x 16 271 / 139; backward 8 x 8 192, 8 x 16 201, 4 x 16 205,
+// 16 x 8 227, 16 x 4 221.  (One workgroup a channel block walking all steps by itself: 3650 / 157 and 273.)
+constexpr int kForwardSteps = 16, kForwardWaves = 8, kBackwardSteps = 8, kBackwardWaves = 8;
+int tile_of(bool backward) { return backward ? kBackwardSteps * kBackwardWaves : kForwardSteps * kForwardWaves; }
+int64_t tiles_of(const plmpm_scan* s, bool backward) { return (s->steps + tile_of(backward) - 1) / tile_of(backward); }
+// workspace: one word for the ticket, the words, and (backward) the rows of d decay's sums
+size_t word_bytes(const plmpm_scan* s, bool backward) {
+    const int64_t tiles = tiles_of(s, backward);
+    return tiles > 1 ? sizeof(Word) * (1 + (size_t)tiles * s->batch * s->width) : 0;
+}
+
+template <class T, int VEC, bool RESET> void launch(const ScanArgs& A, bool backward, hipStream_t st) {
+    const int S = backward ? kBackwardSteps : kForwardSteps, W = backward ? kBackwardWaves : kForwardWaves;
     const int64_t need = (A.T + S - 1) / S;
-    const int waves = (int)(need < kTile / S ? need : kTile / S);
-    const dim3 grid((unsigned)(A.B * A.cblks)), block((unsigned)(waves * 64));
-    if (backward) hipLaunchKernelGGL((k_scan_backward<T, VEC, S, RESET>), grid, block, 0, st, A);
-    else hipLaunchKernelGGL((k_scan_forward<T, VEC, S, RESET>), grid, block, 0, st, A);
+    const int waves = (int)(need < W ? need : W);
+    const dim3 grid((unsigned)(A.B * A.cblks * A.tiles)), block((unsigned)(waves * 64));
+    if (backward) hipLaunchKernelGGL((k_scan_backward<T, VEC, kBackwardSteps, kBackwardWaves, RESET>), grid, block, 0, st, A);
+    else hipLaunchKernelGGL((k_scan_forward<T, VEC, kForwardSteps, kForwardWaves, RESET>), grid, block, 0, st, A);
 }
 template <class T, int VEC> void launch(const ScanArgs& A, bool backward, hipStream_t st) {
-    if (A.reset) launch<T, VEC, 8, true>(A, backward, st);
-    else launch<T, VEC, 8, false>(A, backward, st);
+    if (A.reset) launch<T, VEC, true>(A, backward, st);
+    else launch<T, VEC, false>(A, backward, st);
 }
 template <class T> void launch(const ScanArgs& A, int vec, bool backward, hipStream_t st) {
     if (vec == 2) launch<T, 2>(A, backward, st);
@@ -340,7 +442,8 @@ int check(const plmpm_scan* s, bool backward, bool pointers) {
     NN_REQUIRE(s->batch >= 0 && s->steps >= 0 && s->width >= 0, "scan: negative size");
     NN_REQUIRE(s->width < (1 << 30), "scan: width %lld is too large", (long long)s->width);
     NN_REQUIRE(s->steps < ((int64_t)1 << 36), "scan: %lld steps are too many", (long long)s->steps);
-    NN_REQUIRE(s->batch < (1 << 30) && s->batch * ((s->width + 63) / 64) < ((int64_t)1 << 31), "scan: batch x width is too large for one launch");
+    NN_REQUIRE(s->batch < (1 << 30) && s->batch * ((s->width + 63) / 64) < ((int64_t)1 << 31) &&
+               s->batch * ((s->width + 63) / 64) * ((s->steps + kCheckpoint - 1) / kCheckpoint) < ((int64_t)1 << 31), "scan: batch x width x steps is too large for one launch");
     NN_REQUIRE(s->c > 0 && s->c < 1e30, "scan: c has to be positive and finite, got %g", s->c);
     if (!pointers || !s->batch || !s->steps || !s->width) return 0;
     NN_REQUIRE(s->x && s->r && s->i && s->decay, "scan: x, r, i and decay are needed");
@@ -358,17 +461,26 @@ int run(const plmpm_scan* s, bool backward, hipStream_t st) {
     size_t need = 0;
     if (plmpm_scan_workspace(s, backward, &need)) return -1;
     NN_REQUIRE(s->workspace_bytes >= need && (s->workspace || !need), "scan: the workspace has %zu bytes, %zu are needed", s->workspace_bytes, need);
+    NN_REQUIRE((uintptr_t)s->workspace % 8 == 0, "scan: the workspace is not aligned to 8 bytes");
     ScanArgs A{};
     A.in[0] = s->x; A.in[1] = s->r; A.in[2] = s->i;
     for (int k = 0; k < 3; ++k) { A.sb[k] = s->stride_b[k]; A.st[k] = s->stride_t[k]; }
     A.decay = s->decay; A.h0 = s->h0; A.reset = s->reset;
     A.h = s->h; A.h_last = s->h_last; A.ckpt = s->checkpoint;
     A.dh = s->dh; A.dlast = s->dlast; A.out[0] = s->dx; A.out[1] = s->dr; A.out[2] = s->di;
-    A.dh0 = s->dh0; A.part = (float*)s->workspace;
+    A.dh0 = s->dh0;
     A.B = s->batch; A.T = s->steps; A.D = (int)s->width; A.c = (float)s->c;
     const int vec = vector_of(s, backward);
     A.cblks = (A.D + 64 * vec - 1) / (64 * vec);
-    A.tiles = (int)((s->steps + kTile - 1) / kTile);
+    A.tiles = (int)tiles_of(s, backward);
+    const size_t words = word_bytes(s, backward);
+    A.part = (float*)((char*)s->workspace + words);
+    if (words) {
+        A.ticket = (unsigned*)s->workspace;
+        A.words = (Word*)s->workspace + 1;
+        const int64_t n = (int64_t)(words / sizeof(Word)), groups = (n + 1023) / 1024;
+        hipLaunchKernelGGL(k_clear, dim3((unsigned)(groups < 2048 ? groups : 2048)), dim3(256), 0, st, (Word*)s->workspace, n);
+    }
     if (s->dtype == PLMPM_NN_F32) launch<float>(A, vec, backward, st);
     else if (s->dtype == PLMPM_NN_BF16) launch<bf16>(A, vec, backward, st);
     else launch<f16>(A, vec, backward, st);
@@ -385,7 +497,7 @@ extern "C" {
 int plmpm_scan_workspace(const plmpm_scan* s, int backward, size_t* bytes) {
     NN_REQUIRE(bytes, "scan: null argument");
     if (check(s, backward != 0, false)) return -1;
-    *bytes = backward ? (size_t)((s->steps + kTile - 1) / kTile) * s->batch * s->width * sizeof(float) : 0;
+    *bytes = word_bytes(s, backward != 0) + (backward ? (size_t)tiles_of(s, true) * s->batch * s->width * sizeof(float) : 0);
     return 0;
 }
 int plmpm_scan_forward(const plmpm_scan* s, void* hip_stream) { return run(s, false, (hipStream_t)hip_stream); }
