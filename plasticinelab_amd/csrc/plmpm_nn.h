@@ -56,7 +56,7 @@ __device__ __forceinline__ float to_f(f16 x) { _Float16 h; memcpy(&h, &x, 2); re
 __device__ __forceinline__ void from_f(float f, bf16& o) { const __bf16 h = (__bf16)f; memcpy(&o, &h, 2); }
 __device__ __forceinline__ void from_f(float f, f16& o) { const _Float16 h = (_Float16)f; memcpy(&o, &h, 2); }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }       // v_exp_f32: within 1 ulp; exponents below -126 give 0
-__device__ __forceinline__ void sleep_a_little() { __builtin_amdgcn_s_sleep(1); }
+__device__ __forceinline__ void sleep_a_little() { __builtin_amdgcn_s_sleep(8); }        // 8 x 64 cycles
 #endif
 __device__ __forceinline__ void from_f(float f, float& o) { o = f; }
 
@@ -83,6 +83,19 @@ template <class T, int N> struct Vec {
         for (int k = 0; k < parts; ++k) reinterpret_cast<W*>(p)[k] = w[k];
     }
     __device__ __forceinline__ void zero() { memset(w, 0, sizeof(w)); }
+    // unpack again from here on (16-bit elements: the compiler would keep the floats, twice the registers, from an earlier get)
+    __device__ __forceinline__ void forget() {
+#if !defined(PLB_HOST_EMUL)
+        if (sizeof(T) == 2 && part == 4)
+#pragma unroll
+            for (int k = 0; k < parts; ++k) {
+                uint32_t u;
+                memcpy(&u, &w[k], 4);
+                asm("" : "+v"(u));
+                memcpy(&w[k], &u, 4);
+            }
+#endif
+    }
     __device__ __forceinline__ void get(float* f) const {
         T e[N];
         memcpy(e, w, sizeof(w));

@@ -17,6 +17,9 @@
 //
 // A reset makes the run forget what came before, also a NaN: its A is then -0 (every genuine A is +0 or above), and whoever
 // composes runs takes H alone where the sign is set.
+#include <algorithm>
+#include <type_traits>
+
 #include "plmpm_nn.h"
 
 using namespace plbnn;
@@ -39,6 +42,7 @@ struct ScanArgs {
     float *part, *dh0;                  // part: [tiles][batch][width] sums of dla sigmoid(r)
     unsigned* ticket;
     Word* words;                        // [tiles][batch][width], in the order the tiles are handed out
+    float* k2;                          // [width]: -c log2(e) softplus(decay), where there is more than one tile
     int64_t B, T;
     int D, cblks, tiles;
     float c;
@@ -63,10 +67,43 @@ __device__ __forceinline__ Gates gates(float r, float i, float k2) {
 }
 
 // which of the S steps from t on are resets: a bit each (uniform over the wave)
-template <int S> __device__ __forceinline__ unsigned reset_bits(const ScanArgs& A, int64_t b, int64_t t) {
+template <int S> __device__ __forceinline__ unsigned reset_bits(const ScanArgs& A, int64_t b, int64_t t, int left) {
     const int lane = threadIdx.x & 63;
-    const int hit = lane < S && t + lane < A.T ? A.reset[b * A.T + t + lane] != 0 : 0;
+    const int hit = lane < S && lane < left ? A.reset[b * A.T + t + lane] != 0 : 0;
     return (unsigned)__ballot(hit);
+}
+
+// a row's address, the same for the whole wave, plus a lane's 32-bit offset: the empty asm keeps the row's address in scalar registers (the compiler
+// would otherwise add row and offset once a lane in 64 bits, and hold two vector registers for each of the 48 loads in flight)
+template <class T> __device__ __forceinline__ T* at_offset(T* row, unsigned bytes) {
+#if defined(PLB_HOST_EMUL)
+    return (T*)((char*)row + bytes);
+#else
+    typedef char __attribute__((address_space(1))) * Global;
+    const uint64_t r = (uint64_t)row;
+    unsigned lo = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)r), hi = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(r >> 32));
+    uint64_t u = ((uint64_t)hi << 32) | lo;
+    asm("" : "+s"(u));
+    return (T*)(char*)((Global)u + bytes);
+#endif
+}
+
+// S steps from t on, `stride` elements apart: whole, or the first `left` of them (those behind load the last one again)
+template <bool WHOLE, class T, int VEC, int S> __device__ __forceinline__ void load_steps(const void* base, int64_t stride, int left, unsigned offset, Vec<T, VEC> (&raw)[S]) {
+    T* row = (T*)base;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        raw[s].load(at_offset(row, offset));
+        if (WHOLE || s + 1 < left) row += stride;
+    }
+}
+template <int VEC> __device__ __forceinline__ void load_k2(const ScanArgs& A, int d, float (&k2)[VEC]) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) k2[v] = A.k2 ? A.k2[d + v] : -A.c * kLog2e * softplus(A.decay[d + v]);
+}
+__device__ __forceinline__ int steps_left(int64_t T, int64_t t, int most) {
+    const int64_t n = T - t;
+    return n < most ? (n < 0 ? 0 : (int)n) : most;
 }
 
 // What a tile publishes for a channel: the state behind it in the high half; in the low half 0 (nothing yet), the bits of its A plus one (A and
@@ -81,17 +118,18 @@ __device__ __forceinline__ void publish(Word* p, Word w) { __hip_atomic_store(p,
 __device__ __forceinline__ Word look(const Word* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 // the state that position `pos` starts with: back over the positions before it (`p`: this channel's word at position 0, `stride` words
-// apart), four at a time.  Position 0 publishes its state, so the walk ends there at the latest.
+// apart), two at a time (each poll goes past the caches: 65537 x 1024 forward / 8 x 2047 x 2048 backward 134 / 131 us, four at a time 133 / 143, eight
+// 143 / 171 without the later steps; without any of this, wrong, 118 / 129).  Position 0 publishes its state, so the walk ends there at the latest.
 __device__ __forceinline__ float state_before(const Word* p, int64_t stride, int pos) {
     float A = 1.0f, H = 0.0f;
     int j = pos - 1;
     for (;;) {
-        Word w[4];
+        Word w[2];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) w[q] = look(p + (j > q ? j - q : 0) * stride);
+        for (int q = 0; q < 2; ++q) w[q] = look(p + (j > q ? j - q : 0) * stride);
         bool waits = false;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < 2; ++q) {
             if (waits || j < 0) continue;
             const unsigned low = (unsigned)w[q];
             const float h = as_f((unsigned)(w[q] >> 32));
@@ -115,8 +153,10 @@ template <int NCH> __device__ __forceinline__ Place place(const ScanArgs& A, uns
         __syncthreads();
         id = (unsigned)__builtin_amdgcn_readfirstlane((int)*shared);
     }
-    const unsigned blocks = (unsigned)(A.B * A.cblks), rest = id % blocks;
-    return {(int64_t)(rest / (unsigned)A.cblks), (int)(id / blocks), (int)(rest % (unsigned)A.cblks) * NCH};
+    // (divisions run in vector registers: back to scalar ones, or every row's address would be built a lane)
+    const unsigned blocks = (unsigned)(A.B * A.cblks), pos = (unsigned)__builtin_amdgcn_readfirstlane((int)(id / blocks)), rest = id - pos * blocks;
+    const unsigned b = (unsigned)__builtin_amdgcn_readfirstlane((int)(rest / (unsigned)A.cblks));
+    return {(int64_t)b, (int)pos, (int)(rest - b * (unsigned)A.cblks) * NCH};
 }
 
 template <class T, int VEC, int S, int W, bool RESET>
@@ -131,43 +171,46 @@ __global__ __launch_bounds__(W * 64) void k_scan_forward(ScanArgs A) {
     const bool live = d0 < A.D;                          // VEC divides the width: a lane's channels are all there or none is
     const int dl = live ? d0 : 0;
     const int64_t t0 = (int64_t)at.pos * (S * W) + wave * S;
-    Vec<T, VEC> raw[3][S];
-#pragma unroll
-    for (int k = 0; k < 3; ++k) {
-        const T* p = (const T*)A.in[k] + b * A.sb[k];
-#pragma unroll
-        for (int s = 0; s < S; ++s) raw[k][s].load(p + (t0 + s < A.T ? t0 + s : A.T - 1) * A.st[k] + dl);
-    }
-    const unsigned cut = RESET ? reset_bits<S>(A, b, t0) : 0u;
+    const int left = __builtin_amdgcn_readfirstlane(steps_left(A.T, t0, S));
+    const int64_t from = left ? t0 : A.T - 1;            // (a wave whole behind the end loads the last step)
+    const unsigned offset = (unsigned)dl * (unsigned)sizeof(T), cut = RESET ? reset_bits<S>(A, b, t0, left) : 0u;
     float k2[VEC], a[S][VEC], u[S][VEC], PA[VEC], PH[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-        k2[v] = -A.c * kLog2e * softplus(A.decay[dl + v]);
         PA[v] = 1.0f;
         PH[v] = 0.0f;
     }
+    const auto walk = [&](auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        Vec<T, VEC> raw[3][S];
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-        float x[VEC], r[VEC], i[VEC];
-        raw[0][s].get(x);
-        raw[1][s].get(r);
-        raw[2][s].get(i);
-        const bool there = t0 + s < A.T;                 // a step behind the end leaves the state as it is
+        for (int k = 0; k < 3; ++k) load_steps<WHOLE>((const T*)A.in[k] + b * A.sb[k] + from * A.st[k], A.st[k], left, offset, raw[k]);
+        load_k2<VEC>(A, dl, k2);
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const Gates g = gates(r[v], i[v], k2[v]);
-            a[s][v] = there ? g.a : 1.0f;
-            u[s][v] = there ? __builtin_amdgcn_sqrtf(g.m2) * g.si * x[v] : 0.0f;
-            if (RESET && (cut >> s & 1)) {
+        for (int s = 0; s < S; ++s) {
+            float x[VEC], r[VEC], i[VEC];
+            raw[0][s].get(x);
+            raw[1][s].get(r);
+            raw[2][s].get(i);
+            const bool there = WHOLE || s < left;        // a step behind the end leaves the state as it is
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const Gates g = gates(r[v], i[v], k2[v]);
+                a[s][v] = there ? g.a : 1.0f;
                 u[s][v] = g.si * x[v];
-                PA[v] = -0.0f;
-                PH[v] = u[s][v];
-            } else {
-                PA[v] *= a[s][v];
-                PH[v] = fmaf(a[s][v], PH[v], u[s][v]);
+                if (RESET && (cut >> s & 1)) {
+                    PA[v] = -0.0f;
+                    PH[v] = u[s][v];
+                } else {
+                    u[s][v] = there ? u[s][v] * __builtin_amdgcn_sqrtf(g.m2) : 0.0f;
+                    PA[v] *= a[s][v];
+                    PH[v] = fmaf(a[s][v], PH[v], u[s][v]);
+                }
             }
         }
-    }
+    };
+    if (left == S) walk(std::true_type());
+    else walk(std::false_type());
 #pragma unroll
     for (int v = 0; v < VEC; ++v) { sA[wave][lane * VEC + v] = PA[v]; sH[wave][lane * VEC + v] = PH[v]; }
     __syncthreads();
@@ -200,16 +243,16 @@ __global__ __launch_bounds__(W * 64) void k_scan_forward(ScanArgs A) {
     float now[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) now[v] = sA[wave][lane * VEC + v];
-    T* out = (T*)A.h + (b * A.T + t0) * A.D + d0;
+    if (!live) return;
+    T* out = (T*)A.h + (b * A.T + t0) * A.D;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
+        if (s >= left) continue;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) now[v] = RESET && (cut >> s & 1) ? u[s][v] : fmaf(a[s][v], now[v], u[s][v]);
-        if (live && t0 + s < A.T) {
-            Vec<T, VEC> o;
-            o.set(now);
-            o.store(out + (int64_t)s * A.D);
-        }
+        Vec<T, VEC> o;
+        o.set(now);
+        o.store(at_offset(out + (int64_t)s * A.D, (unsigned)d0 * (unsigned)sizeof(T)));
     }
 }
 
@@ -219,7 +262,7 @@ __global__ __launch_bounds__(W * 64) void k_scan_forward(ScanArgs A) {
 //   dx = g m s_i   di = g m x s_i (1 - s_i)   dla = g (a h_{t-1} - s_i x a^2 / m)   dr = dla la (1 - s_r)
 // For la -> 0 the product la a^2 / m goes to 0 (m ~ sqrt(-2 la)): where m is 0 that term is left out.
 template <class T, int VEC, int S, int W, bool RESET>
-__global__ __launch_bounds__(W * 64) void k_scan_backward(ScanArgs A) {
+__global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
     static_assert(S * W % kCheckpoint == 0, "a tile starts at a checkpoint");
     constexpr int NCH = 64 * VEC;
     __shared__ float sA[W][NCH], sH[W][NCH], sE[W][NCH];
@@ -232,56 +275,64 @@ __global__ __launch_bounds__(W * 64) void k_scan_backward(ScanArgs A) {
     const bool live = d0 < A.D;
     const int dl = live ? d0 : 0;
     const int64_t t0 = (int64_t)tile * (S * W) + wave * S;
-    Vec<T, VEC> raw[3][S], rawg[S];
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-        const int64_t t = t0 + s < A.T ? t0 + s : A.T - 1;
-#pragma unroll
-        for (int k = 0; k < 3; ++k) raw[k][s].load((const T*)A.in[k] + b * A.sb[k] + t * A.st[k] + dl);
-        if (A.dh) rawg[s].load((const T*)A.dh + (b * A.T + t) * A.D + dl);
-        else rawg[s].zero();
-    }
-    const unsigned cut = RESET ? reset_bits<S>(A, b, t0) : 0u;
-    float k2[VEC], a[S][VEC], m2[S][VEC], sr[S][VEC], si[S][VEC], PA[VEC], PH[VEC], PE[VEC];
+    const int left = __builtin_amdgcn_readfirstlane(steps_left(A.T, t0, S));
+    const int64_t from = left ? t0 : A.T - 1;
+    const unsigned offset = (unsigned)dl * (unsigned)sizeof(T), cut = RESET ? reset_bits<S>(A, b, t0, left) : 0u;
+    // kept for the second walk: x and dh as they came, a, the gates, m s_i, and s_i x a^2 / m
+    Vec<T, VEC> rawx[S], rawg[S];
+    float k2[VEC], a[S][VEC], sr[S][VEC], si[S][VEC], ms[S][VEC], pull[S][VEC], PA[VEC], PH[VEC], PE[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-        k2[v] = -A.c * kLog2e * softplus(A.decay[dl + v]);
         PA[v] = 1.0f;
         PH[v] = PE[v] = 0.0f;
     }
+    const auto walk = [&](auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        Vec<T, VEC> rawr[S], rawi[S];
+        load_steps<WHOLE>((const T*)A.in[1] + b * A.sb[1] + from * A.st[1], A.st[1], left, offset, rawr);
+        load_steps<WHOLE>((const T*)A.in[2] + b * A.sb[2] + from * A.st[2], A.st[2], left, offset, rawi);
+        load_steps<WHOLE>((const T*)A.in[0] + b * A.sb[0] + from * A.st[0], A.st[0], left, offset, rawx);
+        if (A.dh) load_steps<WHOLE>((const T*)A.dh + (b * A.T + from) * A.D, (int64_t)A.D, left, offset, rawg);
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-        float x[VEC], r[VEC], i[VEC];
-        raw[0][s].get(x);
-        raw[1][s].get(r);
-        raw[2][s].get(i);
-        const bool there = t0 + s < A.T;
+        for (int s = 0; s < S; ++s) if (!A.dh || !(WHOLE || s < left)) rawg[s].zero();
+        load_k2<VEC>(A, dl, k2);
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const Gates g = gates(r[v], i[v], k2[v]);
-            a[s][v] = there ? g.a : 1.0f;
-            m2[s][v] = there ? g.m2 : 0.0f;
-            sr[s][v] = g.sr;
-            si[s][v] = g.si;
-            const float u = there ? __builtin_amdgcn_sqrtf(g.m2) * g.si * x[v] : 0.0f;
-            if (RESET && (cut >> s & 1)) {
-                a[s][v] = 0.0f;
-                m2[s][v] = 1.0f;
-                PA[v] = -0.0f;
-                PH[v] = g.si * x[v];
-            } else {
-                PA[v] *= a[s][v];
-                PH[v] = fmaf(a[s][v], PH[v], u);
+        for (int s = 0; s < S; ++s) {
+            float x[VEC], r[VEC], i[VEC];
+            rawx[s].get(x);
+            rawr[s].get(r);
+            rawi[s].get(i);
+            const bool there = WHOLE || s < left;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const Gates g = gates(r[v], i[v], k2[v]);
+                sr[s][v] = there ? g.sr : 0.0f;
+                si[s][v] = g.si;
+                if (RESET && (cut >> s & 1)) {
+                    a[s][v] = 0.0f;
+                    ms[s][v] = g.si;
+                    pull[s][v] = 0.0f;
+                    PA[v] = -0.0f;
+                    PH[v] = g.si * x[v];
+                } else {
+                    const float inv = g.m2 == 0.0f ? 0.0f : __builtin_amdgcn_rsqf(g.m2);
+                    a[s][v] = there ? g.a : 1.0f;
+                    ms[s][v] = there ? g.m2 * inv * g.si : 0.0f;
+                    pull[s][v] = g.si * x[v] * (g.a * g.a * inv);
+                    PA[v] *= a[s][v];
+                    PH[v] = fmaf(a[s][v], PH[v], ms[s][v] * x[v]);
+                }
             }
         }
-    }
+    };
+    if (left == S) walk(std::true_type());
+    else walk(std::false_type());
 #pragma unroll
     for (int s = S - 1; s >= 0; --s) {
         float g[VEC];
         rawg[s].get(g);
 #pragma unroll
-        for (int v = 0; v < VEC; ++v)
-            PE[v] = RESET && (cut >> s & 1) ? 0.0f : t0 + s < A.T ? a[s][v] * (g[v] + PE[v]) : PE[v];
+        for (int v = 0; v < VEC; ++v) PE[v] = RESET && (cut >> s & 1) ? 0.0f : a[s][v] * (g[v] + PE[v]);
     }
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
@@ -319,7 +370,9 @@ __global__ __launch_bounds__(W * 64) void k_scan_backward(ScanArgs A) {
         }
     }
     __syncthreads();
-    float now[VEC], e[VEC], hp[S][VEC], sum[VEC];
+#pragma unroll
+    for (int s = 0; s < S; ++s) { rawx[s].forget(); rawg[s].forget(); }
+    float now[VEC], e[VEC], sum[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
         now[v] = sA[wave][lane * VEC + v];
@@ -329,39 +382,38 @@ __global__ __launch_bounds__(W * 64) void k_scan_backward(ScanArgs A) {
 #pragma unroll
     for (int s = 0; s < S; ++s) {
         float x[VEC];
-        raw[0][s].get(x);
+        rawx[s].get(x);
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            hp[s][v] = now[v];
-            const float u = __builtin_amdgcn_sqrtf(m2[s][v]) * si[s][v] * x[v];
-            now[v] = RESET && (cut >> s & 1) ? u : fmaf(a[s][v], now[v], u);
+            const bool reset = RESET && (cut >> s & 1);
+            const float u = ms[s][v] * x[v];
+            pull[s][v] = reset ? 0.0f : fmaf(a[s][v], now[v], -pull[s][v]);        // now: dla / g
+            now[v] = reset ? u : fmaf(a[s][v], now[v], u);
         }
     }
 #pragma unroll
     for (int s = S - 1; s >= 0; --s) {
         float x[VEC], g[VEC], dx[VEC], dr[VEC], di[VEC];
-        raw[0][s].get(x);
+        rawx[s].get(x);
         rawg[s].get(g);
-        const bool there = t0 + s < A.T;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            g[v] = (there ? g[v] : 0.0f) + e[v];
             const bool reset = RESET && (cut >> s & 1);
+            g[v] += e[v];
             e[v] = reset ? 0.0f : a[s][v] * g[v];
-            const float inv = m2[s][v] > 0.0f ? __builtin_amdgcn_rsqf(m2[s][v]) : 0.0f;
-            const float sx = si[s][v] * x[v], m = m2[s][v] * inv, gm = g[v] * m;
-            dx[v] = gm * si[s][v];
-            di[v] = gm * sx * (1.0f - si[s][v]);
-            const float dla = reset || !there ? 0.0f : g[v] * (a[s][v] * hp[s][v] - sx * (a[s][v] * a[s][v] * inv));
-            dr[v] = dla * (k2[v] * kLn2 * sr[s][v]) * (1.0f - sr[s][v]);
-            sum[v] += dla * sr[s][v];
+            dx[v] = g[v] * ms[s][v];
+            const float gu = dx[v] * x[v];
+            di[v] = fmaf(-gu, si[s][v], gu);
+            const float q = reset ? 0.0f : g[v] * pull[s][v] * sr[s][v];
+            dr[v] = q * (k2[v] * kLn2) * (1.0f - sr[s][v]);
+            sum[v] += q;
         }
-        if (live && there) {
-            const int64_t to = (b * A.T + t0 + s) * A.D + d0;
+        if (live && s < left) {
+            const int64_t to = (b * A.T + t0 + s) * A.D;
             Vec<T, VEC> o;
-            o.set(dx); o.store((T*)A.out[0] + to);
-            o.set(dr); o.store((T*)A.out[1] + to);
-            o.set(di); o.store((T*)A.out[2] + to);
+            o.set(dx); o.store(at_offset((T*)A.out[0] + to, offset));
+            o.set(dr); o.store(at_offset((T*)A.out[1] + to, offset));
+            o.set(di); o.store(at_offset((T*)A.out[2] + to, offset));
         }
     }
     // the tile's share of d decay: one row of `part`, summed over the waves (sH is free: its last reader is behind the barrier)
@@ -376,8 +428,11 @@ __global__ __launch_bounds__(W * 64) void k_scan_backward(ScanArgs A) {
         }
 }
 
-__global__ __launch_bounds__(256) void k_clear(Word* p, int64_t n) {
-    for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < n; k += (int64_t)gridDim.x * 256) p[k] = 0;
+// before a launch of more than one tile: the ticket and the words cleared, and the channels' k2 (softplus is more work than a step)
+__global__ __launch_bounds__(256) void k_prepare(Word* p, int64_t n, float* k2, const float* decay, int D, float c) {
+    const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)gridDim.x * 256;
+    for (int64_t k = first; k < n; k += all) p[k] = 0;
+    for (int64_t d = first; d < D; d += all) k2[d] = -c * kLog2e * softplus(decay[d]);
 }
 
 // d decay[d] = -c sigmoid(decay[d]) * (sum of column d of part[rows][D]): 64 columns and 16 strips of rows a workgroup, strips joined in a
@@ -387,6 +442,7 @@ __global__ __launch_bounds__(1024) void k_decay_grad(const float* part, const fl
     const int col = threadIdx.x & 63, s = threadIdx.x >> 6, d = blockIdx.x * 64 + col;
     float sum = 0.0f;
     if (d < D)
+#pragma unroll 8
         for (int64_t r = s; r < rows; r += 16) sum += part[r * D + d];
     strip[s][col] = sum;
     __syncthreads();
@@ -397,16 +453,17 @@ __global__ __launch_bounds__(1024) void k_decay_grad(const float* part, const fl
 }
 
 // Steps a wave and waves a workgroup of the two kernels.  Measured at 65537 steps x 1024 channels (forward) and 8 x 2047 x 2048 (both), bf16, us:
-// forward 16 x 8 141 / 83, 8 x 8 186 / 84, 8 x 16 181 / 104, 16 x 16 168 / 99, 4 x 16 271 / 139; backward 8 x 8 192, 8 x 16 201, 4 x 16 205,
-// 16 x 8 227, 16 x 4 221.  (One workgroup a channel block walking all steps by itself: 3650 / 157 and 273.)
+// forward 16 x 8 135 / 75, 8 x 8 155 / 73, 8 x 16 162 / 83, 16 x 4 149 / 81; backward 8 x 8 at 136 registers 171, held to 128 (two workgroups a
+// CU, for some twenty spilled registers) 142; 4 x 16 167, 8 x 16 180, 16 x 4 202.
 constexpr int kForwardSteps = 16, kForwardWaves = 8, kBackwardSteps = 8, kBackwardWaves = 8;
 int tile_of(bool backward) { return backward ? kBackwardSteps * kBackwardWaves : kForwardSteps * kForwardWaves; }
 int64_t tiles_of(const plmpm_scan* s, bool backward) { return (s->steps + tile_of(backward) - 1) / tile_of(backward); }
-// workspace: one word for the ticket, the words, and (backward) the rows of d decay's sums
+// workspace: one word for the ticket, the words, k2 (an even number of floats), and (backward) the rows of d decay's sums
 size_t word_bytes(const plmpm_scan* s, bool backward) {
     const int64_t tiles = tiles_of(s, backward);
     return tiles > 1 ? sizeof(Word) * (1 + (size_t)tiles * s->batch * s->width) : 0;
 }
+size_t k2_bytes(const plmpm_scan* s, bool backward) { return tiles_of(s, backward) > 1 ? round_up(s->width * sizeof(float), 8) : 0; }
 
 template <class T, int VEC, bool RESET> void launch(const ScanArgs& A, bool backward, hipStream_t st) {
     const int S = backward ? kBackwardSteps : kForwardSteps, W = backward ? kBackwardWaves : kForwardWaves;
@@ -421,11 +478,14 @@ template <class T, int VEC> void launch(const ScanArgs& A, bool backward, hipStr
     else launch<T, VEC, false>(A, backward, st);
 }
 template <class T> void launch(const ScanArgs& A, int vec, bool backward, hipStream_t st) {
-    if (vec == 2) launch<T, 2>(A, backward, st);
-    else launch<T, 1>(A, backward, st);
+    if constexpr (sizeof(T) == 2)
+        if (vec == 2) return launch<T, 2>(A, backward, st);
+    launch<T, 1>(A, backward, st);
 }
 
-// channels a lane: 2 where rows and pointers keep to it and a wave's 128 channels are not mostly behind the width
+// Channels a lane: 4 bytes' worth, so that a wave's rows are 256 bytes -- 2 channels of 16 bits where rows and pointers keep to it and at least half
+// of a wave's 128 channels are there, else 1.  (16 bits, 8 x 2047 x 2048, forward and backward: 2 channels 70 + 141 us, 1 channel 80 + 158, 4
+// channels 72 + 202; 32 bits, 16 x 50 x 256: 1 channel 7.2 + 9.0 us, 2 channels 8.1 + 11.9.)
 int vector_of(const plmpm_scan* s, bool backward) {
     const int size = dtype_size(s->dtype);
     int bytes = 16;
@@ -433,7 +493,7 @@ int vector_of(const plmpm_scan* s, bool backward) {
     for (int k = 0; k < 3; ++k) bytes = std::min(bytes, std::min(aligned_to(in[k], s->stride_b[k], size), aligned_to(in[k], s->stride_t[k], size)));
     if (backward) for (const void* p : {(const void*)s->dh, (const void*)s->dx, (const void*)s->dr, (const void*)s->di}) bytes = std::min(bytes, aligned_to(p, s->width, size));
     else bytes = std::min(bytes, aligned_to(s->h, s->width, size));
-    return s->width % 2 == 0 && s->width >= 128 && bytes >= 2 * size ? 2 : 1;
+    return size == 2 && s->width % 2 == 0 && s->width >= 64 && bytes >= 4 ? 2 : 1;
 }
 
 int check(const plmpm_scan* s, bool backward, bool pointers) {
@@ -474,12 +534,13 @@ int run(const plmpm_scan* s, bool backward, hipStream_t st) {
     A.cblks = (A.D + 64 * vec - 1) / (64 * vec);
     A.tiles = (int)tiles_of(s, backward);
     const size_t words = word_bytes(s, backward);
-    A.part = (float*)((char*)s->workspace + words);
+    A.part = (float*)((char*)s->workspace + words + k2_bytes(s, backward));
     if (words) {
         A.ticket = (unsigned*)s->workspace;
         A.words = (Word*)s->workspace + 1;
+        A.k2 = (float*)((char*)s->workspace + words);
         const int64_t n = (int64_t)(words / sizeof(Word)), groups = (n + 1023) / 1024;
-        hipLaunchKernelGGL(k_clear, dim3((unsigned)(groups < 2048 ? groups : 2048)), dim3(256), 0, st, (Word*)s->workspace, n);
+        hipLaunchKernelGGL(k_prepare, dim3((unsigned)(groups < 2048 ? groups : 2048)), dim3(256), 0, st, (Word*)s->workspace, n, A.k2, A.decay, A.D, A.c);
     }
     if (s->dtype == PLMPM_NN_F32) launch<float>(A, vec, backward, st);
     else if (s->dtype == PLMPM_NN_BF16) launch<bf16>(A, vec, backward, st);
@@ -497,7 +558,7 @@ extern "C" {
 int plmpm_scan_workspace(const plmpm_scan* s, int backward, size_t* bytes) {
     NN_REQUIRE(bytes, "scan: null argument");
     if (check(s, backward != 0, false)) return -1;
-    *bytes = word_bytes(s, backward != 0) + (backward ? (size_t)tiles_of(s, true) * s->batch * s->width * sizeof(float) : 0);
+    *bytes = word_bytes(s, backward != 0) + k2_bytes(s, backward != 0) + (backward ? (size_t)tiles_of(s, true) * s->batch * s->width * sizeof(float) : 0);
     return 0;
 }
 int plmpm_scan_forward(const plmpm_scan* s, void* hip_stream) { return run(s, false, (hipStream_t)hip_stream); }
