@@ -11,9 +11,7 @@ There is no CPU path.  The reference's counterpart is a per-step MLP (plb/engine
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
-import math
 
 import torch
 
@@ -31,75 +29,88 @@ def _library():
 
 
 def _site(t: torch.Tensor):
-    """-> (stream handle, device guard) of a call on ``t``'s GPU."""
-    if t.device.type != "cuda":
+    """-> (stream handle, device guard or None) of a call on ``t``'s GPU."""
+    index = t.get_device()
+    if index < 0:
         raise L.EngineError(f"policy operators run on a ROCm device, got a tensor on {t.device}: there is no CPU path")
-    guard = contextlib.nullcontext() if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
-    return torch.cuda.current_stream(t.device).cuda_stream, guard
+    return torch._C._cuda_getCurrentRawStream(index), None if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
 
 def _call(name, t, *args):
     stream, guard = _site(t)
     lib = _library()
-    with guard:
-        L.check(getattr(lib, name)(*args, C.c_void_p(stream)), lib)
+    if guard is None:
+        L.check(getattr(lib, name)(*args, stream), lib)
+    else:
+        with guard:
+            L.check(getattr(lib, name)(*args, stream), lib)
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _need(cond, message):
-    if not cond:
-        raise ValueError(message)
+def _refuse(message):
+    raise ValueError(message)
 
 
 def _same_device(first, **others):
+    where = first.get_device()
     for name, t in others.items():
         if t is not None:
-            _need(isinstance(t, torch.Tensor), f"{name} has to be a tensor")
-            _need(t.device == first.device, f"{name} is on {t.device}, not on {first.device}")
+            if not isinstance(t, torch.Tensor):
+                _refuse(f"{name} has to be a tensor")
+            if t.get_device() != where:
+                _refuse(f"{name} is on {t.device}, not on {first.device}")
+
+
+def _tracked(*ts):
+    """Whether autograd has to know of a call (without it the kernels are called directly: Function.apply costs more than they do)."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
 def _rows(t):
     """Unit stride over the last dimension (a copy if need be)."""
-    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
 # ---------------------------------------------------------------------------------------------- gated linear recurrence
 def _scan_args(x, r, i, decay, h0, reset, c):
     B, T, D = x.shape
-    s = L.Scan(dtype=DTYPES[x.dtype], batch=B, steps=T, width=D, c=c, x=_ptr(x), r=_ptr(r), i=_ptr(i), decay=_ptr(decay), h0=_ptr(h0), reset=_ptr(reset))
-    for k, t in enumerate((x, r, i)):
-        s.stride_b[k], s.stride_t[k] = t.stride(0), t.stride(1)
-    return s
+    (xb, xt, _), (rb, rt, _), (ib, it, _) = x.stride(), r.stride(), i.stride()
+    return L.Scan(DTYPES[x.dtype], 0, B, T, D, (xb, rb, ib), (xt, rt, it), c, x.data_ptr(), r.data_ptr(), i.data_ptr(), decay.data_ptr(), _ptr(h0), _ptr(reset))
 
 
 def _scan_run(name, s, x, backward):
     lib, need = _library(), C.c_size_t()
-    L.check(lib.plmpm_scan_workspace(C.byref(s), int(backward), C.byref(need)), lib)
-    work = torch.empty(need.value, dtype=torch.uint8, device=x.device) if need.value else None
-    s.workspace, s.workspace_bytes = _ptr(work), need.value
-    _call(name, x, C.byref(s))
+    L.check(lib.plmpm_scan_workspace(s, backward, need), lib)
+    if need.value:
+        work = torch.empty(need.value, dtype=torch.uint8, device=x.device)
+        s.workspace, s.workspace_bytes = work.data_ptr(), need.value
+    _call(name, x, s)
+
+
+def _scan_forward(x, r, i, decay, h0, reset, c, keep):
+    """-> h, last, checkpoint (what the backward pass starts from; None unless ``keep``)."""
+    B, T, D = x.shape
+    h = torch.empty((B, T, D), dtype=x.dtype, device=x.device)
+    last = torch.empty((B, D), dtype=torch.float32, device=x.device)
+    checkpoint = torch.empty(((T + CHECKPOINT - 1) // CHECKPOINT, B, D), dtype=torch.float32, device=x.device) if keep else None
+    if B and T and D:
+        s = _scan_args(x, r, i, decay, h0, reset, c)
+        s.h, s.h_last, s.checkpoint = h.data_ptr(), last.data_ptr(), _ptr(checkpoint)
+        _scan_run("plmpm_scan_forward", s, x, 0)
+    elif h0 is not None:
+        last.copy_(h0)
+    else:
+        last.zero_()
+    return h, last, checkpoint
 
 
 class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, r, i, decay, h0, reset, c):
-        x, r, i = _rows(x), _rows(r), _rows(i)
-        B, T, D = x.shape
-        h = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
-        last = torch.empty(B, D, dtype=torch.float32, device=x.device)
-        keep = any(ctx.needs_input_grad[:5])
-        checkpoint = torch.empty((T + CHECKPOINT - 1) // CHECKPOINT, B, D, dtype=torch.float32, device=x.device) if keep else None
-        if h.numel():
-            s = _scan_args(x, r, i, decay, h0, reset, c)
-            s.h, s.h_last, s.checkpoint = _ptr(h), _ptr(last), _ptr(checkpoint)
-            _scan_run("plmpm_scan_forward", s, x, False)
-        elif h0 is not None:
-            last.copy_(h0)
-        else:
-            last.zero_()
+        h, last, checkpoint = _scan_forward(x, r, i, decay, h0, reset, c, True)
         ctx.save_for_backward(x, r, i, decay, reset, checkpoint)
         ctx.c, ctx.has_h0 = c, h0 is not None
         ctx.set_materialize_grads(False)
@@ -110,16 +121,16 @@ class _GatedScan(torch.autograd.Function):
     def backward(ctx, dh, dlast):
         x, r, i, decay, reset, checkpoint = ctx.saved_tensors
         B, T, D = x.shape
-        dx, dr, di = (torch.empty(B, T, D, dtype=x.dtype, device=x.device) for _ in range(3))
+        dx, dr, di = (torch.empty((B, T, D), dtype=x.dtype, device=x.device) for _ in range(3))
         ddecay = torch.empty_like(decay)
-        dh0 = torch.empty(B, D, dtype=torch.float32, device=x.device) if ctx.has_h0 else None
+        dh0 = torch.empty((B, D), dtype=torch.float32, device=x.device) if ctx.has_h0 else None
         dh = None if dh is None else dh.contiguous()
         dlast = None if dlast is None else dlast.contiguous()
-        if dx.numel():
+        if B and T and D:
             s = _scan_args(x, r, i, decay, None, reset, ctx.c)
-            s.checkpoint, s.dh, s.dlast = _ptr(checkpoint), _ptr(dh), _ptr(dlast)
-            s.dx, s.dr, s.di, s.ddecay, s.dh0 = _ptr(dx), _ptr(dr), _ptr(di), _ptr(ddecay), _ptr(dh0)
-            _scan_run("plmpm_scan_backward", s, x, True)
+            s.checkpoint, s.dh, s.dlast = checkpoint.data_ptr(), _ptr(dh), _ptr(dlast)
+            s.dx, s.dr, s.di, s.ddecay, s.dh0 = dx.data_ptr(), dr.data_ptr(), di.data_ptr(), ddecay.data_ptr(), _ptr(dh0)
+            _scan_run("plmpm_scan_backward", s, x, 1)
         else:
             ddecay.zero_()
             if dh0 is not None:
@@ -128,14 +139,18 @@ class _GatedScan(torch.autograd.Function):
 
 
 def _scan_checks(x, r, i, decay, c, dims):
-    _need(isinstance(x, torch.Tensor) and x.dim() == dims, f"x has to be a tensor of {dims} dimensions")
+    if not isinstance(x, torch.Tensor) or x.dim() != dims:
+        _refuse(f"x has to be a tensor of {dims} dimensions")
     _same_device(x, r=r, i=i, decay=decay)
-    _need(x.dtype in DTYPES, f"x has to be float32, bfloat16 or float16, got {x.dtype}")
-    for name, t in (("r", r), ("i", i)):
-        _need(t.shape == x.shape and t.dtype == x.dtype, f"{name} has to match x: {tuple(x.shape)} {x.dtype}, got {tuple(t.shape)} {t.dtype}")
-    _need(decay.shape == x.shape[-1:] and decay.dtype == torch.float32 and decay.is_contiguous(),
-          f"decay has to be a contiguous float32 tensor of {x.shape[-1]} values")
-    _need(0.0 < c < 1e30, f"c has to be positive and finite, got {c}")
+    shape, dtype = x.shape, x.dtype
+    if dtype not in DTYPES:
+        _refuse(f"x has to be float32, bfloat16 or float16, got {dtype}")
+    if r.shape != shape or i.shape != shape or r.dtype != dtype or i.dtype != dtype:
+        _refuse(f"r and i have to match x: {tuple(shape)} {dtype}, got {tuple(r.shape)} {r.dtype} and {tuple(i.shape)} {i.dtype}")
+    if decay.shape != shape[-1:] or decay.dtype != torch.float32 or not decay.is_contiguous():
+        _refuse(f"decay has to be a contiguous float32 tensor of {shape[-1]} values")
+    if not 0.0 < c < 1e30:
+        _refuse(f"c has to be positive and finite, got {c}")
 
 
 def gated_scan(x, r, i, decay, h0=None, reset=None, *, c: float = 8.0):
@@ -151,14 +166,20 @@ def gated_scan(x, r, i, decay, h0=None, reset=None, *, c: float = 8.0):
     """
     _scan_checks(x, r, i, decay, c, 3)
     B, T, D = x.shape
-    _same_device(x, h0=h0, reset=reset)
     if h0 is not None:
-        _need(h0.shape == (B, D) and h0.dtype == torch.float32, f"h0 has to be float32 ({B}, {D}), got {tuple(h0.shape)} {h0.dtype}")
+        _same_device(x, h0=h0)
+        if h0.shape != (B, D) or h0.dtype != torch.float32:
+            _refuse(f"h0 has to be float32 ({B}, {D}), got {tuple(h0.shape)} {h0.dtype}")
         h0 = h0.contiguous()
     if reset is not None:
-        _need(reset.shape == (B, T) and reset.dtype == torch.bool, f"reset has to be bool ({B}, {T}), got {tuple(reset.shape)} {reset.dtype}")
+        _same_device(x, reset=reset)
+        if reset.shape != (B, T) or reset.dtype != torch.bool:
+            _refuse(f"reset has to be bool ({B}, {T}), got {tuple(reset.shape)} {reset.dtype}")
         reset = reset.contiguous()
-    return _GatedScan.apply(x, r, i, decay, h0, reset, float(c))
+    x, r, i = _rows(x), _rows(r), _rows(i)
+    if _tracked(x, r, i, decay, h0):
+        return _GatedScan.apply(x, r, i, decay, h0, reset, float(c))
+    return _scan_forward(x, r, i, decay, h0, reset, float(c), False)[:2]
 
 
 def gated_scan_step(x, r, i, decay, state, *, c: float = 8.0):
@@ -166,88 +187,90 @@ def gated_scan_step(x, r, i, decay, state, *, c: float = 8.0):
     evaluation; a differentiable step is ``gated_scan`` with T = 1)."""
     _scan_checks(x, r, i, decay, c, 2)
     _same_device(x, state=state)
-    _need(state is not None and state.shape == x.shape and state.dtype == torch.float32 and state.is_contiguous(),
-          f"state has to be a contiguous float32 tensor of {tuple(x.shape)}")
-    _need(not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, r, i, decay, state))),
-          "gated_scan_step has no gradients: call it under torch.no_grad(), or gated_scan with one step")
+    if state is None or state.shape != x.shape or state.dtype != torch.float32 or not state.is_contiguous():
+        _refuse(f"state has to be a contiguous float32 tensor of {tuple(x.shape)}")
+    if _tracked(x, r, i, decay, state):
+        _refuse("gated_scan_step has no gradients: call it under torch.no_grad(), or gated_scan with one step")
     x, r, i = _rows(x), _rows(r), _rows(i)
     B, D = x.shape
-    h = torch.empty(B, D, dtype=x.dtype, device=x.device)
-    if h.numel():
-        s = L.Scan(dtype=DTYPES[x.dtype], batch=B, steps=1, width=D, c=c, x=_ptr(x), r=_ptr(r), i=_ptr(i), decay=_ptr(decay), h0=_ptr(state), h=_ptr(h), h_last=_ptr(state))
-        for k, t in enumerate((x, r, i)):
-            s.stride_b[k] = t.stride(0)
-        _scan_run("plmpm_scan_forward", s, x, False)
+    h = torch.empty((B, D), dtype=x.dtype, device=x.device)
+    if B and D:
+        p = state.data_ptr()
+        s = L.Scan(DTYPES[x.dtype], 0, B, 1, D, (x.stride(0), r.stride(0), i.stride(0)), (0, 0, 0), c, x.data_ptr(), r.data_ptr(), i.data_ptr(), decay.data_ptr(), p, None,
+                   h.data_ptr(), p)
+        _call("plmpm_scan_forward", x, s)           # (a single step needs no workspace)
         torch.autograd.graph.increment_version(state)
     return h
 
 
 # ---------------------------------------------------------------------------------------------- norms around a block
 def _as_rows(t, D):
-    t = _rows(t.reshape(-1, D))
+    t = _rows(t) if t.dim() == 2 else _rows(t.reshape(-1, D))
     return t, (t.stride(0) if t.shape[0] > 1 else D)
 
 
 def _norm_args(x, u, gate, scale, post, pre, u_dtype, eps, fn, keep):
     D = x.shape[-1]
-    n = L.Norm(x_dtype=DTYPES[x.dtype], u_dtype=DTYPES[u_dtype], gate_fn=fn, width=D, eps=eps, scale=_ptr(scale), post=_ptr(post), pre=_ptr(pre))
-    n.w_dtype = next((DTYPES[w.dtype] for w in (pre, post, scale) if w is not None), 0)
-    for name, t in (("x", x), ("u", u), ("gate", gate)):
+    w = pre if pre is not None else post if post is not None else scale
+    at = [0, 0, 0]
+    strides = [0, 0, 0]
+    for k, t in enumerate((x, u, gate)):
         if t is not None:
-            t, stride = _as_rows(t, D)
+            t, strides[k] = _as_rows(t, D)
             keep.append(t)
-            setattr(n, name, _ptr(t))
-            setattr(n, "stride_" + name, stride)
-    n.rows = keep[0].shape[0]
-    return n
+            at[k] = t.data_ptr()
+    return L.Norm(DTYPES[x.dtype], DTYPES[u_dtype], 0 if w is None else DTYPES[w.dtype], fn, keep[0].shape[0], D, strides[0], strides[1], strides[2], 0, 0, eps,
+                  at[0], at[1], at[2], _ptr(scale), _ptr(post), _ptr(pre))
+
+
+def _norm_forward(x, u, gate, scale, post, pre, u_dtype, eps, fn):
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if u is not None else None
+    z = torch.empty(x.shape, dtype=u_dtype, device=x.device) if pre is not None else None
+    if x.numel():
+        keep = []
+        n = _norm_args(x, u, gate, scale, post, pre, u_dtype, eps, fn, keep)
+        n.y, n.z = _ptr(y), _ptr(z)
+        _call("plmpm_norm_forward", x, n)
+    return y, z
 
 
 class _BlockNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, u, gate, scale, post, pre, u_dtype, eps, fn):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if u is not None else None
-        z = torch.empty(x.shape, dtype=u_dtype, device=x.device) if pre is not None else None
-        if x.numel():
-            keep = []
-            n = _norm_args(x, u, gate, scale, post, pre, u_dtype, eps, fn, keep)
-            n.y, n.z = _ptr(y), _ptr(z)
-            _call("plmpm_norm_forward", x, C.byref(n))
         ctx.save_for_backward(x, u, gate, scale, post, pre)
         ctx.how = (u_dtype, eps, fn)
         ctx.set_materialize_grads(False)
-        return y, z
+        return _norm_forward(x, u, gate, scale, post, pre, u_dtype, eps, fn)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dz):
-        x, u, gate, scale, post, pre = ctx.saved_tensors
+        x, u, gate, scale, post, pre = saved = ctx.saved_tensors
         u_dtype, eps, fn = ctx.how
         if dy is None and dz is None:
             return (None,) * 9
         D = x.shape[-1]
-        keep, out = [], {}
-        for name, t in (("dx", x), ("du", u), ("dgate", gate), ("dscale", scale), ("dpost", post), ("dpre", pre)):
-            out[name] = None if t is None else torch.empty(t.shape, dtype=t.dtype, device=x.device)
+        out = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=x.device) for t in saved]
         if x.numel():
+            keep = []
             n = _norm_args(x, u, gate, scale, post, pre, u_dtype, eps, fn, keep)
-            for name, t in (("dy", dy), ("dz", dz)):
-                if t is not None:
-                    t, stride = _as_rows(t, D)
-                    keep.append(t)
-                    setattr(n, name, _ptr(t))
-                    setattr(n, "stride_" + name, stride)
-            for name, t in out.items():
-                setattr(n, name, _ptr(t))
+            if dy is not None:
+                dy, n.stride_dy = _as_rows(dy, D)
+                n.dy = dy.data_ptr()
+            if dz is not None:
+                dz, n.stride_dz = _as_rows(dz, D)
+                n.dz = dz.data_ptr()
+            n.dx, n.du, n.dgate, n.dscale, n.dpost, n.dpre = (_ptr(t) for t in out)
             lib, need = _library(), C.c_size_t()
-            L.check(lib.plmpm_norm_workspace(C.byref(n), C.byref(need)), lib)
+            L.check(lib.plmpm_norm_workspace(n, need), lib)
             work = torch.empty(need.value, dtype=torch.uint8, device=x.device)
-            n.workspace, n.workspace_bytes = _ptr(work), need.value
-            _call("plmpm_norm_backward", x, C.byref(n))
+            n.workspace, n.workspace_bytes = work.data_ptr(), need.value
+            _call("plmpm_norm_backward", x, n)
         else:
-            for name in ("dscale", "dpost", "dpre"):
-                if out[name] is not None:
-                    out[name].zero_()
-        return out["dx"], out["du"], out["dgate"], out["dscale"], out["dpost"], out["dpre"], None, None, None
+            for t in out[3:]:
+                if t is not None:
+                    t.zero_()
+        return (*out, None, None, None)
 
 
 def block_norm(x, u=None, gate=None, scale=None, post=None, pre=None, *, eps: float = 1e-6, gate_fn: str = "sigmoid", dtype=None):
@@ -262,26 +285,40 @@ def block_norm(x, u=None, gate=None, scale=None, post=None, pre=None, *, eps: fl
     the first block); without pre there is no z (None: behind the last).  z has u's type (without u: ``dtype``, x's by default) and comes
     from the unrounded y.  D is at most 8192.  Sums in float32; gradients reach every tensor given.
     """
-    _need(isinstance(x, torch.Tensor) and x.dim() >= 1, "x has to be a tensor with at least one dimension")
+    if not isinstance(x, torch.Tensor) or x.dim() < 1:
+        _refuse("x has to be a tensor with at least one dimension")
     _same_device(x, u=u, gate=gate, scale=scale, post=post, pre=pre)
-    _need(x.dtype in DTYPES, f"x has to be float32, bfloat16 or float16, got {x.dtype}")
+    if x.dtype not in DTYPES:
+        _refuse(f"x has to be float32, bfloat16 or float16, got {x.dtype}")
     D = x.shape[-1]
-    _need(D <= MAX_WIDTH, f"rows of {D} values, at most {MAX_WIDTH}")
-    _need(u is not None or pre is not None, "u, pre or both are needed")
-    _need(gate_fn in GATES, f"gate_fn has to be one of {sorted(GATES)}, got {gate_fn!r}")
-    _need(0.0 <= eps < 1e30, f"eps has to be zero or above, and finite, got {eps}")
+    if D > MAX_WIDTH:
+        _refuse(f"rows of {D} values, at most {MAX_WIDTH}")
+    if u is None and pre is None:
+        _refuse("u, pre or both are needed")
+    if gate_fn not in GATES:
+        _refuse(f"gate_fn has to be one of {sorted(GATES)}, got {gate_fn!r}")
+    if not 0.0 <= eps < 1e30:
+        _refuse(f"eps has to be zero or above, and finite, got {eps}")
     if u is None:
-        _need(gate is None and scale is None and post is None, "gate, scale and post go with u")
+        if gate is not None or scale is not None or post is not None:
+            _refuse("gate, scale and post go with u")
         u_dtype = x.dtype if dtype is None else dtype
     else:
         u_dtype = u.dtype
-        _need(dtype is None or dtype == u_dtype, f"z has u's type {u_dtype}: dtype is for calls without u")
-    _need(u_dtype in DTYPES and (u_dtype == x.dtype or x.dtype == torch.float32), f"u (or dtype) has to be x's type, or 16 bits next to a float32 x: got {u_dtype} with {x.dtype}")
-    for name, t in (("u", u), ("gate", gate)):
-        _need(t is None or (t.shape == x.shape and t.dtype == u_dtype), f"{name} has to have x's shape {tuple(x.shape)} and the type {u_dtype}")
-    weights = [(n, w) for n, w in (("scale", scale), ("post", post), ("pre", pre)) if w is not None]
-    for name, w in weights:
-        _need(w.shape == (D,) and w.is_contiguous() and w.dtype in DTYPES and w.dtype == weights[0][1].dtype,
-              f"{name} has to be a contiguous tensor of {D} values, of one floating type with the other weights")
-    y, z = _BlockNorm.apply(x, u, gate, scale, post, pre, u_dtype, float(eps), GATES[gate_fn])
+        if dtype is not None and dtype != u_dtype:
+            _refuse(f"z has u's type {u_dtype}: dtype is for calls without u")
+        if u.shape != x.shape:
+            _refuse(f"u has to have x's shape {tuple(x.shape)}, got {tuple(u.shape)}")
+    if u_dtype not in DTYPES or (u_dtype != x.dtype and x.dtype != torch.float32):
+        _refuse(f"u (or dtype) has to be x's type, or 16 bits next to a float32 x: got {u_dtype} with {x.dtype}")
+    if gate is not None and (gate.shape != x.shape or gate.dtype != u_dtype):
+        _refuse(f"gate has to have x's shape {tuple(x.shape)} and the type {u_dtype}, got {tuple(gate.shape)} {gate.dtype}")
+    w_dtype = None
+    for name, w in (("scale", scale), ("post", post), ("pre", pre)):
+        if w is not None:
+            w_dtype = w.dtype if w_dtype is None else w_dtype
+            if w.dim() != 1 or w.shape[0] != D or not w.is_contiguous() or w.dtype != w_dtype or w_dtype not in DTYPES:
+                _refuse(f"{name} has to be a contiguous tensor of {D} values, of one floating type with the other weights")
+    run = _BlockNorm.apply if _tracked(x, u, gate, scale, post, pre) else _norm_forward
+    y, z = run(x, u, gate, scale, post, pre, u_dtype, float(eps), GATES[gate_fn])
     return (x if u is None else y), z

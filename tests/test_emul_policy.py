@@ -28,10 +28,9 @@ def interpreter():
                            "HDRS=" + " ".join(os.path.join("../../plasticinelab_amd/csrc", h) for h in ("plmpm_nn.h", "plmpm_kernels.h")) + " ../../include/plmpm_policy.h",
                            "SRCS=" + SOURCES, out])
     lib = _lib.bind(C.CDLL(os.path.join(HERE, out)), {**_lib.POLICY_SYMBOLS, "plmpm_last_error": _lib.SYMBOLS["plmpm_last_error"]})
-    import contextlib
     patch = pytest.MonkeyPatch()
     patch.setattr(P, "_library", lambda: lib)
-    patch.setattr(P, "_site", lambda t: (0, contextlib.nullcontext()))
+    patch.setattr(P, "_site", lambda t: (0, None))
     yield "cpu"
     patch.undo()
 
