@@ -83,17 +83,16 @@ template <class T, int N> struct Vec {
         for (int k = 0; k < parts; ++k) reinterpret_cast<W*>(p)[k] = w[k];
     }
     __device__ __forceinline__ void zero() { memset(w, 0, sizeof(w)); }
-    // unpack again from here on (16-bit elements: the compiler would keep the floats, twice the registers, from an earlier get)
+    // unpack from here on (else the compiler keeps the floats of an earlier or a later get, twice the registers where elements have 16 bits)
     __device__ __forceinline__ void forget() {
 #if !defined(PLB_HOST_EMUL)
-        if (sizeof(T) == 2 && part == 4)
+        if constexpr (bytes % 4 == 0) {
+            uint32_t u[bytes / 4];
+            memcpy(u, w, bytes);
 #pragma unroll
-            for (int k = 0; k < parts; ++k) {
-                uint32_t u;
-                memcpy(&u, &w[k], 4);
-                asm("" : "+v"(u));
-                memcpy(&w[k], &u, 4);
-            }
+            for (int k = 0; k < bytes / 4; ++k) asm("" : "+v"(u[k]));
+            memcpy(w, u, bytes);
+        }
 #endif
     }
     __device__ __forceinline__ void get(float* f) const {
@@ -110,10 +109,45 @@ template <class T, int N> struct Vec {
     }
 };
 
-__device__ __forceinline__ float wave_sum(float v) {
+// a row's address, the same for the whole wave, plus a lane's 32-bit offset: the empty asm keeps the row's address in scalar registers (the compiler
+// would otherwise add row and offset once a lane in 64 bits, and hold two vector registers for each of the loads in flight)
+template <class T> __device__ __forceinline__ T* at_offset(T* row, unsigned bytes) {
+#if defined(PLB_HOST_EMUL)
+    return (T*)((char*)row + bytes);
+#else
+    typedef char __attribute__((address_space(1))) * Global;
+    const uint64_t r = (uint64_t)row;
+    unsigned lo = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)r), hi = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(r >> 32));
+    uint64_t u = ((uint64_t)hi << 32) | lo;
+    asm("" : "+s"(u));
+    return (T*)(char*)((Global)u + bytes);
+#endif
+}
+
+// sums over groups of n neighbouring lanes (n a power of two up to 64, the same for the wave), every lane gets its group's: steps within 16 lanes
+// are DPP moves (a lane's partner in its pair, its four, its eight, its sixteen), the two above go through LDS crossbar shuffles
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    return as_f((uint32_t)__builtin_amdgcn_update_dpp(0, (int)as_u(v), CTRL, 0xf, 0xf, true));
+}
+template <int K> __device__ __forceinline__ void lane_sums(float (&v)[K], int n) {
+    if (n >= 2)
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
-    return v;
+        for (int k = 0; k < K; ++k) v[k] += dpp<0xB1>(v[k]);           // quad_perm 1 0 3 2
+    if (n >= 4)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] += dpp<0x4E>(v[k]);           // quad_perm 2 3 0 1
+    if (n >= 8)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] += dpp<0x141>(v[k]);          // row_half_mirror
+    if (n >= 16)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] += dpp<0x140>(v[k]);          // row_mirror
+    if (n >= 32)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] += __shfl_xor(v[k], 16);
+    if (n >= 64)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] += __shfl_xor(v[k], 32);
 }
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll

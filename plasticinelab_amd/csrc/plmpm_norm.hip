@@ -22,7 +22,7 @@ namespace {
 constexpr int kCols = 8;                // columns a thread
 constexpr int kMaxRowThreads = 1024;
 constexpr int kMaxWidth = kCols * kMaxRowThreads;
-constexpr int kMaxBlocks = 512;         // workgroups of a backward launch: one partial row of column sums each
+constexpr int kForwardBlocks = 1024;
 
 struct NormArgs {
     const void *x, *u, *gate, *scale, *post, *pre, *dy, *dz;
@@ -33,147 +33,217 @@ struct NormArgs {
     float eps;
 };
 
-// sum over the `tpr` (a power of two) neighbouring threads that hold a row; `lds`: one float a wave, another buffer for each sum of a row
-__device__ __forceinline__ float row_sum(float v, int tpr, float* lds) {
-    const int top = tpr < 64 ? tpr : 64;
-    for (int m = 1; m < top; m <<= 1) v += __shfl_xor(v, m);
-    if (tpr <= 64) return v;
-    const int wave = threadIdx.x >> 6, per = tpr >> 6, first = wave & ~(per - 1);
-    if ((threadIdx.x & 63) == 0) lds[wave] = v;
+// K sums over the `tpr` (a power of two) neighbouring threads that hold a row, in one exchange; `lds`: K floats a wave, another buffer for each
+// exchange of a row
+template <int K> __device__ __forceinline__ void row_sums(float (&v)[K], int tpr, float (*lds)[K]) {
+    lane_sums<K>(v, tpr < 64 ? tpr : 64);
+    if (tpr <= 64) return;
+    const int wave = threadIdx.x >> 6, per = tpr >> 6, from = (wave & ~(per - 1)) + (int)(threadIdx.x & (per - 1));
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int k = 0; k < K; ++k) lds[wave][k] = v[k];
     __syncthreads();
-    v = 0.0f;
-    for (int w = 0; w < per; ++w) v += lds[first + w];
-    return v;
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = lds[from][k];
+    lane_sums<K>(v, per);
 }
 
-__device__ __forceinline__ void gate_of(int fn, float g, float& f, float& df) {
-    if (fn == PLMPM_GATE_IDENTITY) { f = g; df = 1.0f; return; }
-    const float s = sigmoid_fast(g);
-    if (fn == PLMPM_GATE_SIGMOID) { f = s; df = s * (1.0f - s); }
-    else { f = g * s; df = s * fmaf(g, 1.0f - s, 1.0f); }
+// f(g) in place of g, and its derivative (one question a row, not one an element)
+__device__ __forceinline__ void gates_of(int fn, float (&g)[kCols], float (&df)[kCols]) {
+    if (fn == PLMPM_GATE_IDENTITY) {
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) df[k] = 1.0f;
+    } else if (fn == PLMPM_GATE_SIGMOID) {
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) { g[k] = sigmoid_fast(g[k]); df[k] = g[k] * (1.0f - g[k]); }
+    } else {
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) { const float s = sigmoid_fast(g[k]); df[k] = s * fmaf(g[k], 1.0f - s, 1.0f); g[k] *= s; }
+    }
+}
+__device__ __forceinline__ void gates_of(int fn, float (&g)[kCols]) {
+    if (fn == PLMPM_GATE_IDENTITY) return;
+    if (fn == PLMPM_GATE_SIGMOID) {
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) g[k] = sigmoid_fast(g[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) g[k] *= sigmoid_fast(g[k]);
+    }
+}
+// no gate counts as ones
+__device__ __forceinline__ void open_gates(float (&g)[kCols]) {
+#pragma unroll
+    for (int k = 0; k < kCols; ++k) g[k] = 1.0f;
 }
 
 // column of element k of piece j: pieces of VW neighbouring columns, TPR pieces apart
 template <int VW> __device__ __forceinline__ int column(int tpr, int j) { return (j * tpr + (int)(threadIdx.x & (tpr - 1))) * VW; }
 
-template <int VW> __device__ __forceinline__ void load_weight(const void* w, int dtype, int D, int tpr, float* out) {
+// where a piece is read: pieces behind the width read the last one again (no condition around a load)
+template <int VW, bool EVEN> __device__ __forceinline__ int place(int D, int tpr, int j) {
+    const int c = column<VW>(tpr, j);
+    return EVEN || c < D ? c : D - VW;
+}
+// sum over a thread's columns that are there, of term(k)
+template <int VW, bool EVEN, class F> __device__ __forceinline__ float sum_columns(int D, int tpr, F term) {
+    float s = 0.0f;
 #pragma unroll
     for (int j = 0; j < kCols / VW; ++j) {
-        const int c = column<VW>(tpr, j);
+        float p = 0.0f;
 #pragma unroll
-        for (int k = 0; k < VW; ++k) out[j * VW + k] = w ? 0.0f : 1.0f;
-        if (!w || c >= D) continue;
+        for (int k = j * VW; k < (j + 1) * VW; ++k) p = term(k, p);
+        s += EVEN || column<VW>(tpr, j) < D ? p : 0.0f;
+    }
+    return s;
+}
+
+template <int VW, bool ALL, bool EVEN> __device__ __forceinline__ void load_weight(const void* w, int dtype, int D, int tpr, float* out) {
+#pragma unroll
+    for (int j = 0; j < kCols / VW; ++j) {
+        const int c = place<VW, EVEN>(D, tpr, j);
+#pragma unroll
+        for (int k = 0; k < VW; ++k) out[j * VW + k] = 1.0f;
+        if (!ALL && !w) continue;
         if (dtype == PLMPM_NN_F32) { Vec<float, VW> v; v.load((const float*)w + c); v.get(out + j * VW); }
         else if (dtype == PLMPM_NN_BF16) { Vec<bf16, VW> v; v.load((const bf16*)w + c); v.get(out + j * VW); }
         else { Vec<f16, VW> v; v.load((const f16*)w + c); v.get(out + j * VW); }
     }
 }
-template <class T, int VW> __device__ __forceinline__ void load_row(const void* p, int64_t row, int64_t stride, int D, int tpr, float* out) {
+// a thread's columns of a row, all loads before the first use
+template <class T, int VW, bool ALL, bool EVEN> struct Row {
+    Vec<T, VW> v[kCols / VW];
+    // row `base` is the workgroup's, `mine` rows behind it this thread's (the host sees to it that the offset fits 32 bits)
+    __device__ __forceinline__ void load(const void* p, int64_t base, int mine, int64_t stride, int D, int tpr) {
+        T* row = (T*)p + base * stride;
+        const unsigned ahead = (unsigned)mine * (unsigned)stride;
 #pragma unroll
-    for (int j = 0; j < kCols / VW; ++j) {
-        const int c = column<VW>(tpr, j);
-        Vec<T, VW> v;
-        if (p && c < D) v.load((const T*)p + row * stride + c);
-        else v.zero();
-        v.get(out + j * VW);
+        for (int j = 0; j < kCols / VW; ++j) {
+            if (ALL || p) v[j].load(at_offset(row, (ahead + (unsigned)place<VW, EVEN>(D, tpr, j)) * (unsigned)sizeof(T)));
+            else v[j].zero();
+        }
     }
-}
-template <class T, int VW> __device__ __forceinline__ void store_row(void* p, int64_t row, int D, int tpr, const float* in) {
+    // unpacked where it is used, each time: in between only the elements as they came are held
+    __device__ __forceinline__ void get(float* out) {
+#pragma unroll
+        for (int j = 0; j < kCols / VW; ++j) {
+            v[j].forget();
+            v[j].get(out + j * VW);
+        }
+    }
+};
+template <class T, int VW, bool EVEN> __device__ __forceinline__ void store_row(void* p, int64_t base, int mine, int D, int tpr, const float* in) {
+    T* row = (T*)p + base * D;
 #pragma unroll
     for (int j = 0; j < kCols / VW; ++j) {
         const int c = column<VW>(tpr, j);
-        if (c >= D) continue;
+        if (!EVEN && c >= D) continue;
         Vec<T, VW> v;
         v.set(in + j * VW);
-        v.store((T*)p + row * D + c);
+        v.store(at_offset(row, ((unsigned)mine * (unsigned)D + (unsigned)c) * (unsigned)sizeof(T)));
     }
 }
 
-template <class TX, class TU, int VW>
+// ALL: every tensor is there; EVEN: the width is what the threads hold (TPR x 8) and the rows come out even.  A condition around a load keeps the
+// compiler from counting what is in flight (it then waits for everything) and holds registers: with conditions 8192 x 4096 backward
+// took 220 us, without 157.
+template <class TX, class TU, int VW, bool ALL, bool EVEN>
 __global__ __launch_bounds__(1024) void k_norm_forward(NormArgs A) {
-    __shared__ float lds[2][16];
+    __shared__ float lds[2][16][1];
     const int tpr = A.tpr, group = threadIdx.x / tpr, groups = blockDim.x / tpr;
+    const int64_t step = (int64_t)gridDim.x * groups;
     const float inv = 1.0f / (float)A.D;
     float scale[kCols], post[kCols], pre[kCols];
-    load_weight<VW>(A.scale, A.wt, A.D, tpr, scale);
-    load_weight<VW>(A.post, A.wt, A.D, tpr, post);
-    load_weight<VW>(A.pre, A.wt, A.D, tpr, pre);
-    for (int64_t base = (int64_t)blockIdx.x * groups; base < A.rows; base += (int64_t)gridDim.x * groups) {
-        const bool there = base + group < A.rows;              // every thread takes part in the sums
-        const int64_t row = there ? base + group : A.rows - 1;
+    load_weight<VW, ALL, EVEN>(A.scale, A.wt, A.D, tpr, scale);
+    load_weight<VW, ALL, EVEN>(A.post, A.wt, A.D, tpr, post);
+    load_weight<VW, ALL, EVEN>(A.pre, A.wt, A.D, tpr, pre);
+    Row<TX, VW, ALL, EVEN> rx;
+    Row<TU, VW, ALL, EVEN> ru, rg;
+    const auto fetch = [&](int64_t base) {
+        const int mine = EVEN || base + group < A.rows ? group : (int)(A.rows - 1 - base);
+        rx.load(A.x, base, mine, A.sx, A.D, tpr);
+        ru.load(A.u, base, mine, A.su, A.D, tpr);
+        rg.load(A.gate, base, mine, A.sg, A.D, tpr);
+    };
+    for (int64_t base = (int64_t)blockIdx.x * groups; base < A.rows; base += step) {
+        const bool there = EVEN || base + group < A.rows;              // every thread takes part in the sums
         float y[kCols], u[kCols], g[kCols];
-        load_row<TX, VW>(A.x, row, A.sx, A.D, tpr, y);
-        if (A.u) {
-            load_row<TU, VW>(A.u, row, A.su, A.D, tpr, u);
-            load_row<TU, VW>(A.gate, row, A.sg, A.D, tpr, g);
-            float s = 0.0f;
+        fetch(base);
+        rx.get(y);
+        ru.get(u);
+        rg.get(g);
+        if (ALL || A.u) {
+            float s[1] = {sum_columns<VW, EVEN>(A.D, tpr, [&](int k, float p) { return fmaf(u[k], u[k], p); })};
+            row_sums<1>(s, tpr, lds[0]);
+            const float r = __builtin_amdgcn_rsqf(fmaf(s[0], inv, A.eps));
+            if (ALL || A.gate) gates_of(A.fn, g);
+            else open_gates(g);
 #pragma unroll
-            for (int k = 0; k < kCols; ++k) s = fmaf(u[k], u[k], s);
-            const float ru = __builtin_amdgcn_rsqf(fmaf(row_sum(s, tpr, lds[0]), inv, A.eps));
-#pragma unroll
-            for (int k = 0; k < kCols; ++k) {
-                float f = 1.0f, df;
-                if (A.gate) gate_of(A.fn, g[k], f, df);
-                y[k] = fmaf(scale[k] * f, post[k] * (u[k] * ru), y[k]);
-            }
-            if (there) store_row<TX, VW>(A.y, row, A.D, tpr, y);
+            for (int k = 0; k < kCols; ++k) y[k] = fmaf(scale[k] * g[k], post[k] * (u[k] * r), y[k]);
+            if (there) store_row<TX, VW, EVEN>(A.y, base, group, A.D, tpr, y);
         }
-        if (A.z) {
-            float s = 0.0f;
+        if (ALL || A.z) {
+            float s[1] = {sum_columns<VW, EVEN>(A.D, tpr, [&](int k, float p) { return fmaf(y[k], y[k], p); })};
+            row_sums<1>(s, tpr, lds[1]);
+            const float r = __builtin_amdgcn_rsqf(fmaf(s[0], inv, A.eps));
 #pragma unroll
-            for (int k = 0; k < kCols; ++k) s = fmaf(y[k], y[k], s);
-            const float ry = __builtin_amdgcn_rsqf(fmaf(row_sum(s, tpr, lds[1]), inv, A.eps));
-#pragma unroll
-            for (int k = 0; k < kCols; ++k) y[k] = pre[k] * (y[k] * ry);
-            if (there) store_row<TU, VW>(A.z, row, A.D, tpr, y);
+            for (int k = 0; k < kCols; ++k) y[k] = pre[k] * (y[k] * r);
+            if (there) store_row<TU, VW, EVEN>(A.z, base, group, A.D, tpr, y);
         }
-        if (tpr > 64 && !(A.u && A.z)) __syncthreads();        // with one sum a row its buffer is written again at once; with two, the other's barrier lies between
+        if (!ALL && tpr > 64 && !(A.u && A.z)) __syncthreads();        // with one exchange a row its buffer is written again at once; with two, the other's barrier lies between
     }
 }
 
-template <class TX, class TU, int VW>
-__global__ __launch_bounds__(1024) void k_norm_backward(NormArgs A) {
-    __shared__ float lds[4][16], fold[kCols * 256];
+template <class TX, class TU, int VW, int THREADS, bool ALL, bool EVEN>
+__global__ __launch_bounds__(THREADS) void k_norm_backward(NormArgs A) {
+    __shared__ float lds[2][16][1], lds2[16][2], fold[kCols * 256];
     const int tpr = A.tpr, group = threadIdx.x / tpr, groups = blockDim.x / tpr;
+    const int64_t step = (int64_t)gridDim.x * groups;
     const float inv = 1.0f / (float)A.D;
     float scale[kCols], post[kCols], pre[kCols], sums[3][kCols];
-    load_weight<VW>(A.scale, A.wt, A.D, tpr, scale);
-    load_weight<VW>(A.post, A.wt, A.D, tpr, post);
-    load_weight<VW>(A.pre, A.wt, A.D, tpr, pre);
+    load_weight<VW, ALL, EVEN>(A.scale, A.wt, A.D, tpr, scale);
+    load_weight<VW, ALL, EVEN>(A.post, A.wt, A.D, tpr, post);
+    load_weight<VW, ALL, EVEN>(A.pre, A.wt, A.D, tpr, pre);
 #pragma unroll
     for (int k = 0; k < kCols; ++k) sums[0][k] = sums[1][k] = sums[2][k] = 0.0f;
-    for (int64_t base = (int64_t)blockIdx.x * groups; base < A.rows; base += (int64_t)gridDim.x * groups) {
-        const bool there = base + group < A.rows;
-        const int64_t row = there ? base + group : A.rows - 1;
-        float y[kCols], uh[kCols], g[kCols], dy[kCols], dz[kCols], f[kCols], df[kCols], ru = 0.0f;
-        load_row<TX, VW>(A.x, row, A.sx, A.D, tpr, y);
-        load_row<TU, VW>(A.u, row, A.su, A.D, tpr, uh);
-        load_row<TU, VW>(A.gate, row, A.sg, A.D, tpr, g);
-        load_row<TX, VW>(A.dy, row, A.sdy, A.D, tpr, dy);
-        load_row<TU, VW>(A.dz, row, A.sdz, A.D, tpr, dz);
-        if (A.u) {
-            float s = 0.0f;
+    Row<TX, VW, ALL, EVEN> rx, rdy;
+    Row<TU, VW, ALL, EVEN> ru, rg, rdz;
+    const auto fetch = [&](int64_t base) {
+        const int mine = EVEN || base + group < A.rows ? group : (int)(A.rows - 1 - base);
+        rx.load(A.x, base, mine, A.sx, A.D, tpr);
+        ru.load(A.u, base, mine, A.su, A.D, tpr);
+        rg.load(A.gate, base, mine, A.sg, A.D, tpr);
+        rdy.load(A.dy, base, mine, A.sdy, A.D, tpr);
+        rdz.load(A.dz, base, mine, A.sdz, A.D, tpr);
+    };
+    for (int64_t base = (int64_t)blockIdx.x * groups; base < A.rows; base += step) {
+        const bool there = EVEN || base + group < A.rows;
+        float y[kCols], dy[kCols], r = 0.0f;
+        fetch(base);
+        rx.get(y);
+        if (ALL || A.u) {
+            float u[kCols], g[kCols];
+            ru.get(u);
+            float s[1] = {sum_columns<VW, EVEN>(A.D, tpr, [&](int k, float p) { return fmaf(u[k], u[k], p); })};
+            row_sums<1>(s, tpr, lds[0]);
+            r = __builtin_amdgcn_rsqf(fmaf(s[0], inv, A.eps));
+            ru.get(u);
+            rg.get(g);
+            if (ALL || A.gate) gates_of(A.fn, g);
+            else open_gates(g);
 #pragma unroll
-            for (int k = 0; k < kCols; ++k) s = fmaf(uh[k], uh[k], s);
-            ru = __builtin_amdgcn_rsqf(fmaf(row_sum(s, tpr, lds[0]), inv, A.eps));
-#pragma unroll
-            for (int k = 0; k < kCols; ++k) {
-                uh[k] *= ru;
-                f[k] = 1.0f;
-                df[k] = 0.0f;
-                if (A.gate) gate_of(A.fn, g[k], f[k], df[k]);
-                y[k] = fmaf(scale[k] * f[k], post[k] * uh[k], y[k]);
-            }
+            for (int k = 0; k < kCols; ++k) y[k] = fmaf(scale[k] * g[k], post[k] * (u[k] * r), y[k]);
         }
-        if (A.dz) {
-            float s = 0.0f, t = 0.0f;
-#pragma unroll
-            for (int k = 0; k < kCols; ++k) {
-                s = fmaf(y[k], y[k], s);
-                t = fmaf(dz[k] * pre[k], y[k], t);
-            }
-            const float ry = __builtin_amdgcn_rsqf(fmaf(row_sum(s, tpr, lds[1]), inv, A.eps));
-            const float mean = row_sum(t, tpr, lds[2]) * inv * ry;
+        rdy.get(dy);
+        if (ALL || A.dz) {
+            float dz[kCols];
+            rdz.get(dz);
+            float s[2] = {sum_columns<VW, EVEN>(A.D, tpr, [&](int k, float p) { return fmaf(y[k], y[k], p); }),
+                          sum_columns<VW, EVEN>(A.D, tpr, [&](int k, float p) { return fmaf(dz[k] * pre[k], y[k], p); })};
+            row_sums<2>(s, tpr, lds2);
+            const float ry = __builtin_amdgcn_rsqf(fmaf(s[0], inv, A.eps)), mean = s[1] * inv * ry;
+            rdz.get(dz);
+            rdy.get(dy);
 #pragma unroll
             for (int k = 0; k < kCols; ++k) {
                 const float yh = y[k] * ry;
@@ -181,29 +251,32 @@ __global__ __launch_bounds__(1024) void k_norm_backward(NormArgs A) {
                 dy[k] = fmaf(ry, fmaf(-yh, mean, dz[k] * pre[k]), dy[k]);
             }
         }
-        if (there) store_row<TX, VW>(A.dx, row, A.D, tpr, dy);
-        if (A.u) {
-            float w[kCols], s = 0.0f;
+        if (there) store_row<TX, VW, EVEN>(A.dx, base, group, A.D, tpr, dy);
+        if (ALL || A.u) {
+            float u[kCols], g[kCols], df[kCols];
+            ru.get(u);
+            rg.get(g);
+            if (ALL || A.gate) gates_of(A.fn, g, df);
+            else open_gates(g);
 #pragma unroll
             for (int k = 0; k < kCols; ++k) {
-                w[k] = dy[k] * scale[k] * f[k];
-                const float vh = post[k] * uh[k];
+                const float uh = u[k] * r, t = dy[k] * scale[k], w = t * g[k], vh = post[k] * uh;
                 if (there) {
-                    sums[0][k] = fmaf(dy[k] * f[k], vh, sums[0][k]);
-                    sums[1][k] = fmaf(w[k], uh[k], sums[1][k]);
+                    sums[0][k] = fmaf(dy[k] * g[k], vh, sums[0][k]);
+                    sums[1][k] = fmaf(w, uh, sums[1][k]);
                 }
-                g[k] = dy[k] * scale[k] * vh * df[k];
-                w[k] *= post[k];
-                s = fmaf(w[k], uh[k], s);
+                if (ALL || A.gate) g[k] = t * vh * df[k];
+                dy[k] = w * post[k];
             }
-            const float mean = row_sum(s, tpr, lds[3]) * inv;
+            float s[1] = {sum_columns<VW, EVEN>(A.D, tpr, [&](int k, float p) { return fmaf(dy[k], u[k] * r, p); })};
+            if ((ALL || A.gate) && there) store_row<TU, VW, EVEN>(A.dgate, base, group, A.D, tpr, g);
+            row_sums<1>(s, tpr, lds[1]);
+            const float mean = s[0] * inv;
+            ru.get(u);
 #pragma unroll
-            for (int k = 0; k < kCols; ++k) w[k] = ru * fmaf(-uh[k], mean, w[k]);
-            if (there) {
-                store_row<TU, VW>(A.du, row, A.D, tpr, w);
-                if (A.gate) store_row<TU, VW>(A.dgate, row, A.D, tpr, g);
-            }
-        } else if (tpr > 64) __syncthreads();                  // the two sums of this row share one barrier's worth of distance to the next row's
+            for (int k = 0; k < kCols; ++k) u[k] = r * fmaf(-(u[k] * r), mean, dy[k]);
+            if (there) store_row<TU, VW, EVEN>(A.du, base, group, A.D, tpr, u);
+        } else if (tpr > 64) __syncthreads();                  // (without u a row has one exchange: its buffer is free again behind this)
     }
     // a workgroup's column sums: rows side by side in it are folded through LDS first
     for (int n = 0; n < 3; ++n) {
@@ -238,6 +311,7 @@ __global__ __launch_bounds__(1024) void k_column_sums(const float* part, int blo
     if (!out) return;
     float sum = 0.0f;
     if (d < D)
+#pragma unroll 8
         for (int r = s; r < blocks; r += 16) sum += part[((int64_t)r * 3 + n) * D + d];
     strip[s][col] = sum;
     __syncthreads();
@@ -254,10 +328,13 @@ int row_threads(int64_t width) {
     return tpr;
 }
 int block_of(int tpr) { return tpr > 256 ? tpr : 256; }
-int blocks_of(const plmpm_norm* n) {
+int blocks_of(const plmpm_norm* n, bool backward) {
     const int groups = block_of(row_threads(n->width)) / row_threads(n->width);
     const int64_t need = (n->rows + groups - 1) / groups;
-    return (int)std::min<int64_t>(need, kMaxBlocks);
+    // backward: as many as run at once (each leaves a partial row of column sums), one a CU of 512 threads or more, two of 256: 8192 x 4096 157 us
+    // with 256 workgroups, 165 with 512; 2999 x 1214 29 us with 512, 41 with 256 (27 with 768, whose sums then take 2 us more)
+    const int most = !backward ? kForwardBlocks : groups == 1 && row_threads(n->width) >= 512 ? 256 : 512;
+    return (int)std::min<int64_t>(need, most);
 }
 
 int check(const plmpm_norm* n, bool backward) {
@@ -272,6 +349,9 @@ int check(const plmpm_norm* n, bool backward) {
     if (!n->rows || !n->width) return 0;
     NN_REQUIRE(n->x, "norm: x is needed");
     NN_REQUIRE(n->u || (!n->gate && !n->scale && !n->post), "norm: gate, scale and post go with u");
+    const int groups = block_of(row_threads(n->width)) / row_threads(n->width);
+    for (int64_t stride : {n->stride_x, n->stride_u, n->stride_gate, n->stride_dy, n->stride_dz})
+        NN_REQUIRE(stride >= 0 && (groups == 1 || stride < ((int64_t)1 << 29) / groups), "norm: a row stride of %lld is negative, or too large for rows of %lld", (long long)stride, (long long)n->width);
     if (backward) {
         NN_REQUIRE(n->dx && (!n->u || n->du) && (!n->gate || n->dgate), "norm backward: dx, du (with u) and dgate (with gate) are needed");
         NN_REQUIRE(!n->dz || n->pre, "norm backward: dz goes with pre");
@@ -310,10 +390,18 @@ int vector_of(const plmpm_norm* n, bool backward) {
     return 1;
 }
 
-template <class TX, class TU, int VW> void launch(const NormArgs& A, bool backward, int blocks, hipStream_t st) {
+template <class TX, class TU, int VW, bool ALL, bool EVEN> void launch(const NormArgs& A, bool backward, int blocks, hipStream_t st) {
     const dim3 grid((unsigned)blocks), block((unsigned)block_of(A.tpr));
-    if (backward) hipLaunchKernelGGL((k_norm_backward<TX, TU, VW>), grid, block, 0, st, A);
-    else hipLaunchKernelGGL((k_norm_forward<TX, TU, VW>), grid, block, 0, st, A);
+    if (!backward) hipLaunchKernelGGL((k_norm_forward<TX, TU, VW, ALL, EVEN>), grid, block, 0, st, A);
+    else if (A.tpr == 1024) hipLaunchKernelGGL((k_norm_backward<TX, TU, VW, 1024, ALL, EVEN>), grid, block, 0, st, A);
+    else hipLaunchKernelGGL((k_norm_backward<TX, TU, VW, 512, ALL, EVEN>), grid, block, 0, st, A);
+}
+template <class TX, class TU, int VW> void launch(const NormArgs& A, bool backward, int blocks, hipStream_t st) {
+    const bool all = A.u && A.gate && A.scale && A.post && A.pre && (backward ? A.dy && A.dz : A.y && A.z);
+    const bool even = VW == 8 && A.D == A.tpr * kCols && A.rows % (block_of(A.tpr) / A.tpr) == 0;
+    if (VW == 8 && all && even) launch<TX, TU, 8, true, true>(A, backward, blocks, st);
+    else if (all) launch<TX, TU, VW, true, false>(A, backward, blocks, st);
+    else launch<TX, TU, VW, false, false>(A, backward, blocks, st);
 }
 template <class TX, class TU> void launch(const NormArgs& A, int vw, bool backward, int blocks, hipStream_t st) {
     if (vw == 8) launch<TX, TU, 8>(A, backward, blocks, st);
@@ -334,7 +422,7 @@ int run(const plmpm_norm* n, bool backward, hipStream_t st) {
     A.rows = n->rows; A.sx = n->stride_x; A.su = n->stride_u; A.sg = n->stride_gate; A.sdy = n->stride_dy; A.sdz = n->stride_dz;
     A.D = (int)n->width; A.fn = n->gate_fn; A.wt = n->w_dtype; A.eps = (float)n->eps;
     A.tpr = row_threads(n->width);
-    const int vw = vector_of(n, backward), blocks = blocks_of(n);
+    const int vw = vector_of(n, backward), blocks = blocks_of(n, backward);
     if (blocks) {
         if (n->x_dtype == PLMPM_NN_BF16) launch<bf16, bf16>(A, vw, backward, blocks, st);
         else if (n->x_dtype == PLMPM_NN_F16) launch<f16, f16>(A, vw, backward, blocks, st);
@@ -355,7 +443,7 @@ extern "C" {
 int plmpm_norm_workspace(const plmpm_norm* n, size_t* bytes) {
     NN_REQUIRE(n && bytes, "norm: null argument");
     NN_REQUIRE(n->rows >= 0 && n->width >= 0 && n->width <= kMaxWidth, "norm: rows %lld x width %lld: negative, or wider than %d", (long long)n->rows, (long long)n->width, kMaxWidth);
-    *bytes = n->width ? (size_t)blocks_of(n) * 3 * n->width * sizeof(float) : 0;
+    *bytes = n->width ? (size_t)blocks_of(n, true) * 3 * n->width * sizeof(float) : 0;
     return 0;
 }
 int plmpm_norm_forward(const plmpm_norm* n, void* hip_stream) { return run(n, false, (hipStream_t)hip_stream); }

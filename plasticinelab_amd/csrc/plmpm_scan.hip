@@ -73,21 +73,6 @@ template <int S> __device__ __forceinline__ unsigned reset_bits(const ScanArgs& 
     return (unsigned)__ballot(hit);
 }
 
-// a row's address, the same for the whole wave, plus a lane's 32-bit offset: the empty asm keeps the row's address in scalar registers (the compiler
-// would otherwise add row and offset once a lane in 64 bits, and hold two vector registers for each of the 48 loads in flight)
-template <class T> __device__ __forceinline__ T* at_offset(T* row, unsigned bytes) {
-#if defined(PLB_HOST_EMUL)
-    return (T*)((char*)row + bytes);
-#else
-    typedef char __attribute__((address_space(1))) * Global;
-    const uint64_t r = (uint64_t)row;
-    unsigned lo = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)r), hi = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(r >> 32));
-    uint64_t u = ((uint64_t)hi << 32) | lo;
-    asm("" : "+s"(u));
-    return (T*)(char*)((Global)u + bytes);
-#endif
-}
-
 // S steps from t on, `stride` elements apart: whole, or the first `left` of them (those behind load the last one again)
 template <bool WHOLE, class T, int VEC, int S> __device__ __forceinline__ void load_steps(const void* base, int64_t stride, int left, unsigned offset, Vec<T, VEC> (&raw)[S]) {
     T* row = (T*)base;
