@@ -93,7 +93,7 @@ typedef struct plmpm_adamw_tensor {
 typedef struct plmpm_adamw {
     int32_t state_bits, reserved;
     double lr, beta_1, beta_2, epsilon, weight_decay, max_norm, lo, hi;
-    int64_t* step;                          /* device, two words: updates done (read, then incremented), and a word that is zero between calls */
+    int64_t* step;                          /* device, two words: updates done, updates begun (equal between calls; set the first) */
     float* grad_norm;                       /* device, where max_norm > 0: the norm before clipping; may be null */
     void* workspace;
     size_t workspace_bytes;

@@ -23,7 +23,7 @@ namespace {
 constexpr int kChunk = 4096, kBlock = 256, kThreads = 256;
 constexpr int kMaxTensors = 48;         // 72 bytes each + their first chunks: the kernel arguments stay below 4 KB
 constexpr int kMaxGroups = 2048;        // workgroups of a launch (8 a CU)
-constexpr int kNormGroups = 1024;
+constexpr int kNormGroups = 2048;
 
 struct Table {
     plmpm_adamw_tensor t[kMaxTensors];
@@ -65,39 +65,49 @@ __device__ __forceinline__ int tensor_of(const Table& tab, int chunk) {
     return lo;
 }
 
-template <class T> __device__ __forceinline__ double chunk_squares(const T* g, int64_t at, int n) {
-    double sum = 0.0;
-    if (n == kChunk && ((uintptr_t)g & 15) == 0) {
-        constexpr int V = 16 / (int)sizeof(T), R = kChunk / kThreads / V;
-        Vec<T, V> v[R];
+// sum of the squares of g[at, stop): four vectors in flight a thread, then element by element
+template <class T> __device__ __forceinline__ double run_squares(const T* g, int64_t at, int64_t stop) {
+    constexpr int V = 16 / (int)sizeof(T), R = 4, whole = kThreads * V * R;
+    double sum[2] = {0.0, 0.0};
+    if (((uintptr_t)g & 15) == 0)
+        for (; at + whole <= stop; at += whole) {
+            Vec<T, V> v[R];
 #pragma unroll
-        for (int r = 0; r < R; ++r) v[r].load(g + at + (r * kThreads + threadIdx.x) * V);
+            for (int r = 0; r < R; ++r) v[r].load(g + at + (r * kThreads + threadIdx.x) * V);
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float f[V];
-            v[r].get(f);
+            for (int r = 0; r < R; ++r) {
+                float f[V];
+                v[r].get(f);
 #pragma unroll
-            for (int e = 0; e < V; ++e) sum = fma((double)f[e], (double)f[e], sum);
+                for (int e = 0; e < V; ++e) sum[e & 1] = fma((double)f[e], (double)f[e], sum[e & 1]);
+            }
         }
-    } else
-        for (int e = threadIdx.x; e < n; e += kThreads) {
-            const double f = (double)to_f(g[at + e]);
-            sum = fma(f, f, sum);
-        }
-    return sum;
+    for (at += threadIdx.x; at < stop; at += kThreads) {
+        const double f = (double)to_f(g[at]);
+        sum[0] = fma(f, f, sum[0]);
+    }
+    return sum[0] + sum[1];
 }
 
-__global__ __launch_bounds__(kThreads) void k_square_sums(Table tab, double* partial) {
+// The update's count: the launch before an update writes done + 1 into the word of those begun, which every workgroup of the update reads, and the
+// update's first workgroup copies it to the word of those done, which none of them reads.  (Counting with an atomic in the update itself, the last
+// workgroup to arrive, costs some 20 us for 1024 of them: they queue at the one address.)
+__device__ __forceinline__ void begin_update(int64_t* step) { step[1] = step[0] + 1; }
+__global__ void k_begin(int64_t* step) { begin_update(step); }
+
+__global__ __launch_bounds__(kThreads) void k_square_sums(Table tab, double* partial, int64_t* step) {
+    if (step && blockIdx.x == 0 && threadIdx.x == 0) begin_update(step);
     __shared__ double lds[kThreads / 64];
     const int begin = blockIdx.x * tab.per, end = min(begin + tab.per, tab.first[tab.count]);
     double sum = 0.0;
     int k = begin < end ? tensor_of(tab, begin) : 0;
-    for (int chunk = begin; chunk < end; ++chunk) {
+    for (int chunk = begin; chunk < end;) {
         while (chunk >= tab.first[k + 1]) ++k;
         const plmpm_adamw_tensor& t = tab.t[k];
-        const int64_t at = (int64_t)(chunk - tab.first[k]) * kChunk;
-        const int n = (int)min((int64_t)kChunk, t.n - at);
-        sum += t.dtype == PLMPM_NN_F32 ? chunk_squares((const float*)t.g, at, n) : t.dtype == PLMPM_NN_BF16 ? chunk_squares((const bf16*)t.g, at, n) : chunk_squares((const f16*)t.g, at, n);
+        const int to = min(end, tab.first[k + 1]);             // this workgroup's run of chunks in the tensor
+        const int64_t at = (int64_t)(chunk - tab.first[k]) * kChunk, stop = min(t.n, (int64_t)(to - tab.first[k]) * kChunk);
+        sum += t.dtype == PLMPM_NN_F32 ? run_squares((const float*)t.g, at, stop) : t.dtype == PLMPM_NN_BF16 ? run_squares((const bf16*)t.g, at, stop) : run_squares((const f16*)t.g, at, stop);
+        chunk = to;
     }
     sum = block_sum(sum, lds);
     if (threadIdx.x == 0) partial[blockIdx.x] = sum;
@@ -129,13 +139,39 @@ __device__ __forceinline__ float value_second(int code, float scale) {
     const float q = (float)code * (1.0f / 255.0f), r = q * q, a = r * r;
     return a * scale;
 }
-__device__ __forceinline__ int code_first(float m, float safe) {
-    const float q = rintf(sqrtf(fabsf(m) / safe) * 127.0f);
-    return m < 0.0f ? -(int)q : (int)q;
+// The codes are those of correctly rounded division and roots, which is some seventy instructions for the two of an element.  So first with
+// the hardware's approximations (each within one unit in the last place: at most 4 units, 5e-7, of the result, which is 6e-5 of a code of 127 and
+// 1.2e-4 of one of 255): they give the same code unless they come that near to the border of two, and only then is it computed in full.
+// `plain`: the scale lies where its reciprocal and the quotient are ordinary numbers.
+__device__ __forceinline__ bool ordinary(float scale) { return scale > 1e-30f && scale < 1e30f; }
+__device__ __forceinline__ bool near_border(float q) {
+    const float off = fabsf(q - rintf(q));
+    return off > 0.5f - 5e-4f;
 }
-__device__ __forceinline__ int code_second(float v, float safe) {
-    const float q = rintf(sqrtf(sqrtf(fabsf(v) / safe)) * 255.0f);
-    return v > 0.0f ? max((int)q, 1) : (int)q;
+__device__ __forceinline__ float exact_first(float m, float safe) { return sqrtf(fabsf(m) / safe) * 127.0f; }
+__device__ __forceinline__ float exact_second(float v, float safe) { return sqrtf(sqrtf(fabsf(v) / safe)) * 255.0f; }
+__device__ __forceinline__ void codes_of(const float (&m)[4], const float (&v)[4], float safe_m, float safe_v, int8_t (&cm)[4], uint8_t (&cv)[4]) {
+    float qm[4], qv[4];
+    const float im = __builtin_amdgcn_rcpf(safe_m), iv = __builtin_amdgcn_rcpf(safe_v);
+    bool again = !ordinary(safe_m) || !ordinary(safe_v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        qm[e] = __builtin_amdgcn_sqrtf(fabsf(m[e]) * im) * 127.0f;
+        qv[e] = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(fabsf(v[e]) * iv)) * 255.0f;
+        again = again || near_border(qm[e]) || near_border(qv[e]);
+    }
+    if (again)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            qm[e] = exact_first(m[e], safe_m);
+            qv[e] = exact_second(v[e], safe_v);
+        }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int a = (int)rintf(qm[e]), b = (int)rintf(qv[e]);
+        cm[e] = (int8_t)(m[e] < 0.0f ? -a : a);
+        cv[e] = (uint8_t)(v[e] > 0.0f ? max(b, 1) : b);
+    }
 }
 
 // four neighbouring elements: loaded, updated and written back, whole or up to `n`
@@ -185,55 +221,73 @@ template <class U, bool VECTOR> __device__ __forceinline__ void store4(U* p, int
         for (int e = 0; e < 4; ++e) if (e < n) p[at + e] = in[e];
 }
 
-// a chunk, `n` elements from `at`: rounds of 4 elements a thread
+// a chunk, `n` elements from `at`: rounds of 4 elements a thread.  Two rounds are loaded before the first is stored (the compiler cannot move a
+// load over another round's stores: they might be the same memory); four rounds need twice the registers and gain nothing.
 template <class T, int BITS, bool VECTOR> __device__ __forceinline__ void chunk_step(const Step& S, const Now& N, const plmpm_adamw_tensor& t, int64_t at, int n) {
-    constexpr int R = kChunk / kThreads / 4;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int e0 = (r * kThreads + (int)threadIdx.x) * 4, left = n - e0;
-        if (!VECTOR && r * kThreads * 4 >= n) break;           // (uniform)
-        const int64_t p = at + e0;
-        Quad<T, VECTOR> q;
-        q.load(t, p, left);
+    constexpr int R = VECTOR ? 2 : 1;
+    for (int first = 0; first < n; first += R * kThreads * 4) {
+        const int64_t from = at + first;
+        const int tid4 = (int)threadIdx.x * 4, lane4 = (int)(threadIdx.x & 63) * 4;
+        Quad<T, VECTOR> q[R];
         if (BITS == 32) {
-            float m[4], v[4];
-            load4<float, VECTOR>((const float*)t.m, p, left, m);
-            load4<float, VECTOR>((const float*)t.v, p, left, v);
+            float m[R][4], v[R][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) update(S, N, q.g[e], m[e], v[e], q.w[e]);
-            store4<float, VECTOR>((float*)t.m, p, left, m);
-            store4<float, VECTOR>((float*)t.v, p, left, v);
+            for (int r = 0; r < R; ++r) {
+                const int e0 = r * kThreads * 4 + tid4, left = n - first - e0;
+                q[r].load(t, from + e0, left);
+                load4<float, VECTOR>((const float*)t.m, from + e0, left, m[r]);
+                load4<float, VECTOR>((const float*)t.v, from + e0, left, v[r]);
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int e0 = r * kThreads * 4 + tid4, left = n - first - e0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) update(S, N, q[r].g[e], m[r][e], v[r][e], q[r].w[e]);
+                store4<float, VECTOR>((float*)t.m, from + e0, left, m[r]);
+                store4<float, VECTOR>((float*)t.v, from + e0, left, v[r]);
+                q[r].store(t, from + e0, left);
+            }
         } else {
-            const int64_t blk = p / kBlock;                    // the wave's block: 64 lanes x 4
-            int8_t cm[4];
-            uint8_t cv[4];
-            load4<int8_t, VECTOR>((const int8_t*)t.m, p, left, cm);
-            load4<uint8_t, VECTOR>((const uint8_t*)t.v, p, left, cv);
-            const bool any = (left + (int)(threadIdx.x & 63) * 4) > 0;       // the block has an element at all
-            const float sm = any ? t.m_scale[blk] : 0.0f, sv = any ? t.v_scale[blk] : 0.0f;
-            float m[4], v[4];
-            uint32_t tm = 0, tv = 0;
+            int8_t cm[R][4];
+            uint8_t cv[R][4];
+            float sm[R], sv[R];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                m[e] = value_first(cm[e], sm);
-                v[e] = value_second(cv[e], sv);
-                update(S, N, q.g[e], m[e], v[e], q.w[e]);
-                if (!VECTOR && e >= left) continue;
-                tm = max(tm, as_u(m[e]) & 0x7fffffffu);
-                tv = max(tv, as_u(v[e]) & 0x7fffffffu);
+            for (int r = 0; r < R; ++r) {
+                const int e0 = r * kThreads * 4 + tid4, left = n - first - e0;
+                q[r].load(t, from + e0, left);
+                load4<int8_t, VECTOR>((const int8_t*)t.m, from + e0, left, cm[r]);
+                load4<uint8_t, VECTOR>((const uint8_t*)t.v, from + e0, left, cv[r]);
+                const int64_t blk = (from + e0) / kBlock;      // the wave's block: 64 lanes x 4
+                const bool any = VECTOR || left + lane4 > 0;   // it has an element at all
+                sm[r] = any ? t.m_scale[blk] : 0.0f;
+                sv[r] = any ? t.v_scale[blk] : 0.0f;
             }
-            const float top_m = as_f(wave_max(tm)), top_v = as_f(wave_max(tv));
-            const float safe_m = top_m > 0.0f ? top_m : 1.0f, safe_v = top_v > 0.0f ? top_v : 1.0f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                cm[e] = (int8_t)code_first(m[e], safe_m);
-                cv[e] = (uint8_t)code_second(v[e], safe_v);
+            for (int r = 0; r < R; ++r) {
+                const int e0 = r * kThreads * 4 + tid4, left = n - first - e0;
+                float m[4], v[4];
+                uint32_t tm = 0, tv = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    m[e] = value_first(cm[r][e], sm[r]);
+                    v[e] = value_second(cv[r][e], sv[r]);
+                    update(S, N, q[r].g[e], m[e], v[e], q[r].w[e]);
+                    if (!VECTOR && e >= left) continue;
+                    tm = max(tm, as_u(m[e]) & 0x7fffffffu);
+                    tv = max(tv, as_u(v[e]) & 0x7fffffffu);
+                }
+                const float top_m = as_f(wave_max(tm)), top_v = as_f(wave_max(tv));
+                codes_of(m, v, top_m > 0.0f ? top_m : 1.0f, top_v > 0.0f ? top_v : 1.0f, cm[r], cv[r]);
+                store4<int8_t, VECTOR>((int8_t*)t.m, from + e0, left, cm[r]);
+                store4<uint8_t, VECTOR>((uint8_t*)t.v, from + e0, left, cv[r]);
+                if ((VECTOR || left + lane4 > 0) && lane4 == 0) {
+                    const int64_t blk = (from + e0) / kBlock;
+                    t.m_scale[blk] = top_m;
+                    t.v_scale[blk] = top_v;
+                }
+                q[r].store(t, from + e0, left);
             }
-            store4<int8_t, VECTOR>((int8_t*)t.m, p, left, cm);
-            store4<uint8_t, VECTOR>((uint8_t*)t.v, p, left, cv);
-            if (any && (threadIdx.x & 63) == 0) { t.m_scale[blk] = top_m; t.v_scale[blk] = top_v; }
         }
-        q.store(t, p, left);
     }
 }
 
@@ -245,7 +299,7 @@ template <class T, int BITS> __device__ __forceinline__ void chunk_step(const St
 
 template <int BITS> __global__ __launch_bounds__(kThreads) void k_adamw(Table tab, Step S) {
     __shared__ double lds[kThreads / 64];
-    const int64_t t = S.step[0] + 1;
+    const int64_t t = S.step[1];
     Now N{1.0f, (float)(S.lr64 / (1.0 - power(S.beta_1, t))), (float)(1.0 / sqrt(1.0 - power(S.beta_2, t)))};
     if (S.partial) {
         double sum = 0.0;
@@ -265,16 +319,7 @@ template <int BITS> __global__ __launch_bounds__(kThreads) void k_adamw(Table ta
         else if (x.dtype == PLMPM_NN_BF16) chunk_step<bf16, BITS>(S, N, x, at, n);
         else chunk_step<f16, BITS>(S, N, x, at, n);
     }
-    // the last workgroup to get here counts the update: every other one has read the count by then
-    if (!S.last) return;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        unsigned* done = (unsigned*)(S.step + 1);
-        if (__hip_atomic_fetch_add(done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1) {
-            S.step[0] = t;
-            __hip_atomic_store(done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-    }
+    if (S.last && blockIdx.x == 0 && threadIdx.x == 0) S.step[0] = t;
 }
 
 struct Values {
@@ -384,9 +429,11 @@ int plmpm_adamw_step(const plmpm_adamw* a, const plmpm_adamw_tensor* tensors, in
         for (int from = 0, n = 0; n < launches; ++n) {
             from = fill(tab, tensors, count, from);
             const int groups = groups_of(tab.first[tab.count], kNormGroups, tab.per);
-            hipLaunchKernelGGL(k_square_sums, dim3((unsigned)groups), dim3(kThreads), 0, st, tab, partial + partials);
+            hipLaunchKernelGGL(k_square_sums, dim3((unsigned)groups), dim3(kThreads), 0, st, tab, partial + partials, n ? nullptr : a->step);
             partials += groups;
         }
+    else
+        hipLaunchKernelGGL(k_begin, dim3(1), dim3(1), 0, st, a->step);
     Step S{};
     S.decay = (float)(a->lr * a->weight_decay);
     S.b1 = (float)a->beta_1; S.b2 = (float)a->beta_2; S.c1 = (float)(1.0 - a->beta_1); S.c2 = (float)(1.0 - a->beta_2);

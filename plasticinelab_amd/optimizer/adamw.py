@@ -50,7 +50,7 @@ def adamw_step(params, grads, first, second, step, *, lr=1e-3, beta_1=0.9, beta_
     bits: int8 codes (first) and uint8 codes (second) of the parameter's size, one float32 scale for each 256 of them; all of one kind, zeros at
     the start.  masters: for each parameter a float32 copy that is updated in its place, the parameter being its rounding, or None; without one
     a 16-bit parameter is itself updated in float32 and rounded, and loses updates below its last bit.  step: int64 (2,) on the GPU, zeros at the
-    start: the updates done, and a word that the kernels use.  lr and the other numbers are fixed in a captured graph; the count is not.
+    start: the updates done, and those begun.  lr and the other numbers are fixed in a captured graph; the count is not.
     A gradient that is not finite makes its element's moments and weight not finite (with max_norm: all of them).
     """
     count = len(params)

@@ -178,7 +178,7 @@ def run_adamw(dev, seed, sizes, dtypes=("f32",), bits=32, steps=3, offset=0, mas
         else:
             a, b = adamw_values([first[k], second[k]])
             assert np.array_equal(a.cpu().numpy(), m[k]) and np.array_equal(b.cpu().numpy(), v[k])
-    assert step.cpu().tolist() == [steps, 0]
+    assert step.cpu().tolist() == [steps, steps]
     for buf, n in places:
         rest = torch.cat([buf[:offset], buf[offset + n:]]).cpu()
         assert torch.equal(rest, torch.full_like(rest, 7))
