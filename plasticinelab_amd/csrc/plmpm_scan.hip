@@ -241,6 +241,44 @@ __global__ __launch_bounds__(W * 64) void k_scan_forward(ScanArgs A) {
     }
 }
 
+// One step (a rollout's): nothing to chain, so a wave takes 64 VEC channels of a row and the rows below it, 4 waves a workgroup.  The state may move
+// on in place (h0 = h_last): a thread reads and writes its own channels only.  500 x 2048, bf16: 5 us; as a tile of the kernel above, whose
+// waves then walk 15 steps behind the end, 23.
+template <class T, int VEC>
+__global__ __launch_bounds__(256) void k_scan_step(ScanArgs A) {
+    const int d = (blockIdx.x * 64 + (threadIdx.x & 63)) * VEC;
+    if (d >= A.D) return;
+    float k2[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) k2[v] = -A.c * kLog2e * softplus(A.decay[d + v]);
+    for (int64_t b = blockIdx.y * 4 + (threadIdx.x >> 6); b < A.B; b += gridDim.y * 4) {
+        Vec<T, VEC> in[3], out;
+        Vec<float, VEC> state;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) in[k].load((const T*)A.in[k] + b * A.sb[k] + d);
+        const int64_t at = b * A.D + d;
+        if (A.h0) state.load(A.h0 + at);
+        else state.zero();
+        if (A.ckpt) state.store(A.ckpt + at);
+        const bool cut = A.reset && A.reset[b];
+        float x[VEC], r[VEC], i[VEC], h[VEC];
+        in[0].get(x);
+        in[1].get(r);
+        in[2].get(i);
+        state.get(h);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            const Gates g = gates(r[v], i[v], k2[v]);
+            const float u = g.si * x[v];
+            h[v] = cut ? u : fmaf(g.a, h[v], u * __builtin_amdgcn_sqrtf(g.m2));
+        }
+        out.set(h);
+        out.store((T*)A.h + at);
+        state.set(h);
+        if (A.h_last) state.store(A.h_last + at);
+    }
+}
+
 // Backward: g_t = dh_t + a_{t+1} g_{t+1}, walked from the end.  With e_t = a_t g_t as what a step hands to the one before it, a run acts
 // on what comes in from behind as e -> A e + E with the same A, so both walks (forward again from the tile's checkpoint, which gives
 // h_{t-1} in 32 bits, and backward) go through one exchange; tiles are handed out from the last to the first.
@@ -468,6 +506,18 @@ template <class T> void launch(const ScanArgs& A, int vec, bool backward, hipStr
     launch<T, 1>(A, backward, st);
 }
 
+// one step: four channels a lane where everything keeps to them
+template <class T> void launch_step(const ScanArgs& A, hipStream_t st) {
+    bool four = A.D % 4 == 0 && aligned_to(A.h, 0, 1) >= 4 * (int)sizeof(T);
+    for (int k = 0; k < 3; ++k) four = four && aligned_to(A.in[k], A.sb[k], (int)sizeof(T)) >= 4 * (int)sizeof(T);
+    for (const void* p : {(const void*)A.h0, (const void*)A.h_last, (const void*)A.ckpt}) four = four && aligned_to(p, 0, 1) >= 16;
+    const int vec = four ? 4 : 1;
+    const int64_t across = (A.D + 64 * vec - 1) / (64 * vec), down = std::min<int64_t>((A.B + 3) / 4, std::max<int64_t>(1, 4096 / across));
+    const dim3 grid((unsigned)across, (unsigned)down);
+    if (four) hipLaunchKernelGGL((k_scan_step<T, 4>), grid, dim3(256), 0, st, A);
+    else hipLaunchKernelGGL((k_scan_step<T, 1>), grid, dim3(256), 0, st, A);
+}
+
 // Channels a lane: 4 bytes' worth, so that a wave's rows are 256 bytes -- 2 channels of 16 bits where rows and pointers keep to it and at least half
 // of a wave's 128 channels are there, else 1.  (16 bits, 8 x 2047 x 2048, forward and backward: 2 channels 70 + 141 us, 1 channel 80 + 158, 4
 // channels 72 + 202; 32 bits, 16 x 50 x 256: 1 channel 7.2 + 9.0 us, 2 channels 8.1 + 11.9.)
@@ -515,6 +565,13 @@ int run(const plmpm_scan* s, bool backward, hipStream_t st) {
     A.dh = s->dh; A.dlast = s->dlast; A.out[0] = s->dx; A.out[1] = s->dr; A.out[2] = s->di;
     A.dh0 = s->dh0;
     A.B = s->batch; A.T = s->steps; A.D = (int)s->width; A.c = (float)s->c;
+    if (!backward && s->steps == 1) {
+        if (s->dtype == PLMPM_NN_F32) launch_step<float>(A, st);
+        else if (s->dtype == PLMPM_NN_BF16) launch_step<bf16>(A, st);
+        else launch_step<f16>(A, st);
+        NN_LAUNCHED("scan forward");
+        return 0;
+    }
     const int vec = vector_of(s, backward);
     A.cblks = (A.D + 64 * vec - 1) / (64 * vec);
     A.tiles = (int)tiles_of(s, backward);
