@@ -102,31 +102,39 @@ __device__ __forceinline__ Word state_word(float h) { return ((Word)as_u(h) << 3
 __device__ __forceinline__ void publish(Word* p, Word w) { __hip_atomic_store(p, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ Word look(const Word* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
-// the state that position `pos` starts with: back over the positions before it (`p`: this channel's word at position 0, `stride` words
-// apart), two at a time (each poll goes past the caches: 65537 x 1024 forward / 8 x 2047 x 2048 backward 134 / 131 us, four at a time 133 / 143, eight
-// 143 / 171 without the later steps; without any of this, wrong, 118 / 129).  Position 0 publishes its state, so the walk ends there at the latest.
-__device__ __forceinline__ float state_before(const Word* p, int64_t stride, int pos) {
-    float A = 1.0f, H = 0.0f;
-    int j = pos - 1;
-    for (;;) {
+// The state that position `pos` starts with (`p`: this channel's word at position 0, `stride` words apart): back over the positions before it to one
+// whose state is known, then forward again over what those in between published.  The state behind a position is always its H + A times the
+// state before it, so every route gives the same bits, however far a walk happens to go.  What it meets on the way is kept in `path` (this
+// channel's column of [kPath][NCH]); a walk that has filled it waits for the state of the position it has reached.  Position 0 publishes its
+// state, so no walk goes further.  Two words a poll, each past the caches: 65537 x 1024 forward / 8 x 2047 x 2048 backward 134 / 131 us, with four
+// 133 / 143; without any handing over, wrong, 118 / 129.
+constexpr int kPath = 16;
+struct Run { float A, H; };
+template <int NCH> __device__ __forceinline__ float state_before(const Word* p, int64_t stride, int pos, Run* path) {
+    int n = 0;
+    float h = 0.0f;
+    for (bool found = false; !found;) {
         Word w[2];
 #pragma unroll
-        for (int q = 0; q < 2; ++q) w[q] = look(p + (j > q ? j - q : 0) * stride);
+        for (int q = 0; q < 2; ++q) w[q] = look(p + (pos - 1 - n > q ? pos - 1 - n - q : 0) * stride);
         bool waits = false;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-            if (waits || j < 0) continue;
+            if (found || waits) continue;
             const unsigned low = (unsigned)w[q];
-            const float h = as_f((unsigned)(w[q] >> 32));
-            if (low == 0) { waits = true; continue; }
-            H = fmaf(A, h, H);
-            if (low == kState) return H;
-            A *= as_f(low - 1u);
-            if (forgets(as_f(low - 1u))) return H;
-            --j;
+            const float A = as_f(low - 1u);
+            h = as_f((unsigned)(w[q] >> 32));
+            if (low == kState || (low && forgets(A))) found = true;
+            else if (low == 0 || n == kPath) waits = true;
+            else path[n++ * NCH] = {A, h};
         }
         if (waits) sleep_a_little();
     }
+    while (n) {
+        const Run r = path[--n * NCH];
+        h = fmaf(r.A, h, r.H);
+    }
+    return h;
 }
 
 // which tile and which channels this workgroup takes: in the order of a ticket where there is more than one tile
@@ -148,6 +156,7 @@ template <class T, int VEC, int S, int W, bool RESET>
 __global__ __launch_bounds__(W * 64) void k_scan_forward(ScanArgs A) {
     constexpr int NCH = 64 * VEC;
     __shared__ float sA[W][NCH], sH[W][NCH];
+    __shared__ Run path[kPath][NCH];
     __shared__ unsigned ticket;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const Place at = place<NCH>(A, &ticket);
@@ -202,17 +211,20 @@ __global__ __launch_bounds__(W * 64) void k_scan_forward(ScanArgs A) {
     for (int ch = threadIdx.x; ch < NCH; ch += blockDim.x) {
         if (first + ch >= A.D) continue;
         const int64_t col = b * A.D + first + ch, stride = A.B * A.D;
-        float c;
-        if (at.pos == 0) c = A.h0 ? A.h0[col] : 0.0f;
-        else {
+        float c = at.pos == 0 && A.h0 ? A.h0[col] : 0.0f;
+        if (A.tiles > 1) {
             float ta = 1.0f, th = 0.0f;
             for (int w = 0; w < waves; ++w) {
                 const float pa = sA[w][ch], ph = sH[w][ch];
                 th = forgets(pa) ? ph : fmaf(pa, th, ph);
                 ta = forgets(pa) ? -0.0f : ta * pa;
             }
-            if (at.pos < A.tiles - 1) publish(A.words + (int64_t)at.pos * stride + col, word_of(ta, th));
-            c = state_before(A.words + col, stride, at.pos);
+            Word* mine = A.words + (int64_t)at.pos * stride + col;
+            if (at.pos > 0) {
+                if (at.pos < A.tiles - 1) publish(mine, word_of(ta, th));
+                c = state_before<NCH>(A.words + col, stride, at.pos, &path[0][ch]);
+            }
+            if (at.pos < A.tiles - 1) publish(mine, state_word(forgets(ta) ? th : fmaf(ta, c, th)));
         }
         for (int w = 0; w < waves; ++w) {
             const float pa = sA[w][ch], ph = sH[w][ch];
@@ -221,8 +233,7 @@ __global__ __launch_bounds__(W * 64) void k_scan_forward(ScanArgs A) {
             sA[w][ch] = c;
             c = forgets(pa) ? ph : fmaf(pa, c, ph);
         }
-        if (at.pos < A.tiles - 1) publish(A.words + (int64_t)at.pos * stride + col, state_word(c));
-        else if (A.h_last) A.h_last[col] = c;
+        if (A.h_last && at.pos == A.tiles - 1) A.h_last[col] = c;
     }
     __syncthreads();
     float now[VEC];
@@ -289,6 +300,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
     static_assert(S * W % kCheckpoint == 0, "a tile starts at a checkpoint");
     constexpr int NCH = 64 * VEC;
     __shared__ float sA[W][NCH], sH[W][NCH], sE[W][NCH];
+    __shared__ Run path[kPath][NCH];
     __shared__ unsigned ticket;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const Place at = place<NCH>(A, &ticket);
@@ -367,25 +379,27 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
     for (int ch = threadIdx.x; ch < NCH; ch += blockDim.x) {
         if (first + ch >= A.D) continue;
         const int64_t col = b * A.D + first + ch, stride = A.B * A.D;
-        float c = A.ckpt[(int64_t)tile * (S * W / kCheckpoint) * stride + col], e;
-        if (at.pos == 0) e = A.dlast ? A.dlast[col] : 0.0f;
-        else {
+        float c = A.ckpt[(int64_t)tile * (S * W / kCheckpoint) * stride + col], e = at.pos == 0 && A.dlast ? A.dlast[col] : 0.0f;
+        if (A.tiles > 1) {
             float ta = 1.0f, te = 0.0f;
             for (int w = waves - 1; w >= 0; --w) {
                 const float pa = sA[w][ch], pe = sE[w][ch];
                 te = forgets(pa) ? pe : fmaf(pa, te, pe);
                 ta = forgets(pa) ? -0.0f : ta * pa;
             }
-            if (at.pos < A.tiles - 1) publish(A.words + (int64_t)at.pos * stride + col, word_of(ta, te));
-            e = state_before(A.words + col, stride, at.pos);
+            Word* mine = A.words + (int64_t)at.pos * stride + col;
+            if (at.pos > 0) {
+                if (at.pos < A.tiles - 1) publish(mine, word_of(ta, te));
+                e = state_before<NCH>(A.words + col, stride, at.pos, &path[0][ch]);
+            }
+            if (at.pos < A.tiles - 1) publish(mine, state_word(forgets(ta) ? te : fmaf(ta, e, te)));
         }
         for (int w = waves - 1; w >= 0; --w) {
             const float pa = sA[w][ch], pe = sE[w][ch];
             sE[w][ch] = e;
             e = forgets(pa) ? pe : fmaf(pa, e, pe);
         }
-        if (at.pos < A.tiles - 1) publish(A.words + (int64_t)at.pos * stride + col, state_word(e));
-        else if (A.dh0) A.dh0[col] = e;
+        if (A.dh0 && at.pos == A.tiles - 1) A.dh0[col] = e;
         for (int w = 0; w < waves; ++w) {
             const float pa = sA[w][ch], ph = sH[w][ch];
             sA[w][ch] = c;

@@ -10,6 +10,10 @@ loss w.r.t. the policy parameters flows
          -> d loss / d obs[t] -> back into the HIP adjoint of frame t*substeps (particle x, v and manipulator poses)
 
 the last arrow through ``Tape(after_step_grad=...)`` / ``Engine.add_frame_grad`` / ``add_primitive_grad``.
+
+A policy on the CPU runs in float64.  A policy on a GPU keeps its own type and place, may have a memory (``initial_state`` and ``step``, as
+``policy.RecurrentPolicy`` has them: its gradient then also flows from each step's state to the one before), and is what ``optim.type =
+"AdamW"`` and ``imitate`` are for.
 """
 from __future__ import annotations
 
@@ -18,9 +22,10 @@ import torch
 
 from ..config import CfgNode
 from ..engine.taichi_env import TaichiEnv, Tape
+from .adamw import AdamW
 from .optim import Adam, Momentum
 
-OPTIMS = {"Adam": Adam, "Momentum": Momentum}
+OPTIMS = {"Adam": Adam, "Momentum": Momentum, "AdamW": AdamW}
 
 
 class Observation:
@@ -71,7 +76,10 @@ class SolverNN:
         self.cfg.optim.lr *= 0.001                         # solver_nn.py:6-7
         self.cfg.optim.bounds = (-np.inf, np.inf)
         self.env = env
-        self.policy = policy.double()
+        first = next(policy.parameters(), None)
+        self.policy = policy if first is not None and first.is_cuda else policy.double()
+        first = next(self.policy.parameters(), None)
+        self.place = {"dtype": torch.float64, "device": "cpu"} if first is None else {"dtype": first.dtype, "device": first.device}
         self.logger = logger
         self.obs = Observation(env, n_observed_particles, velocity_weight)
         self.total_steps = 0
@@ -83,7 +91,7 @@ class SolverNN:
 
     # ---- flat parameter vector, as nn.get_params / set_params / get_grad (mlp.py:154-183)
     def get_params(self):
-        return np.concatenate([p.detach().cpu().numpy().reshape(-1) for p in self.policy.parameters()])
+        return np.concatenate([p.detach().double().cpu().numpy().reshape(-1) for p in self.policy.parameters()])
 
     def set_params(self, flat):
         flat = np.asarray(flat, np.float64)
@@ -103,44 +111,93 @@ class SolverNN:
             self.logger.reset()
         for p in self.policy.parameters():
             p.grad = None
-        graph = {}                                         # step -> (obs tensor, action tensor)
+        graph = {}                                         # step -> (obs tensor, action tensor[, state in, state out])
         A = env.primitives.action_dim
+        memory = hasattr(self.policy, "initial_state")
+        state = self.policy.initial_state(1) if memory else None
+        from_later = []                                    # d loss / d state handed to the next step, from the reverse sweep
 
         def after_step_grad(step, first_frame):
-            obs_t, act_t = graph.pop(step)
-            g = torch.as_tensor(sim.engine.get_action_grad(step + 1)[step].reshape(-1)[:A].copy())
-            act_t.backward(g)                              # accumulates into policy.parameters().grad, fills obs_t.grad
-            self.obs.push_grad(first_frame, obs_t.grad.numpy())
+            obs_t, act_t, *states = graph.pop(step)
+            g = torch.as_tensor(sim.engine.get_action_grad(step + 1)[step].reshape(-1)[:A].copy()).to(**self.place)
+            ends, grads = [act_t], [g]
+            if states and from_later:
+                ends.append(states[1])
+                grads.append(from_later.pop())
+            torch.autograd.backward(ends, grads)           # accumulates into policy.parameters().grad, fills obs_t.grad
+            if states:
+                from_later[:] = [states[0].grad]
+            self.obs.push_grad(first_frame, obs_t.grad.double().cpu().numpy())
 
         with Tape(env, after_step_grad=after_step_grad):
             for i in range(self.cfg.horizon):
-                obs_t = torch.tensor(self.obs.read(sim.cur), dtype=torch.float64, requires_grad=True)
-                act_t = torch.clamp(self.policy(obs_t), -1.0, 1.0)          # mlp.py:98
-                graph[i] = (obs_t, act_t)
-                env.step(act_t.detach().numpy())
+                obs_t = torch.tensor(self.obs.read(sim.cur), requires_grad=True, **self.place)
+                if memory:
+                    before = state.detach().requires_grad_()
+                    act_t, state = self.policy.step(obs_t[None], before)
+                    act_t = torch.clamp(act_t[0], -1.0, 1.0)
+                    graph[i] = (obs_t, act_t, before, state)
+                else:
+                    act_t = torch.clamp(self.policy(obs_t), -1.0, 1.0)          # mlp.py:98
+                    graph[i] = (obs_t, act_t)
+                env.step(act_t.detach().double().cpu().numpy())
                 self.total_steps += 1
                 info = env.compute_loss()
                 if self.logger is not None:
                     self.logger.step(None, None, info["reward"], None, i == self.cfg.horizon - 1, info)
-        grad = np.concatenate([(p.grad if p.grad is not None else torch.zeros_like(p)).numpy().reshape(-1)
+        grad = np.concatenate([(p.grad if p.grad is not None else torch.zeros_like(p)).double().cpu().numpy().reshape(-1)
                                for p in self.policy.parameters()])
         return env.loss.loss, grad
 
     def solve(self, callbacks=()):                         # solver_nn.py:14-63
         env = self.env
         params = self.get_params()
-        optim = OPTIMS[self.cfg.optim.type](params, self.cfg.optim)
+        on_device = self.cfg.optim.type == "AdamW"         # updates the policy's tensors where they are; the others a flat vector
+        optim = OPTIMS[self.cfg.optim.type](list(self.policy.parameters()) if on_device else params, self.cfg.optim)
         env_state = env.get_state()
         self.total_steps = 0
         best, best_loss = None, 1e10
         for _ in range(self.cfg.n_iters):
             self.params = params
-            loss, grad = self.forward(env_state["state"], params)
+            loss, grad = self.forward(env_state["state"], None if on_device else params)
             if loss < best_loss:
                 best_loss, best = loss, params.copy()
-            params = optim.step(grad)
+            if on_device:
+                optim.step()
+                params = self.get_params()
+            else:
+                params = optim.step(grad)
             for cb in callbacks:
                 cb(self, optim, loss, grad)
         env.set_state(**env_state)
         self.set_params(best)
         return best
+
+    # ---- a warm start from action sequences that another solver found
+    def record(self, sim_state, actions):
+        """Run ``actions`` (H, action_dim) from ``sim_state``: -> the observations (H, obs.dim) a policy would have seen before each of them."""
+        env, seen = self.env, []
+        env.set_state(sim_state, self.cfg.softness, False)
+        for a in actions:
+            seen.append(self.obs.read(env.simulator.cur))
+            env.step(a)
+        return np.stack(seen)
+
+    def imitate(self, observations, actions, n_iters=100, reset=None):
+        """Fit the policy to recorded sequences by least squares: observations (B, H, obs.dim), actions (B, H, action_dim); ``reset`` (B, H) marks steps
+        that begin an episode (sequences of several).  Whole sequences go through the policy at once; AdamW with this solver's optimiser settings
+        updates it.  -> the mean squared errors, one an iteration."""
+        obs, target = (torch.as_tensor(np.asarray(a)).to(**self.place) for a in (observations, actions))
+        if reset is not None:
+            reset = torch.as_tensor(np.asarray(reset, bool)).to(self.place["device"])
+        optim = AdamW(list(self.policy.parameters()), self.cfg.optim)
+        losses = []
+        for _ in range(int(n_iters)):
+            for p in self.policy.parameters():
+                p.grad = None
+            out = self.policy(obs, reset=reset)[0] if hasattr(self.policy, "initial_state") else self.policy(obs)
+            loss = torch.nn.functional.mse_loss(out.float(), target.float())
+            loss.backward()
+            optim.step()
+            losses.append(loss.detach())
+        return [float(x) for x in losses]

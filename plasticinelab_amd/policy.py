@@ -322,3 +322,80 @@ def block_norm(x, u=None, gate=None, scale=None, post=None, pre=None, *, eps: fl
     run = _BlockNorm.apply if _tracked(x, u, gate, scale, post, pre) else _norm_forward
     y, z = run(x, u, gate, scale, post, pre, u_dtype, float(eps), GATES[gate_fn])
     return (x if u is None else y), z
+
+
+# ---------------------------------------------------------------------------------------------- the policy
+class RecurrentPolicy(torch.nn.Module):
+    """Observations to actions with a memory: a linear embedding, ``depth`` blocks around a gated linear recurrence, and a linear head.
+
+        z = pre * y / rms(y);   x, r, i, g = z W_in;   u = gated_scan(x, r, i) W_out;   y += scale * f(g) * post * u / rms(u)
+
+    ``forward`` takes whole sequences, ``step`` one observation of each row (both differentiable, the same numbers), ``act`` the same without
+    gradients, with the state moved on in place.  ``dtype`` is the type of the matrices and of what passes through them; the residual stream, the norms'
+    weights, the decays and the state are float32.  Actions are not bounded here (SolverNN clamps them, as plb/engine/nn/mlp.py:98 does).
+    """
+
+    def __init__(self, obs_dim, action_dim, width=128, depth=2, *, gate_fn="sigmoid", c=8.0, eps=1e-6, device="cuda", dtype=torch.float32):
+        super().__init__()
+        if dtype not in DTYPES:
+            _refuse(f"dtype has to be float32, bfloat16 or float16, got {dtype}")
+        if not 1 <= width <= MAX_WIDTH or depth < 1:
+            _refuse(f"width has to lie in 1..{MAX_WIDTH} and depth has to be at least 1, got {width} and {depth}")
+        if gate_fn not in GATES:
+            _refuse(f"gate_fn has to be one of {sorted(GATES)}, got {gate_fn!r}")
+        self.width, self.depth, self.gate_fn, self.c, self.eps = int(width), int(depth), gate_fn, float(c), float(eps)
+        how = {"device": device, "dtype": dtype}
+        vectors = lambda n, value: torch.nn.ParameterList([torch.nn.Parameter(torch.full((width,), value, device=device)) for _ in range(n)])    # noqa: E731
+        self.embed = torch.nn.Linear(obs_dim, width, **how)
+        self.into = torch.nn.ModuleList([torch.nn.Linear(width, 4 * width, **how) for _ in range(depth)])
+        self.out = torch.nn.ModuleList([torch.nn.Linear(width, width, **how) for _ in range(depth)])
+        self.head = torch.nn.Linear(width, action_dim, **how)
+        self.pre, self.post, self.scale = vectors(depth + 1, 1.0), vectors(depth, 1.0), vectors(depth, 0.5)
+        # decays of 0.9 .. 0.999 a step at a fully open gate
+        at = torch.linspace(0.9, 0.999, width, dtype=torch.float64)
+        start = torch.log(torch.expm1(-torch.log(at) / c)).float().to(device)
+        self.decay = torch.nn.ParameterList([torch.nn.Parameter(start.clone()) for _ in range(depth)])
+
+    def initial_state(self, batch=1):
+        """The state before the first observation: float32 (depth, batch, width), zeros."""
+        return torch.zeros(self.depth, batch, self.width, device=self.decay[0].device)
+
+    def _run(self, obs, memory):
+        """obs (..., obs_dim) -> actions; ``memory(k, x, r, i)`` is block k's recurrence."""
+        dtype = self.embed.weight.dtype
+        y = self.embed(obs.to(dtype)).float()
+        _, z = block_norm(y, pre=self.pre[0], eps=self.eps, dtype=dtype)
+        for k in range(self.depth):
+            x, r, i, g = self.into[k](z).split(self.width, dim=-1)
+            u = self.out[k](memory(k, x, r, i))
+            y, z = block_norm(y, u, g, self.scale[k], self.post[k], self.pre[k + 1], eps=self.eps, gate_fn=self.gate_fn)
+        return self.head(z)
+
+    def forward(self, obs, state=None, reset=None):
+        """obs (batch, steps, obs_dim) -> (actions (batch, steps, action_dim), state behind the last step).  ``reset``: (batch, steps) bool, where a new
+        episode begins."""
+        if obs.dim() != 3:
+            _refuse(f"obs has to be (batch, steps, obs_dim), got {tuple(obs.shape)}")
+        states = []
+
+        def memory(k, x, r, i):
+            h, last = gated_scan(x, r, i, self.decay[k], None if state is None else state[k], reset, c=self.c)
+            states.append(last)
+            return h
+
+        actions = self._run(obs, memory)
+        return actions, torch.stack(states)
+
+    def step(self, obs, state):
+        """obs (batch, obs_dim), state -> (actions (batch, action_dim), next state)."""
+        if obs.dim() != 2:
+            _refuse(f"obs has to be (batch, obs_dim), got {tuple(obs.shape)}")
+        actions, state = self.forward(obs[:, None], state)
+        return actions[:, 0], state
+
+    @torch.no_grad()
+    def act(self, obs, state):
+        """``step`` without gradients: -> actions; ``state`` moves on in place."""
+        if obs.dim() != 2:
+            _refuse(f"obs has to be (batch, obs_dim), got {tuple(obs.shape)}")
+        return self._run(obs, lambda k, x, r, i: gated_scan_step(x, r, i, self.decay[k], state[k], c=self.c))
