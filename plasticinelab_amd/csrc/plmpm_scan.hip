@@ -313,9 +313,10 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
     const int left = __builtin_amdgcn_readfirstlane(steps_left(A.T, t0, S));
     const int64_t from = left ? t0 : A.T - 1;
     const unsigned offset = (unsigned)dl * (unsigned)sizeof(T), cut = RESET ? reset_bits<S>(A, b, t0, left) : 0u;
-    // kept for the second walk: x and dh as they came, a, the gates, m s_i, and s_i x a^2 / m
+    // Kept for the second walk: x and dh as they came, a, m and the gates.  What can be had from those in a few operations is not (a register more
+    // here is one spilled to memory: with m s_i and s_i x a^2 / m held in m's place, 29 of them, 8 x 2047 x 2048 took 154 us instead of 131).
     Vec<T, VEC> rawx[S], rawg[S];
-    float k2[VEC], a[S][VEC], sr[S][VEC], si[S][VEC], ms[S][VEC], pull[S][VEC], PA[VEC], PH[VEC], PE[VEC];
+    float k2[VEC], a[S][VEC], sr[S][VEC], si[S][VEC], m[S][VEC], PA[VEC], PH[VEC], PE[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
         PA[v] = 1.0f;
@@ -345,17 +346,14 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
                 si[s][v] = g.si;
                 if (RESET && (cut >> s & 1)) {
                     a[s][v] = 0.0f;
-                    ms[s][v] = g.si;
-                    pull[s][v] = 0.0f;
+                    m[s][v] = 1.0f;
                     PA[v] = -0.0f;
                     PH[v] = g.si * x[v];
                 } else {
-                    const float inv = g.m2 == 0.0f ? 0.0f : __builtin_amdgcn_rsqf(g.m2);
                     a[s][v] = there ? g.a : 1.0f;
-                    ms[s][v] = there ? g.m2 * inv * g.si : 0.0f;
-                    pull[s][v] = g.si * x[v] * (g.a * g.a * inv);
+                    m[s][v] = there ? __builtin_amdgcn_sqrtf(g.m2) : 0.0f;
                     PA[v] *= a[s][v];
-                    PH[v] = fmaf(a[s][v], PH[v], ms[s][v] * x[v]);
+                    PH[v] = fmaf(a[s][v], PH[v], m[s][v] * g.si * x[v]);
                 }
             }
         }
@@ -409,7 +407,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
     __syncthreads();
 #pragma unroll
     for (int s = 0; s < S; ++s) { rawx[s].forget(); rawg[s].forget(); }
-    float now[VEC], e[VEC], sum[VEC];
+    float now[VEC], e[VEC], sum[VEC], pull[S][VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
         now[v] = sA[wave][lane * VEC + v];
@@ -423,8 +421,8 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             const bool reset = RESET && (cut >> s & 1);
-            const float u = ms[s][v] * x[v];
-            pull[s][v] = reset ? 0.0f : fmaf(a[s][v], now[v], -pull[s][v]);        // now: dla / g
+            const float sx = si[s][v] * x[v], u = m[s][v] * sx, inv = m[s][v] == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(m[s][v]);
+            pull[s][v] = reset ? 0.0f : a[s][v] * fmaf(-sx * inv, a[s][v], now[v]);        // dla / g
             now[v] = reset ? u : fmaf(a[s][v], now[v], u);
         }
     }
@@ -438,7 +436,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
             const bool reset = RESET && (cut >> s & 1);
             g[v] += e[v];
             e[v] = reset ? 0.0f : a[s][v] * g[v];
-            dx[v] = g[v] * ms[s][v];
+            dx[v] = g[v] * m[s][v] * si[s][v];
             const float gu = dx[v] * x[v];
             di[v] = fmaf(-gu, si[s][v], gu);
             const float q = reset ? 0.0f : g[v] * pull[s][v] * sr[s][v];

@@ -65,3 +65,280 @@ def test_adamw_without_masters_or_a_gradient_and_with_bounds():
 
 def test_adamw_more_tensors_than_one_launch_takes():
     cases.run_adamw(DEV, 34, tuple(range(1, 102)), ("f32",), 32, steps=2, max_norm=0.1)
+
+
+# ---- values that come up: masked rows, resets next to what is not finite, gates at their ends
+def test_a_reset_keeps_what_is_not_finite_out():
+    B, T, D = 2, 300, 64
+    x, r, i, decay, h0, _ = cases.scan_inputs(3, B, T, D, "f32")
+    reset = torch.zeros(B, T, dtype=torch.bool)
+    reset[0, 131], reset[1, 0], reset[1, 299] = True, True, True
+    x[0, 100, 5], h0[1, 7] = float("nan"), float("inf")
+    dh = cases.normal(9, B, T, D)
+    ref, tol = R.scan(x, r, i, decay, h0, reset, dh=dh)
+    assert not torch.isfinite(ref["h"][0, 130, 5]) and torch.isfinite(ref["h"][0, 131:]).all() and torch.isfinite(ref["h"][1]).all()
+    leaves = [t.to(DEV).requires_grad_() for t in (x, r, i, decay, h0)]
+    h, last = P.gated_scan(*leaves, reset.to(DEV))
+    cases.check({"h": h, "last": last}, ref, tol, ["h", "last"])
+    grads = dict(zip(("dx", "dr", "di"), torch.autograd.grad(h, leaves[:3], dh.to(DEV))))
+    for k in grads:                                   # behind the reset, and in the rows without: as if the NaN were not there
+        assert R.far(grads[k][0, 131:], ref[k][0, 131:], tol[k][0, 131:]) <= 1 and R.far(grads[k][1], ref[k][1], tol[k][1]) <= 1
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_scan_gates_at_their_ends(dtype):
+    """r of -inf keeps the state (a = 1), +inf lets it decay at full rate; i of -inf shuts the input; gradients stay finite."""
+    B, T, D = 1, 70, 32
+    x, r, i, decay, h0, _ = cases.scan_inputs(4, B, T, D, dtype)
+    r[:, ::3], r[:, 1::5], i[:, 2::7], i[:, 4::9] = float("-inf"), float("inf"), float("-inf"), float("inf")
+    leaves = [t.to(DEV).requires_grad_() for t in (x, r, i, decay, h0)]
+    h, last = P.gated_scan(*leaves)
+    ref, tol = R.scan(x, r, i, decay, h0)
+    cases.check({"h": h, "last": last}, ref, tol)
+    assert all(torch.isfinite(g).all() for g in torch.autograd.grad((h, last), leaves, (torch.ones_like(h), torch.ones_like(last))))
+
+
+def test_scan_decays_far_out():
+    """softplus(decay) from nothing to hundreds: a from 1 to 0."""
+    D = 64
+    x, r, i, _, h0, _ = cases.scan_inputs(5, 2, 100, D, "f32")
+    decay = torch.linspace(-30, 40, D)
+    leaves = [t.to(DEV).requires_grad_() for t in (x, r, i, decay, h0)]
+    h, last = P.gated_scan(*leaves)
+    ref, tol = R.scan(x, r, i, decay, h0)
+    cases.check({"h": h, "last": last}, ref, tol)
+    assert all(torch.isfinite(g).all() for g in torch.autograd.grad((h, last), leaves, (torch.ones_like(h), torch.ones_like(last))))
+
+
+def test_norm_rows_of_zeros_and_of_what_is_not_finite():
+    x, u, g, scale, post, pre = cases.norm_inputs(6, (9, 200), "f32", "f32")
+    x[2], u[2], u[4], x[6, 3], u[7, 0] = 0, 0, 0, float("nan"), float("inf")
+    given = [t.to(DEV) for t in (x, u, g, scale, post, pre)]
+    y, z = P.block_norm(*given)
+    ref, tol = R.norm(x, u, g, scale, post, pre)
+    fine = [0, 1, 2, 3, 4, 5, 8]
+    cases.check({"y": y[fine], "z": z[fine]}, {k: ref[k][fine] for k in ("y", "z")}, {k: tol[k][fine] for k in ("y", "z")})
+    assert not torch.isfinite(z[6]).any() and not torch.isfinite(z[7]).all()
+
+
+def test_gradients_against_differences():
+    """d/ds of <w, out(inputs + s direction)> in float32, central differences: the step 2^-7 leaves an error of third order, below 1 % of the
+    derivative's scale for these smooth gates, and a rounding of 2^-24 |out| sqrt(n) / step."""
+    torch.manual_seed(0)
+    x, r, i, decay, h0, _ = (None if t is None else t.to(DEV) for t in cases.scan_inputs(8, 2, 40, 24, "f32"))
+    w = cases.normal(1, 2, 40, 24).to(DEV)
+    for k in range(5):
+        ins = [x, r, i, decay, h0]
+        way = torch.randn_like(ins[k])
+        leaf = ins[k].clone().requires_grad_()
+        h, _ = P.gated_scan(*(ins[:k] + [leaf] + ins[k + 1:]))
+        (g,) = torch.autograd.grad(h, leaf, w)
+        f = lambda s: float((P.gated_scan(*(ins[:k] + [ins[k] + s * way] + ins[k + 1:]))[0].double() * w).sum())      # noqa: E731,B023
+        num, exact = (f(2.0 ** -7) - f(-2.0 ** -7)) * 64, float((g.double() * way).sum())
+        assert abs(num - exact) <= 0.01 * float((g.double() * way).norm()) + 0.02
+    given = [t.to(DEV) for t in cases.norm_inputs(9, (6, 40), "f32", "f32")]
+    a, b = cases.normal(2, 6, 40).to(DEV), cases.normal(3, 6, 40).to(DEV)
+    out = lambda ins: sum((o.double() * q).sum() for o, q in zip(P.block_norm(*ins, gate_fn="silu"), (a, b)))          # noqa: E731
+    for k in range(6):
+        way = torch.randn_like(given[k])
+        leaf = given[k].clone().requires_grad_()
+        y, z = P.block_norm(*(given[:k] + [leaf] + given[k + 1:]), gate_fn="silu")
+        (g,) = torch.autograd.grad((y, z), leaf, (a, b))
+        f = lambda s: float(out(given[:k] + [given[k] + s * way] + given[k + 1:]))                                     # noqa: E731,B023
+        num, exact = (f(2.0 ** -7) - f(-2.0 ** -7)) * 64, float((g.double() * way).sum())
+        assert abs(num - exact) <= 0.01 * float((g.double() * way).norm()) + 0.02
+
+
+def test_gradient_of_an_expanded_gate_and_of_the_same_tensor_twice():
+    x, u, g, scale, post, pre = (t.to(DEV) for t in cases.norm_inputs(10, (3, 20, 48), "f32", "f32"))
+    shared = g[:, :1].clone().requires_grad_()
+    y, z = P.block_norm(x, u, shared.expand(3, 20, 48), scale, post, pre)
+    (got,) = torch.autograd.grad(z.sum() + y.sum(), shared)
+    full = shared.detach().expand(3, 20, 48).clone().requires_grad_()
+    y, z = P.block_norm(x, u, full, scale, post, pre)
+    (want,) = torch.autograd.grad(z.sum() + y.sum(), full)
+    assert torch.allclose(got, want.sum(1, keepdim=True), rtol=1e-5, atol=1e-5)
+    t = cases.normal(4, 2, 30, 48).to(DEV).requires_grad_()          # x, r and i one tensor: its gradient is the three's sum
+    decay = torch.full((48,), -4.0, device=DEV)
+    (got,) = torch.autograd.grad(P.gated_scan(t, t, t, decay)[0].sum(), t)
+    three = [t.detach().clone().requires_grad_() for _ in range(3)]
+    parts = torch.autograd.grad(P.gated_scan(*three, decay)[0].sum(), three)
+    assert torch.allclose(got, sum(parts), rtol=1e-5, atol=1e-5)
+
+
+def test_sizes_of_zero():
+    for B, T, D in ((0, 5, 8), (2, 0, 8), (2, 5, 0)):
+        x, r, i = (torch.zeros(B, T, D, device=DEV, requires_grad=True) for _ in range(3))
+        decay, h0 = torch.zeros(D, device=DEV, requires_grad=True), torch.ones(B, D, device=DEV, requires_grad=True)
+        h, last = P.gated_scan(x, r, i, decay, h0)
+        assert h.shape == (B, T, D) and torch.equal(last, h0)
+        gs = torch.autograd.grad((h, last), (x, decay, h0), (torch.ones_like(h), torch.full_like(last, 3.0)))
+        assert float(gs[1].abs().sum()) == 0 and torch.equal(gs[2], torch.full_like(h0, 3.0))
+    for shape in ((0, 8), (3, 0)):
+        x, u = (torch.zeros(shape, device=DEV, requires_grad=True) for _ in range(2))
+        pre = torch.ones(shape[-1], device=DEV, requires_grad=True)
+        y, z = P.block_norm(x, u, pre=pre)
+        (g,) = torch.autograd.grad((y, z), pre, (torch.ones_like(y), torch.ones_like(z)))
+        assert y.shape == z.shape == shape and float(g.abs().sum()) == 0
+    step = torch.zeros(2, dtype=torch.int64, device=DEV)
+    empty = torch.zeros(0, device=DEV)
+    assert adamw_step([empty], [empty], [empty], [empty], step) is None and float(adamw_step([], [], [], [], step, max_norm=1.0)) == 0
+    cases.run_adamw(DEV, 41, (0, 3, 0, 5000), ("f32",), 8, steps=2, max_norm=0.1)
+
+
+# ---- streams, graphs, repeatability
+def everything(ins, adam):
+    """A run of the operators as they are used together: norm, recurrence, norm, their gradients, an update."""
+    x, u, g, scale, post, pre, r, i, decay, dy, dz = ins
+    leaves = [t.detach().requires_grad_() for t in (x, u, g, scale, post, pre, r, i, decay)]
+    _, z0 = P.block_norm(leaves[0], pre=leaves[5])
+    h, last = P.gated_scan(z0, leaves[6], leaves[7], leaves[8])
+    y, z = P.block_norm(leaves[0], h + leaves[1], leaves[2], leaves[3], leaves[4], leaves[5])
+    grads = torch.autograd.grad((y, z), leaves, (dy, dz))
+    params, first, second, step = adam
+    norm = adamw_step(params, [grads[3].clone(), grads[8].clone()], first, second, step, max_norm=0.1, lr=0.01)
+    return [y.detach(), z.detach(), last.detach(), norm, *grads]
+
+
+def inputs_of_everything(seed, shape=(2, 200, 96)):
+    t = cases.norm_inputs(seed, shape, "f32", "f32")
+    r, i = (cases.normal(seed + 20 + k, *shape) for k in range(2))
+    return [v.to(DEV) for v in (*t, r, i, torch.full((shape[-1],), -4.0), cases.normal(seed + 30, *shape), cases.normal(seed + 31, *shape))]
+
+
+def new_adam(D=96):
+    z = lambda: [torch.zeros(D, device=DEV) for _ in range(2)]                                                         # noqa: E731
+    return [torch.ones(D, device=DEV), torch.ones(D, device=DEV)], z(), z(), torch.zeros(2, dtype=torch.int64, device=DEV)
+
+
+def test_captured_and_replayed():
+    ins = inputs_of_everything(50)
+    adam = new_adam()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        everything(ins, new_adam())
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = everything(ins, adam)
+    eager_adam = new_adam()
+    for k in range(4):
+        fresh = inputs_of_everything(60 + k)
+        for a, b in zip(ins, fresh):
+            a.copy_(b)
+        graph.replay()
+        eager = everything(fresh, eager_adam)            # the program's own work between the replays
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, eager)), k
+        assert all(torch.equal(a, b) for a, b in zip(adam[0] + adam[1] + adam[2] + [adam[3]], eager_adam[0] + eager_adam[1] + eager_adam[2] + [eager_adam[3]])), k
+        torch.randn(1 << 20, device=DEV).sum()
+    assert adam[3].tolist() == [4, 4]
+
+
+def test_two_graphs_replayed_in_turn_and_together():
+    one, two = inputs_of_everything(70), inputs_of_everything(80, (1, 333, 96))
+    want = [everything(one, new_adam()), everything(two, new_adam())]
+    graphs = []
+    for ins in (one, two):
+        g, adam = torch.cuda.CUDAGraph(), new_adam()
+        with torch.cuda.graph(g):
+            out = everything(ins, adam)
+        graphs.append((g, out))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for (g, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for (_, out), w in zip(graphs, want):            # (the update's norm and the gradients do not depend on the count)
+            assert all(torch.equal(a, b) for a, b in zip(out, w))
+
+
+def test_calls_on_two_streams_at_once():
+    ins = [inputs_of_everything(90 + k, (2, 700, 96)) for k in range(2)]
+    want = [everything(x, new_adam()) for x in ins]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for x, s in zip(ins, streams):
+            with torch.cuda.stream(s):
+                got.append(everything(x, new_adam()))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+
+
+def test_the_same_bits_each_time():
+    torch.manual_seed(1)
+    x, r, i = (torch.randn(2, 9001, 320, device=DEV).bfloat16() for _ in range(3))
+    decay, dh = torch.full((320,), -6.0, device=DEV), torch.randn(2, 9001, 320, device=DEV).bfloat16()
+
+    def run():
+        leaves = [t.detach().requires_grad_() for t in (x, r, i, decay)]
+        h, last = P.gated_scan(*leaves)
+        return [h.detach(), last.detach(), *torch.autograd.grad(h, leaves, dh)]
+
+    first = run()
+    assert all(torch.equal(a, b) for _ in range(4) for a, b in zip(first, run()))
+
+
+def test_scan_beyond_32_bits_of_elements():
+    """2.2e9 elements of output, the inputs rows that all batches share (stride 0): the last batch is what a batch of one gives, bit for bit."""
+    T, D, B = 65600, 1024, 33
+    x, r, i = (torch.randn(1, T, D, device=DEV, dtype=torch.bfloat16) for _ in range(3))
+    decay = torch.full((D,), -5.0, device=DEV)
+    h, last = P.gated_scan(*(t.expand(B, T, D) for t in (x, r, i)), decay)
+    one, end = P.gated_scan(x, r, i, decay)
+    assert h.numel() > 2 ** 31 and torch.equal(h[-1], one[0]) and torch.equal(h[B // 2], one[0]) and torch.equal(last[-1], end[0])
+
+
+def test_norm_beyond_32_bits_of_elements():
+    D, rows = 4096, 540000
+    x = torch.zeros(rows, D, device=DEV, dtype=torch.bfloat16)
+    x[-3:] = torch.randn(3, D, device=DEV, dtype=torch.bfloat16)
+    pre = torch.ones(D, device=DEV)
+    _, z = P.block_norm(x, pre=pre)
+    _, want = P.block_norm(x[-3:].clone(), pre=pre)
+    assert x.numel() > 2 ** 31 and torch.equal(z[-3:], want)
+
+
+# ---- the optimizer object
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_object(bits):
+    """AdamW over parameters of several types: state, checkpoint and resume, parameters set from outside, a changing lr."""
+    torch.manual_seed(2)
+    make = lambda: [torch.nn.Parameter(t.to(DEV)) for t in (torch.ones(300), torch.ones(7, 5).bfloat16(), torch.ones(4097).half())]      # noqa: E731
+    torch.manual_seed(3)
+    grads = [[torch.randn(p.shape, device=DEV).to(p.dtype) for p in make()] for _ in range(6)]
+    a = AdamW(make(), {"state_bits": bits}, lr=0.01, max_norm=1.0)
+    for g in grads[:3]:
+        a.step(g)
+    assert a.iter == 3 and float(a.grad_norm) > 0 and [m.shape for m in a.momentum_buffer] == [p.shape for p in a.parameters]
+    saved, values = a.state_dict(), [p.detach().clone() for p in a.parameters]
+    b = AdamW(make(), {"state_bits": bits}, lr=0.01, max_norm=1.0)
+    with torch.no_grad():
+        for p, v in zip(b.parameters, values):
+            p.copy_(v)
+    b.load_state_dict(saved)
+    for g in grads[3:]:
+        a.step(g)
+        for p, t in zip(b.parameters, g):
+            p.grad = t
+        b.step()
+    assert all(torch.equal(p, q) for p, q in zip(a.parameters, b.parameters)) and b.iter == 6
+    assert all(torch.equal(p, q) for p, q in zip(a.v_buffer, b.v_buffer))
+    with torch.no_grad():                                 # a 16-bit parameter set from outside takes its master along
+        a.parameters[1].fill_(5.0)
+    a.lr = 0.0
+    a.step(grads[0])
+    assert torch.equal(a.parameters[1], torch.full_like(a.parameters[1], 5.0))
+
+
+def test_a_graph_notices_that_a_parameter_was_updated():
+    p = torch.nn.Parameter(torch.ones(10, device=DEV))
+    loss = (p * p).sum()
+    AdamW([p]).step([torch.ones(10, device=DEV)])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
