@@ -1,5 +1,5 @@
-"""CPU tier: the policy-training operators' device source on the CPU interpreter (tests/host_emul/hipemu), against their 64-bit forms, and the
-refusals of their Python and C surfaces.  tests/test_gpu_policy_ops.py runs the same checks, and larger ones, on a GPU."""
+"""CPU tier: the policy-training operators' device source on the CPU interpreter (tests/host_emul/hipemu), against their 64-bit forms.
+tests/test_gpu_policy_ops.py runs the same checks, and larger ones, on a GPU."""
 import ctypes as C
 import os
 import re
@@ -10,7 +10,7 @@ import torch
 
 from plasticinelab_amd import _lib
 from plasticinelab_amd import policy as P
-from plasticinelab_amd.optimizer import AdamW, adamw_step, adamw_values
+from plasticinelab_amd.optimizer import adamw_step
 from tests import policy_cases as cases
 from tests.util import ROOT
 
@@ -91,3 +91,13 @@ def test_adamw_without_masters_or_a_gradient_and_with_bounds(interpreter):
 
 def test_adamw_more_tensors_than_one_launch_takes(interpreter):
     cases.run_adamw(interpreter, 34, tuple(range(1, 102)), ("f32",), 32, steps=2, max_norm=0.1)
+
+
+def test_numbers_out_of_range_are_refused_at_the_c_entry(interpreter):
+    p, step = torch.zeros(10), torch.zeros(2, dtype=torch.int64)
+    z = lambda: [torch.zeros(10)]                                                                        # noqa: E731
+    for kw, text in (({"beta_1": 1.0}, "betas"), ({"beta_2": -0.1}, "betas"), ({"epsilon": -1.0}, "epsilon"), ({"max_norm": -1.0}, "max_norm"), ({"bounds": (1.0, -1.0)}, "bounds"),
+                     ({"max_norm": float("nan")}, "max_norm")):
+        with pytest.raises(_lib.EngineError, match=text):
+            adamw_step([p], [p], z(), z(), step, **kw)
+    assert float(p.abs().sum()) == 0 and step.tolist() == [0, 0]

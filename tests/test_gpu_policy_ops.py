@@ -342,3 +342,29 @@ def test_a_graph_notices_that_a_parameter_was_updated():
     AdamW([p]).step([torch.ones(10, device=DEV)])
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+def test_scan_of_many_tiles_and_few_channels():
+    """200000 steps of 64 channels: one block of channels, every tile in flight waits for the one before.  The end of it against a run of the last 320
+    steps from the state before them; both sides are within the running bound of the exact values, and the bound has settled by then."""
+    T, D, tail = 200000, 64, 320
+    x, r, i = (torch.randn(1, T, D, device=DEV) for _ in range(3))
+    decay = torch.full((D,), -4.0, device=DEV)
+    h, last = P.gated_scan(x, r, i, decay)
+    _, before = P.gated_scan(*(t[:, :T - tail].contiguous() for t in (x, r, i)), decay)
+    end = [t[:, T - tail:].contiguous().cpu() for t in (x, r, i)]
+    ref, tol = R.scan(*end, decay.cpu(), before.cpu())
+    settled = tol["h"].max()
+    assert float((h[:, T - tail:].cpu().double() - ref["h"]).abs().max()) <= 2 * float(settled)
+    assert float((last.cpu().double() - ref["last"]).abs().max()) <= 2 * float(settled)
+    leaves = [t.requires_grad_() for t in (x, r, i)]
+    h, _ = P.gated_scan(*leaves, decay)
+    dh = torch.randn_like(h)
+    whole = torch.autograd.grad(h, leaves, dh)
+    start = [t.detach()[:, :tail].cpu() for t in leaves]              # the first steps, given what the step behind them hands back
+    after = [t.detach()[:, tail:].contiguous().requires_grad_() for t in leaves]
+    h0 = P.gated_scan(*[t.detach()[:, :tail].contiguous() for t in leaves], decay)[1].requires_grad_()
+    (back,) = torch.autograd.grad(P.gated_scan(*after, decay, h0)[0], h0, dh[:, tail:].contiguous())
+    ref, tol = R.scan(*start, decay.cpu(), dh=dh[:, :tail].cpu(), dlast=back)
+    for k, g in zip(("dx", "dr", "di"), whole):
+        assert float((g[:, :tail].cpu().double() - ref[k]).abs().max()) <= 2 * float(tol[k].max()), k

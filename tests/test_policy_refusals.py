@@ -1,0 +1,110 @@
+"""CPU tier: what the policy-training operators refuse -- in Python before anything is touched, and at the C entries of the library itself."""
+import ctypes as C
+
+import pytest
+import torch
+
+from plasticinelab_amd import _lib
+from plasticinelab_amd import policy as P
+from plasticinelab_amd.optimizer import AdamW, adamw_step, adamw_values
+
+
+def tensors(B=2, T=3, D=8, dtype=torch.float32):
+    return [torch.zeros(B, T, D, dtype=dtype) for _ in range(3)] + [torch.zeros(D)]
+
+
+def test_scan_refusals():
+    x, r, i, decay = tensors()
+    for args, kw, text in (
+            ((x[0], r[0], i[0], decay), {}, "3 dimensions"), ((x.double(), r.double(), i.double(), decay), {}, "float32, bfloat16 or float16"),
+            ((x, r[:, :2], i, decay), {}, "have to match x"), ((x, r.half(), i, decay), {}, "have to match x"), ((x, r, i, decay[:4]), {}, "8 values"),
+            ((x, r, i, decay.half()), {}, "float32"), ((x, r, i, torch.zeros(16)[::2]), {}, "contiguous"), ((x, r, i, decay, torch.zeros(2, 7)), {}, "h0"),
+            ((x, r, i, decay, torch.zeros(2, 8).double()), {}, "h0"), ((x, r, i, decay, None, torch.zeros(2, 3)), {}, "bool"),
+            ((x, r, i, decay, None, torch.zeros(3, 2, dtype=torch.bool)), {}, "bool"), ((x, r, i, decay), {"c": 0.0}, "c has to be positive"),
+            ((x, r, i, decay), {"c": float("nan")}, "c has to be positive"), ((x, 1.0, i, decay), {}, "r has to be a tensor")):
+        with pytest.raises(ValueError, match=text):
+            P.gated_scan(*args, **kw)
+    s = torch.zeros(2, 8)
+    for args, text in (((x, r, i, decay, s), "2 dimensions"), ((x[:, 0], r[:, 0], i[:, 0], decay, s.half()), "state"), ((x[:, 0], r[:, 0], i[:, 0], decay, torch.zeros(8, 2).T), "contiguous"),
+                       ((x[:, 0], r[:, 0], i[:, 0], decay.requires_grad_(), s), "no gradients")):
+        with pytest.raises(ValueError, match=text):
+            P.gated_scan_step(*args)
+    decay = decay.detach()
+    with pytest.raises(_lib.EngineError, match="no CPU path"):
+        P.gated_scan(x, r, i, decay)
+
+
+def test_norm_refusals():
+    x, u, w = torch.zeros(4, 8), torch.zeros(4, 8), torch.ones(8)
+    for kw, text in (({"x": x}, "u, pre or both"), ({"x": x, "gate": u, "pre": w}, "go with u"), ({"x": x, "u": u[:, :4]}, "shape"), ({"x": x, "u": u.double()}, "16 bits"),
+                     ({"x": x.half(), "u": u}, "16 bits"), ({"x": x, "u": u, "gate": u.half()}, "gate"), ({"x": x, "u": u, "pre": w[:4]}, "8 values"),
+                     ({"x": x, "u": u, "pre": w, "post": w.half()}, "one floating type"), ({"x": x, "pre": torch.ones(16)[::2]}, "contiguous"), ({"x": x, "u": u, "gate_fn": "tanh"}, "gate_fn"),
+                     ({"x": x, "u": u, "eps": -1.0}, "eps"), ({"x": x, "u": u, "dtype": torch.float16}, "calls without u"), ({"x": torch.zeros(1, 8193), "pre": torch.ones(8193)}, "at most 8192"),
+                     ({"x": torch.zeros(4, 8, dtype=torch.int32), "pre": w}, "float32, bfloat16 or float16"), ({"x": torch.zeros(()), "pre": w}, "one dimension")):
+        with pytest.raises(ValueError, match=text):
+            P.block_norm(**kw)
+    with pytest.raises(_lib.EngineError, match="no CPU path"):
+        P.block_norm(x, u)
+
+
+def test_adamw_refusals():
+    p, step = torch.zeros(300), torch.zeros(2, dtype=torch.int64)
+    z = lambda n=300, dt=torch.float32: torch.zeros(n, dtype=dt)                                         # noqa: E731
+    eight = lambda: ((z(300, torch.int8), z(2)), (z(300, torch.uint8), z(2)))                            # noqa: E731
+    m8, v8 = eight()
+    for args, kw, text in (
+            (([p], [p], [z()], [], step), {}, "one length"), (([p], [p], [z()], [z()], step[:1]), {}, "two values"), (([p.double()], [p.double()], [z()], [z()], step), {}, "parameter 0"),
+            (([torch.zeros(600)[::2]], [p], [z()], [z()], step), {}, "contiguous"), (([p], [z(299)], [z()], [z()], step), {}, "gradient 0"), (([p], [p.half()], [z()], [z()], step), {}, "gradient 0"),
+            (([p], [p], [z(299)], [z()], step), {}, "first moment"), (([p], [p], [z()], [z().half()], step), {}, "second moment"), (([p], [p], [m8], [z()], step), {}, "all have 8"),
+            (([p], [p], [v8], [v8], step), {}, "int8"), (([p], [p], [m8], [(v8[0], z(1))], step), {}, "2 contiguous float32"), (([p], [p], [z()], [z()], step), {"masters": [z()]}, "goes with 16 bits"),
+            (([p.half()], [p.half()], [z()], [z()], step), {"masters": [z(5)]}, "master")):
+        with pytest.raises(ValueError, match=text):
+            adamw_step(*args, **kw)
+    for entry, text in (((z(), z(2)), "int8 or uint8"), ((z(300, torch.int8), z(3)), "scales")):
+        with pytest.raises(ValueError, match=text):
+            adamw_values([entry])
+    with pytest.raises(ValueError, match="for each moment"):
+        adamw_values([m8], out=[])
+    with pytest.raises(_lib.EngineError, match="no CPU path"):
+        AdamW([p])
+    with pytest.raises(TypeError, match="list of tensors"):
+        AdamW(p)
+    with pytest.raises(ValueError, match="at least one"):
+        AdamW([])
+
+
+def test_c_entries_check_before_they_launch():
+    """Null pointers, sizes and alignments at the C entries of the library itself: a message and non-zero, nothing launched."""
+    lib = _lib.load_policy()
+    error = lambda: lib.plmpm_last_error().decode()                                                      # noqa: E731
+    some = 1 << 20
+    ok = dict(dtype=0, batch=1, steps=300, width=8, c=8.0, x=some, r=some, i=some, decay=some, h=some)
+    need = C.c_size_t()
+    for change, text in (({"dtype": 3}, "dtype"), ({"batch": -1}, "negative"), ({"width": 1 << 31}, "too large"), ({"steps": 1 << 40}, "too many"), ({"c": -1.0}, "c has to be"),
+                         ({"x": None}, "needed"), ({"h": None}, "needed"), ({"r": some + 2}, "aligned"), ({"batch": 1 << 29, "width": 1 << 20}, "too large"), ({}, "workspace")):
+        assert lib.plmpm_scan_forward(_lib.Scan(**{**ok, **change}), None) != 0 and text in error(), (change, error())
+    assert lib.plmpm_scan_forward(None, None) != 0 and lib.plmpm_scan_workspace(_lib.Scan(**ok), 0, None) != 0
+    assert lib.plmpm_scan_workspace(_lib.Scan(**ok), 0, need) == 0 and need.value > 0
+    assert lib.plmpm_scan_backward(_lib.Scan(**ok), None) != 0 and "needed" in error()
+    assert lib.plmpm_scan_forward(_lib.Scan(**{**ok, "workspace": some + 4, "workspace_bytes": 1 << 20}), None) != 0 and "aligned" in error()
+    assert lib.plmpm_scan_forward(_lib.Scan(**{**ok, "steps": 0}), None) == 0                           # nothing to do
+    ok = dict(rows=4, width=8, eps=1e-6, x=some, u=some, y=some, z=some, pre=some, stride_x=8, stride_u=8)
+    for change, text in (({"x_dtype": 5}, "dtype"), ({"x_dtype": 1}, "u has x's type"), ({"rows": -1}, "negative"), ({"width": 9000}, "at most"), ({"gate_fn": 7}, "gate function"),
+                         ({"eps": -1.0}, "eps"), ({"x": None}, "x is needed"), ({"u": None, "gate": some}, "go with u"), ({"y": None}, "y goes with u"), ({"pre": None}, "z with pre"),
+                         ({"x": some + 1}, "aligned"), ({"stride_x": -8}, "stride"), ({"stride_u": 1 << 28}, "stride")):
+        assert lib.plmpm_norm_forward(_lib.Norm(**{**ok, **change}), None) != 0 and text in error(), (change, error())
+    assert lib.plmpm_norm_backward(_lib.Norm(**ok), None) != 0 and "dx" in error()
+    assert lib.plmpm_norm_backward(_lib.Norm(**{**ok, "dx": some, "du": some}), None) != 0 and "workspace" in error()
+    assert lib.plmpm_norm_forward(_lib.Norm(**{**ok, "rows": 0}), None) == 0
+    ok = dict(state_bits=32, lr=0.1, beta_1=0.9, beta_2=0.99, step=some)
+    t = (_lib.AdamWTensor * 1)(_lib.AdamWTensor(p=some, g=some, m=some, v=some, n=5))
+    assert lib.plmpm_adamw_step(_lib.AdamWStep(**{**ok, "state_bits": 16}), t, 1, None) != 0 and "32 or 8" in error()
+    assert lib.plmpm_adamw_step(_lib.AdamWStep(**{**ok, "state_bits": 8}), t, 1, None) != 0 and "null" in error()
+    assert lib.plmpm_adamw_step(_lib.AdamWStep(**{**ok, "step": None}), t, 1, None) != 0 and "step" in error()
+    assert lib.plmpm_adamw_step(_lib.AdamWStep(**{**ok, "max_norm": 1.0}), t, 1, None) != 0 and "workspace" in error()
+    assert lib.plmpm_adamw_step(_lib.AdamWStep(**ok), None, 1, None) != 0 and lib.plmpm_adamw_step(_lib.AdamWStep(**ok), t, -1, None) != 0
+    t[0].master = some
+    assert lib.plmpm_adamw_step(_lib.AdamWStep(**ok), t, 1, None) != 0 and "16-bit" in error()
+    t[0].n = 0
+    assert lib.plmpm_adamw_step(_lib.AdamWStep(**ok), t, 1, None) == 0
+    assert lib.plmpm_adamw_values(None, None, None, None, None, 1, None) != 0 and "null" in error()
