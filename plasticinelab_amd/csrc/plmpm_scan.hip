@@ -137,7 +137,8 @@ template <int NCH> __device__ __forceinline__ float state_before(const Word* p, 
     return h;
 }
 
-// which tile and which channels this workgroup takes: in the order of a ticket where there is more than one tile
+// Which tile and which channels this workgroup takes: in the order of a ticket where there is more than one tile.  (Workgroups that stay and draw their
+// next ticket while they work on one hold tiles back that others wait for: 174 us instead of 133 at 65537 x 1024.)
 struct Place { int64_t b; int pos, first; };
 template <int NCH> __device__ __forceinline__ Place place(const ScanArgs& A, unsigned* shared) {
     unsigned id = blockIdx.x;

@@ -60,32 +60,36 @@ def adamw_step(params, grads, first, second, step, *, lr=1e-3, beta_1=0.9, beta_
         P._refuse("step has to be an int64 tensor of two values")
     where = step.get_device()
     bits = 8 if count and isinstance(first[0], (tuple, list)) else 32
-    flat, keep, touched, total = [], [], [], 0
-    for k, p in enumerate(params):
+    flat, keep, touched, total, codes, f32 = [], [], [], 0, P.DTYPES, torch.float32
+    for k in range(count):
         g = grads[k]
         if g is None:
             continue
+        p, m, v, ms, vs, w = params[k], first[k], second[k], 0, 0, 0
         n, dtype = p.numel(), p.dtype
-        if dtype not in P.DTYPES or not p.is_contiguous() or p.get_device() != where:
+        if dtype not in codes or not p.is_contiguous() or p.get_device() != where:
             P._refuse(f"parameter {k} has to be a contiguous float32, bfloat16 or float16 tensor on {step.device}")
-        if g.dtype != dtype or g.shape != p.shape or g.get_device() != where:
+        if g.dtype != dtype or not g.is_same_size(p) or g.get_device() != where:
             P._refuse(f"gradient {k} has to match its parameter: {tuple(p.shape)} {dtype} on {step.device}")
         if not g.is_contiguous():
             g = g.contiguous()
             keep.append(g)
-        m, v, ms, vs, w = first[k], second[k], 0, 0, 0
         if isinstance(m, (tuple, list)) != (bits == 8) or isinstance(v, (tuple, list)) != (bits == 8):
             P._refuse(f"moments of parameter {k}: all moments have 32 bits, or all have 8")
         if bits == 8:
             m, ms = _pair(m, n, where, torch.int8, f"first moment {k}")
             v, vs = _pair(v, n, where, torch.uint8, f"second moment {k}")
         else:
-            m, v = _plain(m, n, where, "a first moment"), _plain(v, n, where, "a second moment")
+            if (m.dtype != f32 or v.dtype != f32 or m.numel() != n or v.numel() != n or not m.is_contiguous() or not v.is_contiguous()
+                    or m.get_device() != where or v.get_device() != where):
+                _plain(m, n, where, "a first moment")
+                _plain(v, n, where, "a second moment")
+            m, v = m.data_ptr(), v.data_ptr()
         if masters is not None and masters[k] is not None:
-            if dtype == torch.float32:
+            if dtype == f32:
                 P._refuse(f"parameter {k} is float32: a master copy goes with 16 bits")
             w = _plain(masters[k], n, where, "a master")
-        flat += (p.data_ptr(), g.data_ptr(), m, v, ms, vs, w, n, P.DTYPES[dtype], 0)
+        flat += (p.data_ptr(), g.data_ptr(), m, v, ms, vs, w, n, codes[dtype], 0)
         touched.append(p)
         total += n
     norm = torch.empty((), dtype=torch.float32, device=step.device) if max_norm > 0 else None

@@ -54,6 +54,18 @@ def _refuse(message):
     raise ValueError(message)
 
 
+def _together(first, *others):
+    """Whether the others (None left out) are tensors on the device of the first."""
+    where = first.get_device()
+    try:
+        for t in others:
+            if t is not None and t.get_device() != where:
+                return False
+    except AttributeError:
+        return False
+    return True
+
+
 def _same_device(first, **others):
     where = first.get_device()
     for name, t in others.items():
@@ -85,7 +97,7 @@ def _scan_run(name, s, x, backward):
     lib, need = _library(), C.c_size_t()
     L.check(lib.plmpm_scan_workspace(s, backward, need), lib)
     if need.value:
-        work = torch.empty(need.value, dtype=torch.uint8, device=x.device)
+        work = x.new_empty(need.value, dtype=torch.uint8)
         s.workspace, s.workspace_bytes = work.data_ptr(), need.value
     _call(name, x, s)
 
@@ -93,9 +105,8 @@ def _scan_run(name, s, x, backward):
 def _scan_forward(x, r, i, decay, h0, reset, c, keep):
     """-> h, last, checkpoint (what the backward pass starts from; None unless ``keep``)."""
     B, T, D = x.shape
-    h = torch.empty((B, T, D), dtype=x.dtype, device=x.device)
-    last = torch.empty((B, D), dtype=torch.float32, device=x.device)
-    checkpoint = torch.empty(((T + CHECKPOINT - 1) // CHECKPOINT, B, D), dtype=torch.float32, device=x.device) if keep else None
+    h, last = x.new_empty((B, T, D)), decay.new_empty((B, D))
+    checkpoint = decay.new_empty(((T + CHECKPOINT - 1) // CHECKPOINT, B, D)) if keep else None
     if B and T and D:
         s = _scan_args(x, r, i, decay, h0, reset, c)
         s.h, s.h_last, s.checkpoint = h.data_ptr(), last.data_ptr(), _ptr(checkpoint)
@@ -121,9 +132,8 @@ class _GatedScan(torch.autograd.Function):
     def backward(ctx, dh, dlast):
         x, r, i, decay, reset, checkpoint = ctx.saved_tensors
         B, T, D = x.shape
-        dx, dr, di = (torch.empty((B, T, D), dtype=x.dtype, device=x.device) for _ in range(3))
-        ddecay = torch.empty_like(decay)
-        dh0 = torch.empty((B, D), dtype=torch.float32, device=x.device) if ctx.has_h0 else None
+        dx, dr, di, ddecay = x.new_empty((B, T, D)), x.new_empty((B, T, D)), x.new_empty((B, T, D)), decay.new_empty(D)
+        dh0 = decay.new_empty((B, D)) if ctx.has_h0 else None
         dh = None if dh is None else dh.contiguous()
         dlast = None if dlast is None else dlast.contiguous()
         if B and T and D:
@@ -141,7 +151,9 @@ class _GatedScan(torch.autograd.Function):
 def _scan_checks(x, r, i, decay, c, dims):
     if not isinstance(x, torch.Tensor) or x.dim() != dims:
         _refuse(f"x has to be a tensor of {dims} dimensions")
-    _same_device(x, r=r, i=i, decay=decay)
+    if r is None or i is None or decay is None or not _together(x, r, i, decay):
+        _same_device(x, r=r, i=i, decay=decay)
+        _refuse("r, i and decay are needed")
     shape, dtype = x.shape, x.dtype
     if dtype not in DTYPES:
         _refuse(f"x has to be float32, bfloat16 or float16, got {dtype}")
@@ -167,12 +179,14 @@ def gated_scan(x, r, i, decay, h0=None, reset=None, *, c: float = 8.0):
     _scan_checks(x, r, i, decay, c, 3)
     B, T, D = x.shape
     if h0 is not None:
-        _same_device(x, h0=h0)
+        if not _together(x, h0):
+            _same_device(x, h0=h0)
         if h0.shape != (B, D) or h0.dtype != torch.float32:
             _refuse(f"h0 has to be float32 ({B}, {D}), got {tuple(h0.shape)} {h0.dtype}")
         h0 = h0.contiguous()
     if reset is not None:
-        _same_device(x, reset=reset)
+        if not _together(x, reset):
+            _same_device(x, reset=reset)
         if reset.shape != (B, T) or reset.dtype != torch.bool:
             _refuse(f"reset has to be bool ({B}, {T}), got {tuple(reset.shape)} {reset.dtype}")
         reset = reset.contiguous()
@@ -186,14 +200,15 @@ def gated_scan_step(x, r, i, decay, state, *, c: float = 8.0):
     """One step of ``gated_scan`` for (B, D) inputs: -> h (B, D); ``state`` (B, D) float32 moves on in place.  No gradients (serving and
     evaluation; a differentiable step is ``gated_scan`` with T = 1)."""
     _scan_checks(x, r, i, decay, c, 2)
-    _same_device(x, state=state)
+    if not _together(x, state):
+        _same_device(x, state=state)
     if state is None or state.shape != x.shape or state.dtype != torch.float32 or not state.is_contiguous():
         _refuse(f"state has to be a contiguous float32 tensor of {tuple(x.shape)}")
     if _tracked(x, r, i, decay, state):
         _refuse("gated_scan_step has no gradients: call it under torch.no_grad(), or gated_scan with one step")
     x, r, i = _rows(x), _rows(r), _rows(i)
     B, D = x.shape
-    h = torch.empty((B, D), dtype=x.dtype, device=x.device)
+    h = x.new_empty((B, D))
     if B and D:
         p = state.data_ptr()
         s = L.Scan(DTYPES[x.dtype], 0, B, 1, D, (x.stride(0), r.stride(0), i.stride(0)), (0, 0, 0), c, x.data_ptr(), r.data_ptr(), i.data_ptr(), decay.data_ptr(), p, None,
@@ -224,8 +239,8 @@ def _norm_args(x, u, gate, scale, post, pre, u_dtype, eps, fn, keep):
 
 
 def _norm_forward(x, u, gate, scale, post, pre, u_dtype, eps, fn):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if u is not None else None
-    z = torch.empty(x.shape, dtype=u_dtype, device=x.device) if pre is not None else None
+    y = x.new_empty(x.shape) if u is not None else None
+    z = x.new_empty(x.shape, dtype=u_dtype) if pre is not None else None
     if x.numel():
         keep = []
         n = _norm_args(x, u, gate, scale, post, pre, u_dtype, eps, fn, keep)
@@ -250,7 +265,7 @@ class _BlockNorm(torch.autograd.Function):
         if dy is None and dz is None:
             return (None,) * 9
         D = x.shape[-1]
-        out = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=x.device) for t in saved]
+        out = [None if t is None else t.new_empty(t.shape) for t in saved]
         if x.numel():
             keep = []
             n = _norm_args(x, u, gate, scale, post, pre, u_dtype, eps, fn, keep)
@@ -263,7 +278,7 @@ class _BlockNorm(torch.autograd.Function):
             n.dx, n.du, n.dgate, n.dscale, n.dpost, n.dpre = (_ptr(t) for t in out)
             lib, need = _library(), C.c_size_t()
             L.check(lib.plmpm_norm_workspace(n, need), lib)
-            work = torch.empty(need.value, dtype=torch.uint8, device=x.device)
+            work = x.new_empty(need.value, dtype=torch.uint8)
             n.workspace, n.workspace_bytes = work.data_ptr(), need.value
             _call("plmpm_norm_backward", x, n)
         else:
@@ -287,7 +302,8 @@ def block_norm(x, u=None, gate=None, scale=None, post=None, pre=None, *, eps: fl
     """
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         _refuse("x has to be a tensor with at least one dimension")
-    _same_device(x, u=u, gate=gate, scale=scale, post=post, pre=pre)
+    if not _together(x, u, gate, scale, post, pre):
+        _same_device(x, u=u, gate=gate, scale=scale, post=post, pre=pre)
     if x.dtype not in DTYPES:
         _refuse(f"x has to be float32, bfloat16 or float16, got {x.dtype}")
     D = x.shape[-1]
