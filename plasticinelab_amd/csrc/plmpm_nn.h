@@ -64,15 +64,17 @@ constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f
 // 1 / (1 + e^-x): both ends come out right by themselves (e^-x = inf -> 0, 0 -> 1)
 __device__ __forceinline__ float sigmoid_fast(float x) { return __builtin_amdgcn_rcpf(1.0f + exp2_fast(-kLog2e * x)); }
 
-// N neighbouring elements as one access of the widest type their bytes allow (up to 16; more: several)
-template <int BYTES> struct Wide;
+// N neighbouring elements as one access of the widest type their bytes allow (up to 16; more: several).  LOOSE: at any element's address -- global
+// memory takes accesses of 16 bytes at every alignment, and the compiler makes one of a packed type
+template <int BYTES, bool LOOSE = false> struct Wide;
 template <> struct Wide<2> { typedef uint16_t type; };
 template <> struct Wide<4> { typedef uint32_t type; };
 template <> struct Wide<8> { struct alignas(8) type { uint32_t w[2]; }; };
 template <> struct Wide<16> { struct alignas(16) type { uint32_t w[4]; }; };
-template <class T, int N> struct Vec {
+template <> struct Wide<16, true> { struct __attribute__((packed, aligned(2))) type { uint32_t w[4]; }; };
+template <class T, int N, bool LOOSE = false> struct Vec {
     static constexpr int bytes = N * (int)sizeof(T), part = bytes > 16 ? 16 : bytes, parts = bytes / part;
-    typedef typename Wide<part>::type W;
+    typedef typename Wide<part, LOOSE>::type W;
     W w[parts];
     __device__ __forceinline__ void load(const T* p) {
 #pragma unroll

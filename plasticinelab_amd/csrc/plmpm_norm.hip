@@ -49,102 +49,92 @@ template <int K> __device__ __forceinline__ void row_sums(float (&v)[K], int tpr
 }
 
 // f(g) in place of g, and its derivative (one question a row, not one an element)
-__device__ __forceinline__ void gates_of(int fn, float (&g)[kCols], float (&df)[kCols]) {
+template <int VW> __device__ __forceinline__ void gates_of(int fn, float (&g)[VW], float (&df)[VW]) {
     if (fn == PLMPM_GATE_IDENTITY) {
 #pragma unroll
-        for (int k = 0; k < kCols; ++k) df[k] = 1.0f;
+        for (int k = 0; k < VW; ++k) df[k] = 1.0f;
     } else if (fn == PLMPM_GATE_SIGMOID) {
 #pragma unroll
-        for (int k = 0; k < kCols; ++k) { g[k] = sigmoid_fast(g[k]); df[k] = g[k] * (1.0f - g[k]); }
+        for (int k = 0; k < VW; ++k) { g[k] = sigmoid_fast(g[k]); df[k] = g[k] * (1.0f - g[k]); }
     } else {
 #pragma unroll
-        for (int k = 0; k < kCols; ++k) { const float s = sigmoid_fast(g[k]); df[k] = s * fmaf(g[k], 1.0f - s, 1.0f); g[k] *= s; }
+        for (int k = 0; k < VW; ++k) { const float s = sigmoid_fast(g[k]); df[k] = s * fmaf(g[k], 1.0f - s, 1.0f); g[k] *= s; }
     }
 }
-__device__ __forceinline__ void gates_of(int fn, float (&g)[kCols]) {
+template <int VW> __device__ __forceinline__ void gates_of(int fn, float (&g)[VW]) {
     if (fn == PLMPM_GATE_IDENTITY) return;
     if (fn == PLMPM_GATE_SIGMOID) {
 #pragma unroll
-        for (int k = 0; k < kCols; ++k) g[k] = sigmoid_fast(g[k]);
+        for (int k = 0; k < VW; ++k) g[k] = sigmoid_fast(g[k]);
     } else {
 #pragma unroll
-        for (int k = 0; k < kCols; ++k) g[k] *= sigmoid_fast(g[k]);
+        for (int k = 0; k < VW; ++k) g[k] *= sigmoid_fast(g[k]);
     }
 }
 // no gate counts as ones
-__device__ __forceinline__ void open_gates(float (&g)[kCols]) {
+template <int VW> __device__ __forceinline__ void open_gates(float (&g)[VW]) {
 #pragma unroll
-    for (int k = 0; k < kCols; ++k) g[k] = 1.0f;
+    for (int k = 0; k < VW; ++k) g[k] = 1.0f;
 }
 
-// column of element k of piece j: pieces of VW neighbouring columns, TPR pieces apart
-template <int VW> __device__ __forceinline__ int column(int tpr, int j) { return (j * tpr + (int)(threadIdx.x & (tpr - 1))) * VW; }
-
-// where a piece is read: pieces behind the width read the last one again (no condition around a load)
-template <int VW, bool EVEN> __device__ __forceinline__ int place(int D, int tpr, int j) {
-    const int c = column<VW>(tpr, j);
-    return EVEN || c < D ? c : D - VW;
-}
-// sum over a thread's columns that are there, of term(k)
-template <int VW, bool EVEN, class F> __device__ __forceinline__ float sum_columns(int D, int tpr, F term) {
-    float s = 0.0f;
-#pragma unroll
-    for (int j = 0; j < kCols / VW; ++j) {
-        float p = 0.0f;
-#pragma unroll
-        for (int k = j * VW; k < (j + 1) * VW; ++k) p = term(k, p);
-        s += EVEN || column<VW>(tpr, j) < D ? p : 0.0f;
+// The columns of a thread.  VW = 8: eight neighbouring ones in one access; where the width is no multiple of eight, the last thread with columns of
+// its own takes the row's last eight, and `skip` of them are its neighbour's too: both compute and store the same values there, and only the
+// neighbour counts them in sums.  Threads behind the width read the same place and count nothing.  Addresses are then those of elements, not of
+// 16 bytes (global memory takes that; 2999 x 1214, fp16, forward and backward: 12.3 + 28.7 us, with accesses of 4 bytes 13.5 + 28.6).
+// VW = 1, rows of less than eight: a column each, the threads behind them idle.
+template <int VW, bool EVEN> struct Columns {
+    int first, skip;                    // first column; how many of the VW are not this thread's to count
+    bool mine;                          // it has one at all
+    __device__ __forceinline__ Columns(int D, int tpr) {
+        first = (int)(threadIdx.x & (tpr - 1)) * VW;
+        const int over = EVEN ? 0 : first + VW - D;
+        mine = EVEN || first < D;
+        skip = over <= 0 ? 0 : over < VW ? over : VW;
+        first -= EVEN ? 0 : over > 0 ? over : 0;
     }
-    return s;
-}
-
-template <int VW, bool ALL, bool EVEN> __device__ __forceinline__ void load_weight(const void* w, int dtype, int D, int tpr, float* out) {
+    // sum of term(k, sum) over the columns that count
+    template <class F> __device__ __forceinline__ float sum(F term) const {
+        float s = 0.0f;
+        if (EVEN || skip == 0)
 #pragma unroll
-    for (int j = 0; j < kCols / VW; ++j) {
-        const int c = place<VW, EVEN>(D, tpr, j);
+            for (int k = 0; k < VW; ++k) s = term(k, s);
+        else
 #pragma unroll
-        for (int k = 0; k < VW; ++k) out[j * VW + k] = 1.0f;
-        if (!ALL && !w) continue;
-        if (dtype == PLMPM_NN_F32) { Vec<float, VW> v; v.load((const float*)w + c); v.get(out + j * VW); }
-        else if (dtype == PLMPM_NN_BF16) { Vec<bf16, VW> v; v.load((const bf16*)w + c); v.get(out + j * VW); }
-        else { Vec<f16, VW> v; v.load((const f16*)w + c); v.get(out + j * VW); }
+            for (int k = 0; k < VW; ++k) s = k >= skip ? term(k, s) : s;
+        return s;
     }
+};
+
+template <int VW, bool ALL, bool EVEN> __device__ __forceinline__ void load_weight(const void* w, int dtype, const Columns<VW, EVEN>& at, float* out) {
+#pragma unroll
+    for (int k = 0; k < VW; ++k) out[k] = 1.0f;
+    if (!ALL && !w) return;
+    if (dtype == PLMPM_NN_F32) { Vec<float, VW, !EVEN && VW == 8> v; v.load((const float*)w + at.first); v.get(out); }
+    else if (dtype == PLMPM_NN_BF16) { Vec<bf16, VW, !EVEN && VW == 8> v; v.load((const bf16*)w + at.first); v.get(out); }
+    else { Vec<f16, VW, !EVEN && VW == 8> v; v.load((const f16*)w + at.first); v.get(out); }
 }
-// a thread's columns of a row, all loads before the first use
+// a thread's columns of a row, loaded before the first use
 template <class T, int VW, bool ALL, bool EVEN> struct Row {
-    Vec<T, VW> v[kCols / VW];
+    Vec<T, VW, !EVEN && VW == 8> v;
     // row `base` is the workgroup's, `mine` rows behind it this thread's (the host sees to it that the offset fits 32 bits)
-    __device__ __forceinline__ void load(const void* p, int64_t base, int mine, int64_t stride, int D, int tpr) {
-        T* row = (T*)p + base * stride;
-        const unsigned ahead = (unsigned)mine * (unsigned)stride;
-#pragma unroll
-        for (int j = 0; j < kCols / VW; ++j) {
-            if (ALL || p) v[j].load(at_offset(row, (ahead + (unsigned)place<VW, EVEN>(D, tpr, j)) * (unsigned)sizeof(T)));
-            else v[j].zero();
-        }
+    __device__ __forceinline__ void load(const void* p, int64_t base, int mine, int64_t stride, const Columns<VW, EVEN>& at) {
+        if (ALL || p) v.load(at_offset((T*)p + base * stride, ((unsigned)mine * (unsigned)stride + (unsigned)at.first) * (unsigned)sizeof(T)));
+        else v.zero();
     }
     // unpacked where it is used, each time: in between only the elements as they came are held
     __device__ __forceinline__ void get(float* out) {
-#pragma unroll
-        for (int j = 0; j < kCols / VW; ++j) {
-            v[j].forget();
-            v[j].get(out + j * VW);
-        }
+        v.forget();
+        v.get(out);
     }
 };
-template <class T, int VW, bool EVEN> __device__ __forceinline__ void store_row(void* p, int64_t base, int mine, int D, int tpr, const float* in) {
-    T* row = (T*)p + base * D;
-#pragma unroll
-    for (int j = 0; j < kCols / VW; ++j) {
-        const int c = column<VW>(tpr, j);
-        if (!EVEN && c >= D) continue;
-        Vec<T, VW> v;
-        v.set(in + j * VW);
-        v.store(at_offset(row, ((unsigned)mine * (unsigned)D + (unsigned)c) * (unsigned)sizeof(T)));
-    }
+template <class T, int VW, bool EVEN> __device__ __forceinline__ void store_row(void* p, int64_t base, int mine, int D, const Columns<VW, EVEN>& at, const float* in) {
+    if (!at.mine) return;
+    Vec<T, VW, !EVEN && VW == 8> v;
+    v.set(in);
+    v.store(at_offset((T*)p + base * D, ((unsigned)mine * (unsigned)D + (unsigned)at.first) * (unsigned)sizeof(T)));
 }
 
-// ALL: every tensor is there; EVEN: the width is what the threads hold (TPR x 8) and the rows come out even.  A condition around a load keeps the
+// ALL: every tensor is there; EVEN: the width is what the threads hold (TPR x 8), everything keeps to 16 bytes and the rows come out even.  A condition around a load keeps the
 // compiler from counting what is in flight (it then waits for everything) and holds registers: with conditions 8192 x 4096 backward
 // took 220 us, without 157.
 template <class TX, class TU, int VW, bool ALL, bool EVEN>
@@ -153,42 +143,43 @@ __global__ __launch_bounds__(1024) void k_norm_forward(NormArgs A) {
     const int tpr = A.tpr, group = threadIdx.x / tpr, groups = blockDim.x / tpr;
     const int64_t step = (int64_t)gridDim.x * groups;
     const float inv = 1.0f / (float)A.D;
-    float scale[kCols], post[kCols], pre[kCols];
-    load_weight<VW, ALL, EVEN>(A.scale, A.wt, A.D, tpr, scale);
-    load_weight<VW, ALL, EVEN>(A.post, A.wt, A.D, tpr, post);
-    load_weight<VW, ALL, EVEN>(A.pre, A.wt, A.D, tpr, pre);
+    const Columns<VW, EVEN> at(A.D, tpr);
+    float scale[VW], post[VW], pre[VW];
+    load_weight<VW, ALL, EVEN>(A.scale, A.wt, at, scale);
+    load_weight<VW, ALL, EVEN>(A.post, A.wt, at, post);
+    load_weight<VW, ALL, EVEN>(A.pre, A.wt, at, pre);
     Row<TX, VW, ALL, EVEN> rx;
     Row<TU, VW, ALL, EVEN> ru, rg;
     const auto fetch = [&](int64_t base) {
         const int mine = EVEN || base + group < A.rows ? group : (int)(A.rows - 1 - base);
-        rx.load(A.x, base, mine, A.sx, A.D, tpr);
-        ru.load(A.u, base, mine, A.su, A.D, tpr);
-        rg.load(A.gate, base, mine, A.sg, A.D, tpr);
+        rx.load(A.x, base, mine, A.sx, at);
+        ru.load(A.u, base, mine, A.su, at);
+        rg.load(A.gate, base, mine, A.sg, at);
     };
     for (int64_t base = (int64_t)blockIdx.x * groups; base < A.rows; base += step) {
         const bool there = EVEN || base + group < A.rows;              // every thread takes part in the sums
-        float y[kCols], u[kCols], g[kCols];
+        float y[VW], u[VW], g[VW];
         fetch(base);
         rx.get(y);
         ru.get(u);
         rg.get(g);
         if (ALL || A.u) {
-            float s[1] = {sum_columns<VW, EVEN>(A.D, tpr, [&](int k, float p) { return fmaf(u[k], u[k], p); })};
+            float s[1] = {at.sum([&](int k, float p) { return fmaf(u[k], u[k], p); })};
             row_sums<1>(s, tpr, lds[0]);
             const float r = __builtin_amdgcn_rsqf(fmaf(s[0], inv, A.eps));
             if (ALL || A.gate) gates_of(A.fn, g);
             else open_gates(g);
 #pragma unroll
-            for (int k = 0; k < kCols; ++k) y[k] = fmaf(scale[k] * g[k], post[k] * (u[k] * r), y[k]);
-            if (there) store_row<TX, VW, EVEN>(A.y, base, group, A.D, tpr, y);
+            for (int k = 0; k < VW; ++k) y[k] = fmaf(scale[k] * g[k], post[k] * (u[k] * r), y[k]);
+            if (there) store_row<TX, VW, EVEN>(A.y, base, group, A.D, at, y);
         }
         if (ALL || A.z) {
-            float s[1] = {sum_columns<VW, EVEN>(A.D, tpr, [&](int k, float p) { return fmaf(y[k], y[k], p); })};
+            float s[1] = {at.sum([&](int k, float p) { return fmaf(y[k], y[k], p); })};
             row_sums<1>(s, tpr, lds[1]);
             const float r = __builtin_amdgcn_rsqf(fmaf(s[0], inv, A.eps));
 #pragma unroll
-            for (int k = 0; k < kCols; ++k) y[k] = pre[k] * (y[k] * r);
-            if (there) store_row<TU, VW, EVEN>(A.z, base, group, A.D, tpr, y);
+            for (int k = 0; k < VW; ++k) y[k] = pre[k] * (y[k] * r);
+            if (there) store_row<TU, VW, EVEN>(A.z, base, group, A.D, at, y);
         }
         if (!ALL && tpr > 64 && !(A.u && A.z)) __syncthreads();        // with one exchange a row its buffer is written again at once; with two, the other's barrier lies between
     }
@@ -200,31 +191,32 @@ __global__ __launch_bounds__(THREADS) void k_norm_backward(NormArgs A) {
     const int tpr = A.tpr, group = threadIdx.x / tpr, groups = blockDim.x / tpr;
     const int64_t step = (int64_t)gridDim.x * groups;
     const float inv = 1.0f / (float)A.D;
-    float scale[kCols], post[kCols], pre[kCols], sums[3][kCols];
-    load_weight<VW, ALL, EVEN>(A.scale, A.wt, A.D, tpr, scale);
-    load_weight<VW, ALL, EVEN>(A.post, A.wt, A.D, tpr, post);
-    load_weight<VW, ALL, EVEN>(A.pre, A.wt, A.D, tpr, pre);
+    const Columns<VW, EVEN> at(A.D, tpr);
+    float scale[VW], post[VW], pre[VW], sums[3][VW];
+    load_weight<VW, ALL, EVEN>(A.scale, A.wt, at, scale);
+    load_weight<VW, ALL, EVEN>(A.post, A.wt, at, post);
+    load_weight<VW, ALL, EVEN>(A.pre, A.wt, at, pre);
 #pragma unroll
-    for (int k = 0; k < kCols; ++k) sums[0][k] = sums[1][k] = sums[2][k] = 0.0f;
+    for (int k = 0; k < VW; ++k) sums[0][k] = sums[1][k] = sums[2][k] = 0.0f;
     Row<TX, VW, ALL, EVEN> rx, rdy;
     Row<TU, VW, ALL, EVEN> ru, rg, rdz;
     const auto fetch = [&](int64_t base) {
         const int mine = EVEN || base + group < A.rows ? group : (int)(A.rows - 1 - base);
-        rx.load(A.x, base, mine, A.sx, A.D, tpr);
-        ru.load(A.u, base, mine, A.su, A.D, tpr);
-        rg.load(A.gate, base, mine, A.sg, A.D, tpr);
-        rdy.load(A.dy, base, mine, A.sdy, A.D, tpr);
-        rdz.load(A.dz, base, mine, A.sdz, A.D, tpr);
+        rx.load(A.x, base, mine, A.sx, at);
+        ru.load(A.u, base, mine, A.su, at);
+        rg.load(A.gate, base, mine, A.sg, at);
+        rdy.load(A.dy, base, mine, A.sdy, at);
+        rdz.load(A.dz, base, mine, A.sdz, at);
     };
     for (int64_t base = (int64_t)blockIdx.x * groups; base < A.rows; base += step) {
         const bool there = EVEN || base + group < A.rows;
-        float y[kCols], dy[kCols], r = 0.0f;
+        float y[VW], dy[VW], r = 0.0f;
         fetch(base);
         rx.get(y);
         if (ALL || A.u) {
-            float u[kCols], g[kCols];
+            float u[VW], g[VW];
             ru.get(u);
-            float s[1] = {sum_columns<VW, EVEN>(A.D, tpr, [&](int k, float p) { return fmaf(u[k], u[k], p); })};
+            float s[1] = {at.sum([&](int k, float p) { return fmaf(u[k], u[k], p); })};
             row_sums<1>(s, tpr, lds[0]);
             r = __builtin_amdgcn_rsqf(fmaf(s[0], inv, A.eps));
             ru.get(u);
@@ -232,34 +224,34 @@ __global__ __launch_bounds__(THREADS) void k_norm_backward(NormArgs A) {
             if (ALL || A.gate) gates_of(A.fn, g);
             else open_gates(g);
 #pragma unroll
-            for (int k = 0; k < kCols; ++k) y[k] = fmaf(scale[k] * g[k], post[k] * (u[k] * r), y[k]);
+            for (int k = 0; k < VW; ++k) y[k] = fmaf(scale[k] * g[k], post[k] * (u[k] * r), y[k]);
         }
         rdy.get(dy);
         if (ALL || A.dz) {
-            float dz[kCols];
+            float dz[VW];
             rdz.get(dz);
-            float s[2] = {sum_columns<VW, EVEN>(A.D, tpr, [&](int k, float p) { return fmaf(y[k], y[k], p); }),
-                          sum_columns<VW, EVEN>(A.D, tpr, [&](int k, float p) { return fmaf(dz[k] * pre[k], y[k], p); })};
+            float s[2] = {at.sum([&](int k, float p) { return fmaf(y[k], y[k], p); }),
+                          at.sum([&](int k, float p) { return fmaf(dz[k] * pre[k], y[k], p); })};
             row_sums<2>(s, tpr, lds2);
             const float ry = __builtin_amdgcn_rsqf(fmaf(s[0], inv, A.eps)), mean = s[1] * inv * ry;
             rdz.get(dz);
             rdy.get(dy);
 #pragma unroll
-            for (int k = 0; k < kCols; ++k) {
+            for (int k = 0; k < VW; ++k) {
                 const float yh = y[k] * ry;
                 if (there) sums[2][k] = fmaf(dz[k], yh, sums[2][k]);
                 dy[k] = fmaf(ry, fmaf(-yh, mean, dz[k] * pre[k]), dy[k]);
             }
         }
-        if (there) store_row<TX, VW, EVEN>(A.dx, base, group, A.D, tpr, dy);
+        if (there) store_row<TX, VW, EVEN>(A.dx, base, group, A.D, at, dy);
         if (ALL || A.u) {
-            float u[kCols], g[kCols], df[kCols];
+            float u[VW], g[VW], df[VW];
             ru.get(u);
             rg.get(g);
             if (ALL || A.gate) gates_of(A.fn, g, df);
             else open_gates(g);
 #pragma unroll
-            for (int k = 0; k < kCols; ++k) {
+            for (int k = 0; k < VW; ++k) {
                 const float uh = u[k] * r, t = dy[k] * scale[k], w = t * g[k], vh = post[k] * uh;
                 if (there) {
                     sums[0][k] = fmaf(dy[k] * g[k], vh, sums[0][k]);
@@ -268,14 +260,14 @@ __global__ __launch_bounds__(THREADS) void k_norm_backward(NormArgs A) {
                 if (ALL || A.gate) g[k] = t * vh * df[k];
                 dy[k] = w * post[k];
             }
-            float s[1] = {sum_columns<VW, EVEN>(A.D, tpr, [&](int k, float p) { return fmaf(dy[k], u[k] * r, p); })};
-            if ((ALL || A.gate) && there) store_row<TU, VW, EVEN>(A.dgate, base, group, A.D, tpr, g);
+            float s[1] = {at.sum([&](int k, float p) { return fmaf(dy[k], u[k] * r, p); })};
+            if ((ALL || A.gate) && there) store_row<TU, VW, EVEN>(A.dgate, base, group, A.D, at, g);
             row_sums<1>(s, tpr, lds[1]);
             const float mean = s[0] * inv;
             ru.get(u);
 #pragma unroll
-            for (int k = 0; k < kCols; ++k) u[k] = r * fmaf(-(u[k] * r), mean, dy[k]);
-            if (there) store_row<TU, VW, EVEN>(A.du, base, group, A.D, tpr, u);
+            for (int k = 0; k < VW; ++k) u[k] = r * fmaf(-(u[k] * r), mean, dy[k]);
+            if (there) store_row<TU, VW, EVEN>(A.du, base, group, A.D, at, u);
         } else if (tpr > 64) __syncthreads();                  // (without u a row has one exchange: its buffer is free again behind this)
     }
     // a workgroup's column sums: rows side by side in it are folded through LDS first
@@ -283,22 +275,18 @@ __global__ __launch_bounds__(THREADS) void k_norm_backward(NormArgs A) {
         if (groups > 1) {
             __syncthreads();
 #pragma unroll
-            for (int k = 0; k < kCols; ++k) fold[k * 256 + threadIdx.x] = sums[n][k];
+            for (int k = 0; k < VW; ++k) fold[k * 256 + threadIdx.x] = sums[n][k];
             __syncthreads();
             if (group == 0)
 #pragma unroll
-                for (int k = 0; k < kCols; ++k)
+                for (int k = 0; k < VW; ++k)
                     for (int o = 1; o < groups; ++o) sums[n][k] += fold[k * 256 + o * tpr + threadIdx.x];
         }
         if (group == 0) {
-            float* to = A.part + ((int64_t)blockIdx.x * 3 + n) * A.D;
+            float* to = A.part + ((int64_t)blockIdx.x * 3 + n) * A.D + at.first;
 #pragma unroll
-            for (int j = 0; j < kCols / VW; ++j)
-#pragma unroll
-                for (int k = 0; k < VW; ++k) {
-                    const int c = column<VW>(tpr, j) + k;
-                    if (c < A.D) to[c] = sums[n][j * VW + k];
-                }
+            for (int k = 0; k < VW; ++k)
+                if (EVEN || k >= at.skip) to[k] = sums[n][k];
         }
     }
 }
@@ -323,7 +311,7 @@ __global__ __launch_bounds__(1024) void k_column_sums(const float* part, int blo
 }
 
 int row_threads(int64_t width) {
-    int tpr = 4;
+    int tpr = width < kCols ? 8 : 4;       // (less than eight columns: a thread each)
     while (tpr * kCols < width) tpr *= 2;
     return tpr;
 }
@@ -365,29 +353,26 @@ int check(const plmpm_norm* n, bool backward) {
     return 0;
 }
 
-// columns an access: 8 (16 bytes of a 16-bit type), 2, or 1, by what widths, pointers and strides keep to
-int vector_of(const plmpm_norm* n, bool backward) {
+// whether everything keeps to accesses of 16 bytes
+bool keeps_to_16(const plmpm_norm* n, bool backward) {
     const int zx = dtype_size(n->x_dtype), zu = dtype_size(n->u_dtype), zw = dtype_size(n->w_dtype);
-    for (int vw : {8, 2}) {
-        bool ok = n->width % vw == 0;
-        const auto keeps = [&](const void* p, int64_t stride, int size) { if (p) ok = ok && aligned_to(p, stride, size) >= std::min(16, vw * size); };
-        keeps(n->x, n->stride_x, zx);
-        keeps(n->u, n->stride_u, zu);
-        keeps(n->gate, n->stride_gate, zu);
-        for (const void* p : {n->scale, n->post, n->pre}) keeps(p, n->width, zw);
-        if (backward) {
-            keeps(n->dy, n->stride_dy, zx);
-            keeps(n->dz, n->stride_dz, zu);
-            keeps(n->dx, n->width, zx);
-            keeps(n->du, n->width, zu);
-            keeps(n->dgate, n->width, zu);
-        } else {
-            keeps(n->y, n->width, zx);
-            keeps(n->z, n->width, zu);
-        }
-        if (ok) return vw;
+    bool ok = true;
+    const auto keeps = [&](const void* p, int64_t stride, int size) { if (p) ok = ok && aligned_to(p, stride, size) >= 16; };
+    keeps(n->x, n->stride_x, zx);
+    keeps(n->u, n->stride_u, zu);
+    keeps(n->gate, n->stride_gate, zu);
+    for (const void* p : {n->scale, n->post, n->pre}) keeps(p, 0, zw);
+    if (backward) {
+        keeps(n->dy, n->stride_dy, zx);
+        keeps(n->dz, n->stride_dz, zu);
+        keeps(n->dx, n->width, zx);
+        keeps(n->du, n->width, zu);
+        keeps(n->dgate, n->width, zu);
+    } else {
+        keeps(n->y, n->width, zx);
+        keeps(n->z, n->width, zu);
     }
-    return 1;
+    return ok;
 }
 
 template <class TX, class TU, int VW, bool ALL, bool EVEN> void launch(const NormArgs& A, bool backward, int blocks, hipStream_t st) {
@@ -396,17 +381,13 @@ template <class TX, class TU, int VW, bool ALL, bool EVEN> void launch(const Nor
     else if (A.tpr == 1024) hipLaunchKernelGGL((k_norm_backward<TX, TU, VW, 1024, ALL, EVEN>), grid, block, 0, st, A);
     else hipLaunchKernelGGL((k_norm_backward<TX, TU, VW, 512, ALL, EVEN>), grid, block, 0, st, A);
 }
-template <class TX, class TU, int VW> void launch(const NormArgs& A, bool backward, int blocks, hipStream_t st) {
+template <class TX, class TU> void launch(const NormArgs& A, bool even, bool backward, int blocks, hipStream_t st) {
     const bool all = A.u && A.gate && A.scale && A.post && A.pre && (backward ? A.dy && A.dz : A.y && A.z);
-    const bool even = VW == 8 && A.D == A.tpr * kCols && A.rows % (block_of(A.tpr) / A.tpr) == 0;
-    if (VW == 8 && all && even) launch<TX, TU, 8, true, true>(A, backward, blocks, st);
-    else if (all) launch<TX, TU, VW, true, false>(A, backward, blocks, st);
-    else launch<TX, TU, VW, false, false>(A, backward, blocks, st);
-}
-template <class TX, class TU> void launch(const NormArgs& A, int vw, bool backward, int blocks, hipStream_t st) {
-    if (vw == 8) launch<TX, TU, 8>(A, backward, blocks, st);
-    else if (vw == 2) launch<TX, TU, 2>(A, backward, blocks, st);
-    else launch<TX, TU, 1>(A, backward, blocks, st);
+    even = even && A.D == A.tpr * kCols && A.rows % (block_of(A.tpr) / A.tpr) == 0;
+    if (A.D < kCols) launch<TX, TU, 1, false, false>(A, backward, blocks, st);
+    else if (all && even) launch<TX, TU, kCols, true, true>(A, backward, blocks, st);
+    else if (all) launch<TX, TU, kCols, true, false>(A, backward, blocks, st);
+    else launch<TX, TU, kCols, false, false>(A, backward, blocks, st);
 }
 
 int run(const plmpm_norm* n, bool backward, hipStream_t st) {
@@ -422,13 +403,14 @@ int run(const plmpm_norm* n, bool backward, hipStream_t st) {
     A.rows = n->rows; A.sx = n->stride_x; A.su = n->stride_u; A.sg = n->stride_gate; A.sdy = n->stride_dy; A.sdz = n->stride_dz;
     A.D = (int)n->width; A.fn = n->gate_fn; A.wt = n->w_dtype; A.eps = (float)n->eps;
     A.tpr = row_threads(n->width);
-    const int vw = vector_of(n, backward), blocks = blocks_of(n, backward);
+    const bool even = keeps_to_16(n, backward);
+    const int blocks = blocks_of(n, backward);
     if (blocks) {
-        if (n->x_dtype == PLMPM_NN_BF16) launch<bf16, bf16>(A, vw, backward, blocks, st);
-        else if (n->x_dtype == PLMPM_NN_F16) launch<f16, f16>(A, vw, backward, blocks, st);
-        else if (n->u_dtype == PLMPM_NN_F32) launch<float, float>(A, vw, backward, blocks, st);
-        else if (n->u_dtype == PLMPM_NN_BF16) launch<float, bf16>(A, vw, backward, blocks, st);
-        else launch<float, f16>(A, vw, backward, blocks, st);
+        if (n->x_dtype == PLMPM_NN_BF16) launch<bf16, bf16>(A, even, backward, blocks, st);
+        else if (n->x_dtype == PLMPM_NN_F16) launch<f16, f16>(A, even, backward, blocks, st);
+        else if (n->u_dtype == PLMPM_NN_F32) launch<float, float>(A, even, backward, blocks, st);
+        else if (n->u_dtype == PLMPM_NN_BF16) launch<float, bf16>(A, even, backward, blocks, st);
+        else launch<float, f16>(A, even, backward, blocks, st);
     }
     if (backward && (n->dscale || n->dpost || n->dpre))      // (without rows the weights' gradients are zeros)
         hipLaunchKernelGGL(k_column_sums, dim3((unsigned)((A.D + 63) / 64), 3), dim3(1024), 0, st, (const float*)A.part, blocks, A.D, n->dscale, n->dpost, n->dpre, A.wt);

@@ -63,7 +63,8 @@ def test_scan_step(interpreter):
 
 @pytest.mark.parametrize("shape,tx,tu,fn,strided", [
     ((3, 8), "f32", "f32", "sigmoid", False), ((2, 5, 33), "bf16", "bf16", "silu", False), ((9, 130), "f32", "f16", "identity", True),
-    ((5, 520), "f16", "f16", "sigmoid", True), ((2, 2050), "f32", "bf16", "silu", False), ((70, 1), "f32", "f32", "sigmoid", False)])
+    ((5, 520), "f16", "f16", "sigmoid", True), ((2, 2050), "f32", "bf16", "silu", False), ((70, 1), "f32", "f32", "sigmoid", False),
+    ((5, 9), "f16", "f16", "silu", True), ((3, 71), "f32", "bf16", "identity", False), ((2, 7), "bf16", "bf16", "sigmoid", False)])
 def test_norm(interpreter, shape, tx, tu, fn, strided):
     cases.run_norm(interpreter, 21, shape, tx, tu, fn, strided=strided)
 

@@ -38,7 +38,7 @@ def test_scan_step(dtype):
 
 @pytest.mark.parametrize("tx,tu", [("f32", "f32"), ("f32", "bf16"), ("f32", "f16"), ("bf16", "bf16"), ("f16", "f16")])
 @pytest.mark.parametrize("shape,fn,strided", [((1, 1), "sigmoid", False), ((3, 8), "sigmoid", False), ((2, 5, 33), "silu", False), ((9, 130), "identity", True),
-                                              ((700, 64), "sigmoid", False), ((33, 1214), "silu", False), ((17, 4096), "sigmoid", True), ((5, 8192), "silu", False),
+                                              ((700, 64), "sigmoid", False), ((33, 1214), "silu", False), ((5, 9), "silu", True), ((300, 7), "sigmoid", False), ((17, 4096), "sigmoid", True), ((5, 8192), "silu", False),
                                               ((3, 8191), "sigmoid", False), ((1200, 520), "sigmoid", True)])
 def test_norm(shape, tx, tu, fn, strided):
     print(cases.run_norm(DEV, 21, shape, tx, tu, fn, strided=strided))
