@@ -31,8 +31,8 @@ struct Table {
     int32_t count, per;                 // tensors; chunks a workgroup
 };
 struct Step {
-    float decay, lr, b1, b2, c1, c2, eps, max_norm, lo, hi;      // decay = lr * weight_decay; c = 1 - b
-    double beta_1, beta_2, lr64;
+    float decay, b1, b2, c1, c2, eps, lo, hi;      // decay = lr * weight_decay; c = 1 - b
+    double beta_1, beta_2, lr, max_norm;
     int64_t* step;
     float* grad_norm;
     const double* partial;              // sums of squares, or null
@@ -300,11 +300,11 @@ template <class T, int BITS> __device__ __forceinline__ void chunk_step(const St
 template <int BITS> __global__ __launch_bounds__(kThreads) void k_adamw(Table tab, Step S) {
     __shared__ double lds[kThreads / 64];
     const int64_t t = S.step[1];
-    Now N{1.0f, (float)(S.lr64 / (1.0 - power(S.beta_1, t))), (float)(1.0 / sqrt(1.0 - power(S.beta_2, t)))};
+    Now N{1.0f, (float)(S.lr / (1.0 - power(S.beta_1, t))), (float)(1.0 / sqrt(1.0 - power(S.beta_2, t)))};
     if (S.partial) {
         double sum = 0.0;
         for (int k = threadIdx.x; k < S.partials; k += kThreads) sum += S.partial[k];
-        const double norm = sqrt(block_sum(sum, lds)), ratio = (double)S.max_norm / norm;
+        const double norm = sqrt(block_sum(sum, lds)), ratio = S.max_norm / norm;
         N.k = (float)(ratio > 1.0 ? 1.0 : ratio);              // (norm 0: ratio inf -> 1; a NaN norm stays one)
         if (S.grad_norm && S.last && blockIdx.x == 0 && threadIdx.x == 0) *S.grad_norm = (float)norm;
     }
@@ -367,7 +367,7 @@ int check(const plmpm_adamw* a, const plmpm_adamw_tensor* tensors, int count) {
         const int size = dtype_size(t.dtype);
         NN_REQUIRE(t.p && t.g && t.m && t.v && (state == 4 || (t.m_scale && t.v_scale)), "adamw: tensor %d has a null pointer", k);
         NN_REQUIRE(!t.master || t.dtype != PLMPM_NN_F32, "adamw: tensor %d: a master copy goes with 16-bit parameters", k);
-        NN_REQUIRE(((uintptr_t)t.p | (uintptr_t)t.g) % size == 0 && ((uintptr_t)t.m | (uintptr_t)t.v) % state == 0 && (uintptr_t)t.master % 4 == 0,
+        NN_REQUIRE(((uintptr_t)t.p | (uintptr_t)t.g) % size == 0 && ((uintptr_t)t.m | (uintptr_t)t.v) % state == 0 && ((uintptr_t)t.master | (uintptr_t)t.m_scale | (uintptr_t)t.v_scale) % 4 == 0,
                    "adamw: tensor %d: a pointer is not aligned to its type", k);
         total += chunks_of(t.n);
         NN_REQUIRE(total < (1 << 30), "adamw: too many elements for one call");
@@ -437,8 +437,8 @@ int plmpm_adamw_step(const plmpm_adamw* a, const plmpm_adamw_tensor* tensors, in
     Step S{};
     S.decay = (float)(a->lr * a->weight_decay);
     S.b1 = (float)a->beta_1; S.b2 = (float)a->beta_2; S.c1 = (float)(1.0 - a->beta_1); S.c2 = (float)(1.0 - a->beta_2);
-    S.eps = (float)a->epsilon; S.max_norm = (float)a->max_norm; S.lo = (float)a->lo; S.hi = (float)a->hi;
-    S.beta_1 = a->beta_1; S.beta_2 = a->beta_2; S.lr64 = a->lr;
+    S.eps = (float)a->epsilon; S.lo = (float)a->lo; S.hi = (float)a->hi;
+    S.beta_1 = a->beta_1; S.beta_2 = a->beta_2; S.lr = a->lr; S.max_norm = a->max_norm;
     S.step = a->step; S.grad_norm = a->grad_norm;
     S.partial = a->max_norm > 0 ? partial : nullptr;
     S.partials = partials;

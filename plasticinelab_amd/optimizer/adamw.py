@@ -51,6 +51,7 @@ def adamw_step(params, grads, first, second, step, *, lr=1e-3, beta_1=0.9, beta_
     the start.  masters: for each parameter a float32 copy that is updated in its place, the parameter being its rounding, or None; without one
     a 16-bit parameter is itself updated in float32 and rounded, and loses updates below its last bit.  step: int64 (2,) on the GPU, zeros at the
     start: the updates done, and those begun.  lr and the other numbers are fixed in a captured graph; the count is not.
+    No tensor may be in the list twice.  A call without any gradient does nothing.
     A gradient that is not finite makes its element's moments and weight not finite (with max_norm: all of them).
     """
     count = len(params)
@@ -60,7 +61,7 @@ def adamw_step(params, grads, first, second, step, *, lr=1e-3, beta_1=0.9, beta_
         P._refuse("step has to be an int64 tensor of two values")
     where = step.get_device()
     bits = 8 if count and isinstance(first[0], (tuple, list)) else 32
-    flat, keep, touched, total, codes, f32 = [], [], [], 0, P.DTYPES, torch.float32
+    flat, keep, touched, codes, f32 = [], [], [], P.DTYPES, torch.float32
     for k in range(count):
         g = grads[k]
         if g is None:
@@ -89,21 +90,28 @@ def adamw_step(params, grads, first, second, step, *, lr=1e-3, beta_1=0.9, beta_
             if dtype == f32:
                 P._refuse(f"parameter {k} is float32: a master copy goes with 16 bits")
             w = _plain(masters[k], n, where, "a master")
-        flat += (p.data_ptr(), g.data_ptr(), m, v, ms, vs, w, n, codes[dtype], 0)
-        touched.append(p)
-        total += n
+        if n:
+            flat += (p.data_ptr(), g.data_ptr(), m, v, ms, vs, w, n, codes[dtype], 0)
+            touched.append(p)
     norm = torch.empty((), dtype=torch.float32, device=step.device) if max_norm > 0 else None
-    if not total:
+    live = len(touched)
+    if not live:
         return None if norm is None else norm.zero_()
+    if len(set(flat[0::10])) < live or len(set(flat[2::10])) < live or len(set(flat[3::10])) < live:
+        P._refuse("a parameter, or a moment of it, is in the list twice: the updates would race")
     a = L.AdamWStep(bits, 0, lr, beta_1, beta_2, epsilon, weight_decay, max_norm, bounds[0], bounds[1], step.data_ptr(), P._ptr(norm))
-    live, table = len(touched), struct.pack("=" + "8q2i" * len(touched), *flat)
+    table = struct.pack("=" + "8q2i" * live, *flat)
     lib, need = P._library(), C.c_size_t()
     L.check(lib.plmpm_adamw_workspace(a, table, live, need), lib)
     if need.value:
         work = torch.empty(need.value, dtype=torch.uint8, device=step.device)
         a.workspace, a.workspace_bytes = work.data_ptr(), need.value
     P._call("plmpm_adamw_step", step, a, table, live)
-    torch.autograd.graph.increment_version(touched)         # (a graph that saved a parameter notices that it changed)
+    try:
+        torch.autograd.graph.increment_version(touched)     # (a graph that saved a parameter notices that it changed)
+    except RuntimeError:                                    # (tensors of inference mode among them)
+        for p in touched:
+            P._written(p)
     return norm
 
 

@@ -81,6 +81,12 @@ def _tracked(*ts):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
+def _written(t):
+    """A tensor was changed in place: a graph that saved it has to notice (tensors of inference mode are in none)."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 def _rows(t):
     """Unit stride over the last dimension (a copy if need be)."""
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
@@ -214,7 +220,7 @@ def gated_scan_step(x, r, i, decay, state, *, c: float = 8.0):
         s = L.Scan(DTYPES[x.dtype], 0, B, 1, D, (x.stride(0), r.stride(0), i.stride(0)), (0, 0, 0), c, x.data_ptr(), r.data_ptr(), i.data_ptr(), decay.data_ptr(), p, None,
                    h.data_ptr(), p)
         _call("plmpm_scan_forward", x, s)           # (a single step needs no workspace)
-        torch.autograd.graph.increment_version(state)
+        _written(state)
     return h
 
 

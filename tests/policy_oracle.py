@@ -203,7 +203,7 @@ def adamw(w, g, m, v, t, norm=None, lr=1e-3, beta_1=0.9, beta_2=0.999, epsilon=1
     """One update of one tensor in float32, each operation rounded by itself -> (w, m, v).  norm: of all tensors' gradients, in float64."""
     g = g.astype(F)
     if max_norm > 0:
-        g = g * F(min(1.0, float(F(max_norm)) / norm if norm else 1.0))
+        g = g * F(min(1.0, max_norm / norm if norm else 1.0))
     m = F(beta_1) * m + F(1 - beta_1) * g
     v = F(beta_2) * v + F(1 - beta_2) * (g * g)
     den = np.sqrt(v) * F(1.0 / np.sqrt(1 - beta_2 ** t)) + F(epsilon)

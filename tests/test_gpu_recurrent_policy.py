@@ -184,3 +184,15 @@ def test_policy_refusals():
         policy.step(torch.zeros(4, device=DEV), policy.initial_state(1))
     with pytest.raises(ValueError, match="float32"):
         RecurrentPolicy(4, 2, width=8).double()(torch.zeros(1, 2, 4, device=DEV))
+
+
+def test_act_in_inference_mode():
+    policy = RecurrentPolicy(9, 4, width=24, depth=2)
+    obs = torch.randn(5, 3, 9, device=DEV)
+    with torch.no_grad():
+        want, end = policy(obs)
+    with torch.inference_mode():
+        state = policy.initial_state(5)
+        got = torch.stack([policy.act(obs[:, t], state) for t in range(3)], 1)
+        again, last = policy(obs)
+    assert off(got, want) < TOL and off(state, end) < TOL and torch.equal(again, want) and torch.equal(last, end)

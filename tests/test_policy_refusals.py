@@ -60,6 +60,9 @@ def test_adamw_refusals():
             (([p.half()], [p.half()], [z()], [z()], step), {"masters": [z(5)]}, "master")):
         with pytest.raises(ValueError, match=text):
             adamw_step(*args, **kw)
+    for args in (([p, p], [p, p], [z(), z()], [z(), z()], step), ([p, z()], [p, p], [m8[0].float()] * 2, [z(), z()], step)):
+        with pytest.raises(ValueError, match="twice"):
+            adamw_step(*args)
     for entry, text in (((z(), z(2)), "int8 or uint8"), ((z(300, torch.int8), z(3)), "scales")):
         with pytest.raises(ValueError, match=text):
             adamw_values([entry])
