@@ -6,34 +6,32 @@ tensors that the caller keeps; ``adamw_values`` reads 8-bit moments back.
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
-import struct
 
 import numpy as np
 import torch
 
-from .. import _lib as L
 from .. import policy as P
 from .optim import Optimizer
 
 BLOCK = 256                             # elements that share a scale where moments are held in 8 bits
 
 
-def _pair(entry, n, where, codes_dtype, name):
-    """-> the addresses of a moment's codes and scales."""
-    codes, scales = entry
-    if codes.dtype != codes_dtype or codes.numel() != n or not codes.is_contiguous() or codes.get_device() != where:
-        P._refuse(f"{name}: codes have to be {n} contiguous {codes_dtype} values on the parameters' device")
-    if scales.dtype != torch.float32 or scales.numel() != -(-n // BLOCK) or not scales.is_contiguous() or scales.get_device() != where:
-        P._refuse(f"{name}: scales have to be {-(-n // BLOCK)} contiguous float32 values on the parameters' device")
-    return codes.data_ptr(), scales.data_ptr()
+def _split(moments, what):
+    """-> the lists of codes and of scales of a list of (codes, scales) pairs."""
+    for k, entry in enumerate(moments):
+        if not isinstance(entry, (tuple, list)) or len(entry) != 2:
+            P._refuse(f"{what} {k}: all moments have 32 bits, or all have 8 and are pairs of codes and scales")
+    return [entry[0] for entry in moments], [entry[1] for entry in moments]
 
 
-def _plain(t, n, where, name):
-    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous() or t.get_device() != where:
-        P._refuse(f"{name} has to be {n} contiguous float32 values on the parameters' device")
-    return t.data_ptr()
+def _not_tensors(optional=(), **lists):
+    """Called for a TypeError of the binding: a ValueError that names the first entry which is no tensor, if that was it."""
+    for name, entries in lists.items():
+        for k, t in enumerate(entries):
+            if isinstance(t, (tuple, list)):
+                raise ValueError(f"{name} {k}: all moments have 32 bits, or all have 8") from None
+            P._not_tensors((f"{name} {k}",) if name in optional else (), **{f"{name} {k}": t})
 
 
 def adamw_step(params, grads, first, second, step, *, lr=1e-3, beta_1=0.9, beta_2=0.999, epsilon=1e-8, weight_decay=0.01, max_norm=0.0,
@@ -54,92 +52,35 @@ def adamw_step(params, grads, first, second, step, *, lr=1e-3, beta_1=0.9, beta_
     No tensor may be in the list twice.  A call without any gradient does nothing.
     A gradient that is not finite makes its element's moments and weight not finite (with max_norm: all of them).
     """
-    count = len(params)
-    if not len(grads) == len(first) == len(second) == count or (masters is not None and len(masters) != count):
+    bits, first_scales, second_scales = 32, [], []
+    if len(first) and isinstance(first[0], (tuple, list)):
+        bits = 8
+        (first, first_scales), (second, second_scales) = _split(first, "first moment"), _split(second, "second moment")
+    if masters is None:
+        masters = []
+    elif len(masters) != len(params):
         P._refuse("params, grads, first, second and masters have to be of one length")
-    if not isinstance(step, torch.Tensor) or step.shape != (2,) or step.dtype != torch.int64 or not step.is_contiguous():
-        P._refuse("step has to be an int64 tensor of two values")
-    where = step.get_device()
-    bits = 8 if count and isinstance(first[0], (tuple, list)) else 32
-    flat, keep, touched, codes, f32 = [], [], [], P.DTYPES, torch.float32
-    for k in range(count):
-        g = grads[k]
-        if g is None:
-            continue
-        p, m, v, ms, vs, w = params[k], first[k], second[k], 0, 0, 0
-        n, dtype = p.numel(), p.dtype
-        if dtype not in codes or not p.is_contiguous() or p.get_device() != where:
-            P._refuse(f"parameter {k} has to be a contiguous float32, bfloat16 or float16 tensor on {step.device}")
-        if g.dtype != dtype or not g.is_same_size(p) or g.get_device() != where:
-            P._refuse(f"gradient {k} has to match its parameter: {tuple(p.shape)} {dtype} on {step.device}")
-        if not g.is_contiguous():
-            g = g.contiguous()
-            keep.append(g)
-        if isinstance(m, (tuple, list)) != (bits == 8) or isinstance(v, (tuple, list)) != (bits == 8):
-            P._refuse(f"moments of parameter {k}: all moments have 32 bits, or all have 8")
-        if bits == 8:
-            m, ms = _pair(m, n, where, torch.int8, f"first moment {k}")
-            v, vs = _pair(v, n, where, torch.uint8, f"second moment {k}")
-        else:
-            if (m.dtype != f32 or v.dtype != f32 or m.numel() != n or v.numel() != n or not m.is_contiguous() or not v.is_contiguous()
-                    or m.get_device() != where or v.get_device() != where):
-                _plain(m, n, where, "a first moment")
-                _plain(v, n, where, "a second moment")
-            m, v = m.data_ptr(), v.data_ptr()
-        if masters is not None and masters[k] is not None:
-            if dtype == f32:
-                P._refuse(f"parameter {k} is float32: a master copy goes with 16 bits")
-            w = _plain(masters[k], n, where, "a master")
-        if n:
-            flat += (p.data_ptr(), g.data_ptr(), m, v, ms, vs, w, n, codes[dtype], 0)
-            touched.append(p)
-    norm = torch.empty((), dtype=torch.float32, device=step.device) if max_norm > 0 else None
-    live = len(touched)
-    if not live:
-        return None if norm is None else norm.zero_()
-    if len(set(flat[0::10])) < live or len(set(flat[2::10])) < live or len(set(flat[3::10])) < live:
-        P._refuse("a parameter, or a moment of it, is in the list twice: the updates would race")
-    a = L.AdamWStep(bits, 0, lr, beta_1, beta_2, epsilon, weight_decay, max_norm, bounds[0], bounds[1], step.data_ptr(), P._ptr(norm))
-    table = struct.pack("=" + "8q2i" * live, *flat)
-    lib, need = P._library(), C.c_size_t()
-    L.check(lib.plmpm_adamw_workspace(a, table, live, need), lib)
-    if need.value:
-        work = torch.empty(need.value, dtype=torch.uint8, device=step.device)
-        a.workspace, a.workspace_bytes = work.data_ptr(), need.value
-    P._call("plmpm_adamw_step", step, a, table, live)
     try:
-        torch.autograd.graph.increment_version(touched)     # (a graph that saved a parameter notices that it changed)
-    except RuntimeError:                                    # (tensors of inference mode among them)
-        for p in touched:
-            P._written(p)
-    return norm
+        return P._binding().adamw_step(params, grads, first, second, first_scales, second_scales, masters, step, bits, lr, beta_1, beta_2, epsilon, weight_decay, max_norm,
+                                       bounds[0], bounds[1])
+    except TypeError:
+        _not_tensors(("gradient", "master"), **{"parameter": params, "gradient": grads, "first moment": first, "second moment": second, "scales of first moment": first_scales,
+                                                "scales of second moment": second_scales, "master": masters})
+        P._not_tensors(step=step)
+        raise
 
 
 def adamw_values(moments, out=None):
     """The float32 values that 8-bit moments stand for: ``moments`` a list of (codes, scales) pairs, int8 codes for first moments and uint8 for
     second; -> ``out``, a list of float32 tensors of the codes' sizes (made if None)."""
-    moments = list(moments)
+    codes, scales = _split(list(moments), "moment")
     if out is None:
-        out = [torch.empty(codes.shape, dtype=torch.float32, device=codes.device) for codes, _ in moments]
-    n = len(moments)
-    if len(out) != n:
-        P._refuse("out has to have a tensor for each moment")
-    if not n:
-        return out
-    where = moments[0][0].get_device()
-    codes, scales, values, sizes, which = [], [], [], [], []
-    for k, (entry, o) in enumerate(zip(moments, out)):
-        dtype, size = entry[0].dtype, entry[0].numel()
-        if dtype not in (torch.int8, torch.uint8):
-            P._refuse(f"moment {k}: codes have to be int8 or uint8, got {dtype}")
-        c, s = _pair(entry, size, where, dtype, f"moment {k}")
-        codes.append(c)
-        scales.append(s)
-        values.append(_plain(o, size, where, f"out {k}"))
-        sizes.append(size)
-        which.append(int(dtype == torch.uint8))
-    pack = lambda code, xs: struct.pack(f"={n}{code}", *xs)         # noqa: E731
-    P._call("plmpm_adamw_values", moments[0][0], pack("q", codes), pack("q", scales), pack("q", values), pack("q", sizes), pack("i", which), n)
+        out = [torch.empty(t.shape, dtype=torch.float32, device=t.device) for t in codes]
+    try:
+        P._binding().adamw_values(codes, scales, out)
+    except TypeError:
+        _not_tensors(codes=codes, scales=scales, out=out)
+        raise
     return out
 
 
@@ -159,7 +100,7 @@ class AdamW(Optimizer):
         if self.cfg.state_bits not in (8, 32):
             P._refuse(f"state_bits has to be 32 or 8, got {self.cfg.state_bits}")
         device = self.parameters[0].device
-        P._site(self.parameters[0])                      # a GPU's, or refused
+        P._binding().require_device(self.parameters[0])  # a GPU's, or refused
         for k, p in enumerate(self.parameters):
             if p.dtype not in P.DTYPES or not p.is_contiguous() or p.device != device:
                 P._refuse(f"parameter {k} has to be a contiguous float32, bfloat16 or float16 tensor on {device}")

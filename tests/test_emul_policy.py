@@ -28,11 +28,10 @@ def interpreter():
                            "HDRS=" + " ".join(os.path.join("../../plasticinelab_amd/csrc", h) for h in ("plmpm_nn.h", "plmpm_kernels.h")) + " ../../include/plmpm_policy.h",
                            "SRCS=" + SOURCES, out])
     lib = _lib.bind(C.CDLL(os.path.join(HERE, out)), {**_lib.POLICY_SYMBOLS, "plmpm_last_error": _lib.SYMBOLS["plmpm_last_error"]})
-    patch = pytest.MonkeyPatch()
-    patch.setattr(P, "_library", lambda: lib)
-    patch.setattr(P, "_site", lambda t: (0, None))
+    binding = P._binding()
+    P._attach(binding, lib, host=True)
     yield "cpu"
-    patch.undo()
+    P._attach(binding, _lib.load_policy())
 
 
 def test_policy_header_and_binding_agree():
@@ -102,3 +101,52 @@ def test_numbers_out_of_range_are_refused_at_the_c_entry(interpreter):
         with pytest.raises(_lib.EngineError, match=text):
             adamw_step([p], [p], z(), z(), step, **kw)
     assert float(p.abs().sum()) == 0 and step.tolist() == [0, 0]
+
+
+def leaves(*shapes):
+    gen = torch.Generator().manual_seed(3)
+    return [torch.randn(shape, generator=gen).requires_grad_() for shape in shapes]
+
+
+def test_second_derivatives_are_refused(interpreter):
+    x, r, i, decay = leaves((2, 7, 8), (2, 7, 8), (2, 7, 8), (8,))
+    for value, name in ((P.gated_scan(x, r, i, decay)[0], "gated_scan"), (P.block_norm(x, pre=decay)[1], "block_norm")):
+        grad, = torch.autograd.grad(value.square().sum(), [x], create_graph=True)
+        with pytest.raises(RuntimeError, match=f"{name} has no second derivative"):
+            grad.sum().backward()
+
+
+def test_a_saved_tensor_that_was_changed_is_noticed(interpreter):
+    x, r, i, decay = leaves((2, 7, 8), (2, 7, 8), (2, 7, 8), (8,))
+    for value in (P.gated_scan(x, r, i, decay)[0], P.block_norm(x, r, post=decay)[0]):
+        with torch.no_grad():
+            decay.add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            value.sum().backward()
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_under_activation_checkpointing(interpreter, reentrant):
+    from torch.utils.checkpoint import checkpoint
+    args = leaves((2, 70, 8), (2, 70, 8), (2, 70, 8), (8,), (2, 8))
+
+    def run(x, r, i, decay, h0):
+        return P.block_norm(P.gated_scan(x, r, i, decay, h0)[0], r, i, decay, decay, decay, gate_fn="silu")[1]
+
+    run(*args).square().sum().backward()
+    want = [t.grad.clone() for t in args]
+    for t in args:
+        t.grad = None
+    checkpoint(run, *args, use_reentrant=reentrant).square().sum().backward()
+    assert all(torch.equal(t.grad, w) for t, w in zip(args, want))
+
+
+def test_only_the_gradients_that_are_asked_for(interpreter):
+    x, r, i, decay = leaves((2, 7, 8), (2, 7, 8), (2, 7, 8), (8,))
+    full = torch.autograd.grad(P.gated_scan(x, r, i, decay)[1].sum(), [x, r, i, decay])
+    h, last = P.gated_scan(x.detach(), r.detach(), i.detach(), decay)
+    assert torch.equal(torch.autograd.grad(last.sum(), [decay])[0], full[3])
+    y, z = P.block_norm(x, r, pre=decay)
+    assert [t is None for t in torch.autograd.grad(y.sum(), [x, r, decay], allow_unused=True, retain_graph=True)] == [False] * 3
+    assert torch.equal(torch.autograd.grad(y.sum(), [x], retain_graph=True)[0], torch.ones_like(x))
+    assert P.block_norm(x, pre=decay)[0] is x

@@ -76,6 +76,19 @@ def test_adamw_refusals():
         AdamW([])
 
 
+def test_what_is_no_tensor_is_named():
+    x, r, i, decay = tensors()
+    p, step = torch.zeros(300), torch.zeros(2, dtype=torch.int64)
+    for call, text in ((lambda: P.gated_scan(x, r, i, decay, 3), "h0 has to be a tensor"), (lambda: P.gated_scan(None, r, i, decay), "x has to be a tensor, got NoneType"),
+                       (lambda: P.gated_scan_step(x[:, 0], r[:, 0], i[:, 0], decay, None), "state has to be a tensor"), (lambda: P.block_norm(x, 1.0), "u has to be a tensor"),
+                       (lambda: adamw_step([p], [0.0], [p], [p], step), "gradient 0 has to be a tensor"), (lambda: adamw_step([p], [p], [p], [p], None), "step has to be a tensor"),
+                       (lambda: adamw_step([p], [p], [p], [(p, p)], step), "all have 8"), (lambda: adamw_values([p]), "pairs of codes and scales")):
+        with pytest.raises(ValueError, match=text):
+            call()
+    with pytest.raises(TypeError):
+        P.gated_scan(x, r, i, decay, c="8")
+
+
 def test_c_entries_check_before_they_launch():
     """Null pointers, sizes and alignments at the C entries of the library itself: a message and non-zero, nothing launched."""
     lib = _lib.load_policy()
