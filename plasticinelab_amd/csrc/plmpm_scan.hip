@@ -15,8 +15,8 @@
 // and publish before they wait -- the lowest unfinished ticket waits for nobody, so every wait ends.
 // The words and the ticket are cleared by a small kernel before each launch (not a memset node: calls may be captured).
 //
-// A reset makes the run forget what came before, also a NaN: its A is then -0 (every genuine A is +0 or above), and whoever
-// composes runs takes H alone where the sign is set.
+// A reset makes the run forget what came before, also a NaN (and, backward, what comes behind it): its A is then -0, whatever its other steps
+// are (every genuine A is +0 or above), and whoever composes runs takes H alone where the sign is set.
 #include <algorithm>
 #include <type_traits>
 
@@ -193,10 +193,8 @@ __global__ __launch_bounds__(W * 64) void k_scan_forward(ScanArgs A) {
                 const Gates g = gates(r[v], i[v], k2[v]);
                 a[s][v] = there ? g.a : 1.0f;
                 u[s][v] = g.si * x[v];
-                if (RESET && (cut >> s & 1)) {
-                    PA[v] = -0.0f;
-                    PH[v] = u[s][v];
-                } else {
+                if (RESET && (cut >> s & 1)) PH[v] = u[s][v];
+                else {
                     u[s][v] = there ? u[s][v] * __builtin_amdgcn_sqrtf(g.m2) : 0.0f;
                     PA[v] *= a[s][v];
                     PH[v] = fmaf(a[s][v], PH[v], u[s][v]);
@@ -207,7 +205,7 @@ __global__ __launch_bounds__(W * 64) void k_scan_forward(ScanArgs A) {
     if (left == S) walk(std::true_type());
     else walk(std::false_type());
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) { sA[wave][lane * VEC + v] = PA[v]; sH[wave][lane * VEC + v] = PH[v]; }
+    for (int v = 0; v < VEC; ++v) { sA[wave][lane * VEC + v] = RESET && cut ? -0.0f : PA[v]; sH[wave][lane * VEC + v] = PH[v]; }
     __syncthreads();
     for (int ch = threadIdx.x; ch < NCH; ch += blockDim.x) {
         if (first + ch >= A.D) continue;
@@ -348,7 +346,6 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
                 if (RESET && (cut >> s & 1)) {
                     a[s][v] = 0.0f;
                     m[s][v] = 1.0f;
-                    PA[v] = -0.0f;
                     PH[v] = g.si * x[v];
                 } else {
                     a[s][v] = there ? g.a : 1.0f;
@@ -370,7 +367,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
     }
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-        sA[wave][lane * VEC + v] = PA[v];
+        sA[wave][lane * VEC + v] = RESET && cut ? -0.0f : PA[v];
         sH[wave][lane * VEC + v] = PH[v];
         sE[wave][lane * VEC + v] = PE[v];
     }
@@ -440,7 +437,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
             dx[v] = g[v] * m[s][v] * si[s][v];
             const float gu = dx[v] * x[v];
             di[v] = fmaf(-gu, si[s][v], gu);
-            const float q = reset ? 0.0f : g[v] * pull[s][v] * sr[s][v];
+            const float q = reset || s >= left ? 0.0f : g[v] * pull[s][v] * sr[s][v];        // (behind the end: 0 times a state that may be infinite)
             dr[v] = q * (k2[v] * kLn2) * (1.0f - sr[s][v]);
             sum[v] += q;
         }
@@ -501,11 +498,13 @@ size_t word_bytes(const plmpm_scan* s, bool backward) {
 }
 size_t k2_bytes(const plmpm_scan* s, bool backward) { return tiles_of(s, backward) > 1 ? round_up(s->width * sizeof(float), 8) : 0; }
 
-template <class T, int VEC, bool RESET> void launch(const ScanArgs& A, bool backward, hipStream_t st) {
+// a workgroup: the waves of a tile, fewer where the steps end before
+unsigned threads_of(int64_t steps, bool backward) {
     const int S = backward ? kBackwardSteps : kForwardSteps, W = backward ? kBackwardWaves : kForwardWaves;
-    const int64_t need = (A.T + S - 1) / S;
-    const int waves = (int)(need < W ? need : W);
-    const dim3 grid((unsigned)(A.B * A.cblks * A.tiles)), block((unsigned)(waves * 64));
+    return 64u * (unsigned)std::min<int64_t>((steps + S - 1) / S, W);
+}
+template <class T, int VEC, bool RESET> void launch(const ScanArgs& A, bool backward, hipStream_t st) {
+    const dim3 grid((unsigned)(A.B * A.cblks * A.tiles)), block(threads_of(A.T, backward));
     if (backward) hipLaunchKernelGGL((k_scan_backward<T, VEC, kBackwardSteps, kBackwardWaves, RESET>), grid, block, 0, st, A);
     else hipLaunchKernelGGL((k_scan_forward<T, VEC, kForwardSteps, kForwardWaves, RESET>), grid, block, 0, st, A);
 }
@@ -548,7 +547,7 @@ int check(const plmpm_scan* s, bool backward, bool pointers) {
     NN_REQUIRE(s, "scan: null argument");
     NN_REQUIRE(s->dtype >= PLMPM_NN_F32 && s->dtype <= PLMPM_NN_F16, "scan: unknown dtype %d", s->dtype);
     NN_REQUIRE(s->batch >= 0 && s->steps >= 0 && s->width >= 0, "scan: negative size");
-    NN_REQUIRE(s->width < (1 << 30), "scan: width %lld is too large", (long long)s->width);
+    NN_REQUIRE(s->width < (1 << 27), "scan: width %lld is too large", (long long)s->width);
     NN_REQUIRE(s->steps < ((int64_t)1 << 36), "scan: %lld steps are too many", (long long)s->steps);
     NN_REQUIRE(s->batch < (1 << 30) && s->batch * ((s->width + 63) / 64) < ((int64_t)1 << 31) &&
                s->batch * ((s->width + 63) / 64) * ((s->steps + kCheckpoint - 1) / kCheckpoint) < ((int64_t)1 << 31), "scan: batch x width x steps is too large for one launch");
@@ -560,6 +559,8 @@ int check(const plmpm_scan* s, bool backward, bool pointers) {
     const int size = dtype_size(s->dtype);
     for (const void* p : {s->x, s->r, s->i, (const void*)s->h, s->dh, (const void*)s->dx, (const void*)s->dr, (const void*)s->di})
         NN_REQUIRE((uintptr_t)p % size == 0, "scan: a pointer is not aligned to its type");
+    for (const float* p : {s->decay, s->h0, (const float*)s->h_last, (const float*)s->checkpoint, s->dlast, (const float*)s->ddecay, (const float*)s->dh0})
+        NN_REQUIRE((uintptr_t)p % sizeof(float) == 0, "scan: a pointer is not aligned to its type");
     return 0;
 }
 
@@ -588,6 +589,7 @@ int run(const plmpm_scan* s, bool backward, hipStream_t st) {
     const int vec = vector_of(s, backward);
     A.cblks = (A.D + 64 * vec - 1) / (64 * vec);
     A.tiles = (int)tiles_of(s, backward);
+    NN_REQUIRE((uint64_t)A.B * A.cblks * A.tiles * threads_of(A.T, backward) < ((uint64_t)1 << 32), "scan: batch x width x steps is too large for one launch");
     const size_t words = word_bytes(s, backward);
     A.part = (float*)((char*)s->workspace + words + k2_bytes(s, backward));
     if (words) {

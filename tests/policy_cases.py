@@ -182,3 +182,46 @@ def run_adamw(dev, seed, sizes, dtypes=("f32",), bits=32, steps=3, offset=0, mas
     for buf, n in places:
         rest = torch.cat([buf[:offset], buf[offset + n:]]).cpu()
         assert torch.equal(rest, torch.full_like(rest, 7))
+
+
+def run_reset_and_what_is_not_finite_behind_it(dev, T, cut, at):
+    """A NaN gate behind a reset reaches no gradient in front of it: those are the gradients of the steps before the reset alone."""
+    B, D = 2, 8
+    x, r, i, decay, h0, _ = scan_inputs(6, B, T, D, "f32")
+    reset = torch.zeros(B, T, dtype=torch.bool)
+    reset[:, cut] = True
+    r[:, at] = float("nan")
+    leaves = [t.to(dev).requires_grad_() for t in (x, r, i, decay, h0)]
+    h, _ = P.gated_scan(*leaves, reset.to(dev))
+    got = torch.autograd.grad(h, [leaves[0], leaves[1], leaves[2], leaves[4]], torch.ones_like(h))
+    ref, tol = R.scan(x[:, :cut], r[:, :cut], i[:, :cut], decay, h0, dh=torch.ones(B, cut, D))
+    for k, g in zip(("dx", "dr", "di"), got):
+        assert R.far(g[:, :cut].cpu(), ref[k], tol[k]) <= 1, k
+    assert R.far(got[3].cpu(), ref["dh0"], tol["dh0"]) <= 1
+
+
+def run_last_step_reset_to_infinity(dev, T):
+    """The last step begins anew with an infinite input that no loss looks at: the decay's gradient is that of the steps before it."""
+    B, D = 2, 8
+    x, r, i, decay, h0, _ = scan_inputs(7, B, T, D, "f32")
+    reset = torch.zeros(B, T, dtype=torch.bool)
+    reset[:, -1] = True
+    x[:, -1] = float("inf")
+    dh = normal(8, B, T, D)
+    dh[:, -1] = 0
+    leaves = [t.to(dev).requires_grad_() for t in (x, r, i, decay, h0)]
+    h, _ = P.gated_scan(*leaves, reset.to(dev))
+    got, = torch.autograd.grad(h, [leaves[3]], dh.to(dev))
+    ref, tol = R.scan(x[:, :-1], r[:, :-1], i[:, :-1], decay, h0, dh=dh[:, :-1])
+    assert R.far(got.cpu(), ref["ddecay"], tol["ddecay"]) <= 1
+
+
+def run_norm_of_rows_far_apart(dev):
+    """A few columns of very wide rows: the same bits as of a copy."""
+    wide = torch.zeros(3, (1 << 23) + 8, dtype=torch.float16, device=dev)
+    x, u = wide[:, :8], wide[:, 16:24]
+    x.copy_(normal(1, 3, 8))
+    u.copy_(normal(2, 3, 8))
+    pre = torch.ones(8, dtype=torch.float16, device=dev)
+    for a, b in zip(P.block_norm(x, u, pre=pre), P.block_norm(x.contiguous(), u.contiguous(), pre=pre)):
+        assert torch.equal(a, b)

@@ -60,6 +60,16 @@ def test_scan_step(interpreter):
     cases.run_step(interpreter, 3, 5, 66, "bf16")
 
 
+@pytest.mark.parametrize("T,cut,at", [(16, 9, 12), (40, 16, 17), (200, 65, 130), (300, 129, 130)])
+def test_nothing_behind_a_reset_reaches_gradients_before_it(interpreter, T, cut, at):
+    cases.run_reset_and_what_is_not_finite_behind_it(interpreter, T, cut, at)
+
+
+@pytest.mark.parametrize("T", [3, 17, 130])
+def test_a_last_step_that_begins_anew_at_infinity(interpreter, T):
+    cases.run_last_step_reset_to_infinity(interpreter, T)
+
+
 @pytest.mark.parametrize("shape,tx,tu,fn,strided", [
     ((3, 8), "f32", "f32", "sigmoid", False), ((2, 5, 33), "bf16", "bf16", "silu", False), ((9, 130), "f32", "f16", "identity", True),
     ((5, 520), "f16", "f16", "sigmoid", True), ((2, 2050), "f32", "bf16", "silu", False), ((70, 1), "f32", "f32", "sigmoid", False),
@@ -150,3 +160,7 @@ def test_only_the_gradients_that_are_asked_for(interpreter):
     assert [t is None for t in torch.autograd.grad(y.sum(), [x, r, decay], allow_unused=True, retain_graph=True)] == [False] * 3
     assert torch.equal(torch.autograd.grad(y.sum(), [x], retain_graph=True)[0], torch.ones_like(x))
     assert P.block_norm(x, pre=decay)[0] is x
+
+
+def test_norm_of_rows_far_apart(interpreter):
+    cases.run_norm_of_rows_far_apart(interpreter)

@@ -85,6 +85,16 @@ def test_a_reset_keeps_what_is_not_finite_out():
         assert R.far(grads[k][0, 131:], ref[k][0, 131:], tol[k][0, 131:]) <= 1 and R.far(grads[k][1], ref[k][1], tol[k][1]) <= 1
 
 
+@pytest.mark.parametrize("T,cut,at", [(16, 9, 12), (40, 16, 17), (200, 65, 130), (300, 129, 130)])
+def test_nothing_behind_a_reset_reaches_gradients_before_it(T, cut, at):
+    cases.run_reset_and_what_is_not_finite_behind_it(DEV, T, cut, at)
+
+
+@pytest.mark.parametrize("T", [3, 17, 130])
+def test_a_last_step_that_begins_anew_at_infinity(T):
+    cases.run_last_step_reset_to_infinity(DEV, T)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_scan_gates_at_their_ends(dtype):
     """r of -inf keeps the state (a = 1), +inf lets it decay at full rate; i of -inf shuts the input; gradients stay finite."""
@@ -368,3 +378,7 @@ def test_scan_of_many_tiles_and_few_channels():
     ref, tol = R.scan(*start, decay.cpu(), dh=dh[:, :tail].cpu(), dlast=back)
     for k, g in zip(("dx", "dr", "di"), whole):
         assert float((g[:, :tail].cpu().double() - ref[k]).abs().max()) <= 2 * float(tol[k].max()), k
+
+
+def test_norm_of_rows_far_apart():
+    cases.run_norm_of_rows_far_apart(DEV)

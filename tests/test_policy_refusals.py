@@ -60,9 +60,11 @@ def test_adamw_refusals():
             (([p.half()], [p.half()], [z()], [z()], step), {"masters": [z(5)]}, "master")):
         with pytest.raises(ValueError, match=text):
             adamw_step(*args, **kw)
-    for args in (([p, p], [p, p], [z(), z()], [z(), z()], step), ([p, z()], [p, p], [m8[0].float()] * 2, [z(), z()], step)):
+    for args in (([p, p], [p, p], [z(), z()], [z(), z()], step), ([p, z()], [p, p], [m8[0].float()] * 2, [z(), z()], step), ([p, z()], [p, p], [m8, eight()[0]], [v8, (v8[0].clone(), v8[1])], step)):
         with pytest.raises(ValueError, match="twice"):
             adamw_step(*args)
+    with pytest.raises(ValueError, match="twice"):
+        adamw_step([p.half(), z().half()], [p.half()] * 2, [z(), z()], [z(), z()], step, masters=[p, p])
     for entry, text in (((z(), z(2)), "int8 or uint8"), ((z(300, torch.int8), z(3)), "scales")):
         with pytest.raises(ValueError, match=text):
             adamw_values([entry])
@@ -103,6 +105,10 @@ def test_c_entries_check_before_they_launch():
     assert lib.plmpm_scan_workspace(_lib.Scan(**ok), 0, need) == 0 and need.value > 0
     assert lib.plmpm_scan_backward(_lib.Scan(**ok), None) != 0 and "needed" in error()
     assert lib.plmpm_scan_forward(_lib.Scan(**{**ok, "workspace": some + 4, "workspace_bytes": 1 << 20}), None) != 0 and "aligned" in error()
+    room = dict(workspace=some, workspace_bytes=1 << 60)
+    assert lib.plmpm_scan_forward(_lib.Scan(**{**ok, **room, "width": 1 << 27}), None) != 0 and "too large" in error()
+    assert lib.plmpm_scan_forward(_lib.Scan(**{**ok, **room, "batch": 1 << 23, "width": 1}), None) != 0 and "one launch" in error()
+    assert lib.plmpm_scan_forward(_lib.Scan(**{**ok, **room, "h0": some + 2}), None) != 0 and "aligned" in error()
     assert lib.plmpm_scan_forward(_lib.Scan(**{**ok, "steps": 0}), None) == 0                           # nothing to do
     ok = dict(rows=4, width=8, eps=1e-6, x=some, u=some, y=some, z=some, pre=some, stride_x=8, stride_u=8)
     for change, text in (({"x_dtype": 5}, "dtype"), ({"x_dtype": 1}, "u has x's type"), ({"rows": -1}, "negative"), ({"width": 9000}, "at most"), ({"gate_fn": 7}, "gate function"),
