@@ -182,8 +182,8 @@ template <class T, bool VECTOR> struct Quad {
             Vec<T, 4> v;
             v.load((const T*)t.g + at);
             v.get(g);
-            if (t.master) { Vec<float, 4> m; m.load(t.master + at); m.get(w); }
-            else { Vec<T, 4> p; p.load((const T*)t.p + at); p.get(w); }
+            if (t.master) { Vec<float, 4> m; m.load_past(t.master + at); m.get(w); }
+            else { Vec<T, 4> p; p.load_past((const T*)t.p + at); p.get(w); }
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -196,8 +196,8 @@ template <class T, bool VECTOR> struct Quad {
         if (VECTOR) {
             Vec<T, 4> p;
             p.set(w);
-            p.store((T*)t.p + at);
-            if (t.master) { Vec<float, 4> m; m.set(w); m.store(t.master + at); }
+            p.store_past((T*)t.p + at);
+            if (t.master) { Vec<float, 4> m; m.set(w); m.store_past(t.master + at); }
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -208,14 +208,18 @@ template <class T, bool VECTOR> struct Quad {
         }
     }
 };
+// Moments, masters and parameters go past the caches: they are next touched a training step later, while the gradients that the norm has just read
+// (plain loads) are still there for the update, and what a read-back needs stays for it.  8 bits, 55 M elements with masters: the three
+// launches 384 us with ordinary accesses, 356 so; 32 bits, 18 M: 98 and 95; gradients past them too: 357 and 79 with the same gradients at each call,
+// but an update behind a backward pass of 42 M elements then takes 295 us, not 287 (ordinary 298).
 template <class U, bool VECTOR> __device__ __forceinline__ void load4(const U* p, int64_t at, int n, U* out) {
-    if (VECTOR) { typename Wide<4 * sizeof(U)>::type v = *reinterpret_cast<const typename Wide<4 * sizeof(U)>::type*>(p + at); memcpy(out, &v, sizeof v); }
+    if (VECTOR) { Vec<U, 4> v; v.load_past(p + at); memcpy(out, v.w, sizeof v.w); }
     else
 #pragma unroll
         for (int e = 0; e < 4; ++e) out[e] = e < n ? p[at + e] : U(0);
 }
 template <class U, bool VECTOR> __device__ __forceinline__ void store4(U* p, int64_t at, int n, const U* in) {
-    if (VECTOR) { typename Wide<4 * sizeof(U)>::type v; memcpy(&v, in, sizeof v); *reinterpret_cast<typename Wide<4 * sizeof(U)>::type*>(p + at) = v; }
+    if (VECTOR) { Vec<U, 4> v; memcpy(v.w, in, sizeof v.w); v.store_past(p + at); }
     else
 #pragma unroll
         for (int e = 0; e < 4; ++e) if (e < n) p[at + e] = in[e];

@@ -6,6 +6,7 @@
 #include <cmath>
 #include <cstdint>
 #include <cstring>
+#include <type_traits>
 
 #include "../../include/plmpm_policy.h"
 
@@ -76,6 +77,11 @@ template <class T, int N, bool LOOSE = false> struct Vec {
     static constexpr int bytes = N * (int)sizeof(T), part = bytes > 16 ? 16 : bytes, parts = bytes / part;
     typedef typename Wide<part, LOOSE>::type W;
     W w[parts];
+#if !defined(PLB_HOST_EMUL)
+    // the same bytes as a vector of words, as the builtins for such accesses take them
+    typedef std::conditional_t<(part < 4), uint16_t, uint32_t> Word;
+    typedef Word __attribute__((ext_vector_type(part < 4 ? 1 : part / 4), aligned(LOOSE ? 2 : part))) Past;
+#endif
     __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
         for (int k = 0; k < parts; ++k) w[k] = reinterpret_cast<const W*>(p)[k];
@@ -83,6 +89,30 @@ template <class T, int N, bool LOOSE = false> struct Vec {
     __device__ __forceinline__ void store(T* p) const {
 #pragma unroll
         for (int k = 0; k < parts; ++k) reinterpret_cast<W*>(p)[k] = w[k];
+    }
+    // past the caches, for what is not touched again soon: the cache then keeps what is
+    __device__ __forceinline__ void load_past(const T* p) {
+#if defined(PLB_HOST_EMUL)
+        load(p);
+#else
+#pragma unroll
+        for (int k = 0; k < parts; ++k) {
+            const Past v = __builtin_nontemporal_load(reinterpret_cast<const Past*>(p) + k);
+            memcpy(&w[k], &v, part);
+        }
+#endif
+    }
+    __device__ __forceinline__ void store_past(T* p) const {
+#if defined(PLB_HOST_EMUL)
+        store(p);
+#else
+#pragma unroll
+        for (int k = 0; k < parts; ++k) {
+            Past v;
+            memcpy(&v, &w[k], part);
+            __builtin_nontemporal_store(v, reinterpret_cast<Past*>(p) + k);
+        }
+#endif
     }
     __device__ __forceinline__ void zero() { memset(w, 0, sizeof(w)); }
     // unpack from here on (else the compiler keeps the floats of an earlier or a later get, twice the registers where elements have 16 bits)
