@@ -45,6 +45,7 @@ struct ScanArgs {
     float* k2;                          // [width]: -c log2(e) softplus(decay), where there is more than one tile
     int64_t B, T;
     int D, cblks, tiles;
+    bool past;                          // the gradients go past the caches
     float c;
 };
 
@@ -444,9 +445,15 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
         if (live && s < left) {
             const int64_t to = (b * A.T + t0 + s) * A.D;
             Vec<T, VEC> o;
-            o.set(dx); o.store(at_offset((T*)A.out[0] + to, offset));
-            o.set(dr); o.store(at_offset((T*)A.out[1] + to, offset));
-            o.set(di); o.store(at_offset((T*)A.out[2] + to, offset));
+            const auto put = [&](int k, const float* d) {
+                o.set(d);
+                // (an address each: with one the compiler makes one ordinary store of the two)
+                if (A.past) o.store_past(at_offset((T*)A.out[k] + to, offset));
+                else o.store(at_offset((T*)A.out[k] + to, offset));
+            };
+            put(0, dx);
+            put(1, dr);
+            put(2, di);
         }
     }
     // the tile's share of d decay: one row of `part`, summed over the waves (sH is free: its last reader is behind the barrier)
@@ -489,6 +496,10 @@ __global__ __launch_bounds__(1024) void k_decay_grad(const float* part, const fl
 // forward 16 x 8 135 / 75, 8 x 8 155 / 73, 8 x 16 162 / 83, 16 x 4 149 / 81; backward 8 x 8 at 136 registers 171, held to 128 (two workgroups a
 // CU, for some twenty spilled registers) 142; 4 x 16 167, 8 x 16 180, 16 x 4 202.
 constexpr int kForwardSteps = 16, kForwardWaves = 8, kBackwardSteps = 8, kBackwardWaves = 8;
+// Gradients of more bytes than this go past the caches: the first of them would be gone from the 256 MB cache when the last is written, and x, r, i and
+// dh stay in it.  The backward kernel and a copy that reads its gradients, us: 25 MB 25.5 + 19.9 (past the caches 23.0 + 25.4), 75 MB 55.0 + 58.6
+// (54.9 + 72.6), 101 MB 70.8 + 89.9 (70.9 + 104.2), 138 MB 91.8 + 142.7 (90.1 + 139.9), 201 MB 133.4 + 215.1 (131.8 + 208.6).
+constexpr double kPastCaches = 128 << 20;
 int tile_of(bool backward) { return backward ? kBackwardSteps * kBackwardWaves : kForwardSteps * kForwardWaves; }
 int64_t tiles_of(const plmpm_scan* s, bool backward) { return (s->steps + tile_of(backward) - 1) / tile_of(backward); }
 // workspace: one word for the ticket, the words, k2 (an even number of floats), and (backward) the rows of d decay's sums
@@ -589,6 +600,7 @@ int run(const plmpm_scan* s, bool backward, hipStream_t st) {
     const int vec = vector_of(s, backward);
     A.cblks = (A.D + 64 * vec - 1) / (64 * vec);
     A.tiles = (int)tiles_of(s, backward);
+    A.past = 3.0 * dtype_size(s->dtype) * s->batch * s->steps * s->width > kPastCaches;
     NN_REQUIRE((uint64_t)A.B * A.cblks * A.tiles * threads_of(A.T, backward) < ((uint64_t)1 << 32), "scan: batch x width x steps is too large for one launch");
     const size_t words = word_bytes(s, backward);
     A.part = (float*)((char*)s->workspace + words + k2_bytes(s, backward));
