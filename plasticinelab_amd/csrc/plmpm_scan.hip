@@ -50,7 +50,21 @@ struct ScanArgs {
 };
 
 __device__ __forceinline__ bool forgets(float A) { return (as_u(A) >> 31) != 0; }
-__device__ __forceinline__ float softplus(float x) { return fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x))); }
+// max(x, 0) + log(1 + e), e = exp(-|x|): e as a power of two with the product's rounding put right behind it, and log(1 + e) = e P(e) with the polynomial
+// through its values at the Chebyshev points of [0, 1] (relative error 5e-9).  In all within 5.3 x 2^-24, like log1pf(expf(-|x|)), which takes
+// three times as long: 500 x 2048, one step, 7.9 us with those, 5.7 so.
+__device__ __forceinline__ float softplus(float x) {
+    const float far = fabsf(x), to = far > 200.0f ? 200.0f : far;                          // (a NaN stays)
+    const float p = -kLog2e * to, off = fmaf(-1.9259629911266175e-8f, to, fmaf(-kLog2e, to, -p));
+    float e = exp2f(p);
+    e = fmaf(e * off, kLn2, e);
+    constexpr float c[10] = {-0.0031760570127516985f, 0.019542526453733444f, -0.056373611092567444f, 0.10543623566627502f, -0.1526966691017151f,
+                             0.1966327428817749f, -0.24951615929603577f, 0.33329710364341736f, -0.49999892711639404f, 1.0f};
+    float q = c[0];
+#pragma unroll
+    for (int k = 1; k < 10; ++k) q = fmaf(q, e, c[k]);
+    return fmaf(e, q, fmaxf(x, 0.0f));
+}
 
 // sigmoid(r), sigmoid(i), log2 a, a and 1 - a^2.  1 - a^2 = -expm1(2 ln2 l2) cancels for a near 1: above l2 = -0.18 (a^2 > 0.78) it
 // comes from a cubic for -expm1(2 ln2 l) / l, the polynomial through its values at the Chebyshev points (relative error 2.7e-7, half
@@ -254,7 +268,7 @@ __global__ __launch_bounds__(W * 64) void k_scan_forward(ScanArgs A) {
 
 // One step (a rollout's): nothing to chain, so a wave takes 64 VEC channels of a row and the rows below it, 4 waves a workgroup.  The state may move
 // on in place (h0 = h_last): a thread reads and writes its own channels only.  500 x 2048, bf16: 5 us; as a tile of the kernel above, whose
-// waves then walk 15 steps behind the end, 23.
+// waves then walk 15 steps behind the end, 23 (both with a slower softplus).
 template <class T, int VEC>
 __global__ __launch_bounds__(256) void k_scan_step(ScanArgs A) {
     const int d = (blockIdx.x * 64 + (threadIdx.x & 63)) * VEC;
