@@ -485,7 +485,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
 // before a launch of more than one tile: the ticket and the words cleared, and the channels' k2 (softplus is more work than a step)
 __global__ __launch_bounds__(256) void k_prepare(Word* p, int64_t n, float* k2, const float* decay, int D, float c) {
     const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)gridDim.x * 256;
-    for (int64_t k = first; k < n; k += all) p[k] = 0;
+    for (int64_t k = first; k < n; k += all) publish(p + k, 0);        // (4.4 us; with ordinary stores, to be written back at the end, 4.8)
     for (int64_t d = first; d < D; d += all) k2[d] = -c * kLog2e * softplus(decay[d]);
 }
 

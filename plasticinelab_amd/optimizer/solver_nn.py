@@ -121,9 +121,10 @@ class SolverNN:
             obs_t, act_t, *states = graph.pop(step)
             g = torch.as_tensor(sim.engine.get_action_grad(step + 1)[step].reshape(-1)[:A].copy()).to(**self.place)
             ends, grads = [act_t], [g]
-            if states and from_later:
+            later = from_later.pop() if from_later else None
+            if later is not None and states[1].requires_grad:      # (a policy may leave its memory out of the graph)
                 ends.append(states[1])
-                grads.append(from_later.pop())
+                grads.append(later)
             torch.autograd.backward(ends, grads)           # accumulates into policy.parameters().grad, fills obs_t.grad
             if states:
                 from_later[:] = [states[0].grad]

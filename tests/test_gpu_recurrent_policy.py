@@ -143,6 +143,34 @@ def test_recurrent_policy_in_the_loop_matches_oracle(oracle_c):
     assert abs(loss - float(total.detach())) / abs(float(total.detach())) < 1e-5 and np.abs(ref).max() > 0 and relerr(grad, ref) < 4 * TOL
 
 
+class Counting(torch.nn.Module):
+    """A policy whose memory is outside the graph (``how``: a count kept without gradients, or handed on untouched) and does not reach its actions."""
+
+    def __init__(self, obs_dim, action_dim, how):
+        super().__init__()
+        self.lin, self.how = torch.nn.Linear(obs_dim, action_dim, device=DEV), how
+
+    def forward(self, obs):
+        return self.lin(obs)
+
+    def initial_state(self, batch):
+        return torch.zeros(batch, 1, device=DEV)
+
+    def step(self, obs, state):
+        return self.lin(obs), state.detach() + 1 if self.how == "count" else state
+
+
+@pytest.mark.parametrize("how", ["count", "untouched"])
+def test_a_memory_outside_the_graph(how):
+    from plasticinelab_amd.optimizer.solver_nn import SolverNN
+    _, env, obs_dim = make_env(1000, 40)
+    torch.manual_seed(4)
+    policy = Counting(obs_dim, env.primitives.action_dim, how)
+    state = env.get_state()["state"]
+    _, grad = SolverNN(env, policy, horizon=3, n_observed_particles=40).forward(state)
+    _, want = SolverNN(env, policy.lin, horizon=3, n_observed_particles=40).forward(state)
+    assert np.abs(want).max() > 0 and relerr(grad, want) < TOL
+
 
 @pytest.mark.parametrize("bits", [32, 8])
 def test_solver_updates_a_policy_on_the_gpu(bits):
