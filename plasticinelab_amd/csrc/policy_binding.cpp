@@ -535,6 +535,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
             if (p) std::rethrow_exception(p);
         } catch (const EngineError& e) {
             PyErr_SetString(error.ptr(), e.what());
+        } catch (const c10::Error&) {                    // (torch's own, as torch gives them: out of memory above all)
+            torch::translate_exception_to_python(p);
         }
     });
     const auto unlocked = py::call_guard<py::gil_scoped_release>();

@@ -382,3 +382,9 @@ def test_scan_of_many_tiles_and_few_channels():
 
 def test_norm_of_rows_far_apart():
     cases.run_norm_of_rows_far_apart(DEV)
+
+
+def test_out_of_memory_is_torchs_own_error():
+    x = torch.zeros(1, 1, 1024, dtype=torch.bfloat16, device=DEV).expand(1, 1 << 29, 1024)          # a terabyte of outputs, 2 KB of inputs
+    with pytest.raises(torch.OutOfMemoryError):
+        P.gated_scan(x, x, x, torch.zeros(1024, device=DEV))
