@@ -21,7 +21,7 @@ SOURCES = "plmpm_capi.hip plmpm_kinematics.hip plmpm_loss.hip plmpm_migrate.hip 
 @pytest.fixture(scope="module")
 def interpreter():
     """The operators' library compiled by g++ for the interpreter; tensors on the CPU stand for device memory.  (PLMPM_EMUL_VARIANT=asan: under
-    AddressSanitizer, with the LD_PRELOAD of tests/test_emul_tier.py.)"""
+    AddressSanitizer; LD_PRELOAD then holds libasan.so and, for the C++ exceptions of the binding, libstdc++.so.6.)"""
     tag = "_asan" if os.environ.get("PLMPM_EMUL_VARIANT") == "asan" else ""
     out = f"libplmpm_policy_emul{tag}.so"
     subprocess.check_call(["make", "-s", "-j", "6", "-C", HERE, f"OBJDIR=build_emul_policy{tag}", f"OUT={out}", f"SAN={1 if tag else 0}",
