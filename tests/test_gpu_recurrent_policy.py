@@ -224,3 +224,26 @@ def test_act_in_inference_mode():
         got = torch.stack([policy.act(obs[:, t], state) for t in range(3)], 1)
         again, last = policy(obs)
     assert off(got, want) < TOL and off(state, end) < TOL and torch.equal(again, want) and torch.equal(last, end)
+
+
+def test_act_captured_and_replayed():
+    """A rollout's step as a graph: the state moves on from replay to replay, with eager work and synchronisation in between."""
+    policy = RecurrentPolicy(9, 4, width=64, depth=2)
+    obs = torch.randn(8, 5, 9, device=DEV)
+    state, slot = policy.initial_state(5), torch.zeros(5, 9, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        policy.act(slot, state.clone())
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = policy.act(slot, state)
+    state.zero_()
+    eager = policy.initial_state(5)
+    for t in range(8):
+        slot.copy_(obs[t])
+        graph.replay()
+        want = policy.act(obs[t], eager)
+        torch.cuda.synchronize()
+        assert off(out, want) < TOL and off(state, eager) < TOL, t
