@@ -51,6 +51,7 @@ inline void from_f(float f, f16& o) {
 }
 inline float exp2_fast(float x) { return exp2f(x); }
 inline void sleep_a_little() { __builtin_amdgcn_s_sleep(1); }
+inline void wait_for_memory() {}
 #else
 __device__ __forceinline__ float to_f(f16 x) { _Float16 h; memcpy(&h, &x, 2); return (float)h; }
 // round to nearest even, one conversion instruction each
@@ -58,8 +59,16 @@ __device__ __forceinline__ void from_f(float f, bf16& o) { const __bf16 h = (__b
 __device__ __forceinline__ void from_f(float f, f16& o) { const _Float16 h = (_Float16)f; memcpy(&o, &h, 2); }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }       // v_exp_f32: within 1 ulp; exponents below -126 give 0
 __device__ __forceinline__ void sleep_a_little() { __builtin_amdgcn_s_sleep(8); }        // 8 x 64 cycles
+__device__ __forceinline__ void wait_for_memory() { __builtin_amdgcn_s_waitcnt(0x0f70); }       // vmcnt(0)
 #endif
 __device__ __forceinline__ void from_f(float f, float& o) { o = f; }
+
+// what comes of `f` is made anew from here on, as with Vec::forget
+__device__ __forceinline__ void anew(float& f) {
+#if !defined(PLB_HOST_EMUL)
+    asm volatile("" : "+v"(f));
+#endif
+}
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 // 1 / (1 + e^-x): both ends come out right by themselves (e^-x = inf -> 0, 0 -> 1)
@@ -72,6 +81,7 @@ template <> struct Wide<2> { typedef uint16_t type; };
 template <> struct Wide<4> { typedef uint32_t type; };
 template <> struct Wide<8> { struct alignas(8) type { uint32_t w[2]; }; };
 template <> struct Wide<16> { struct alignas(16) type { uint32_t w[4]; }; };
+template <> struct Wide<4, true> { struct __attribute__((packed, aligned(2))) type { uint32_t w; }; };
 template <> struct Wide<16, true> { struct __attribute__((packed, aligned(2))) type { uint32_t w[4]; }; };
 template <class T, int N, bool LOOSE = false> struct Vec {
     static constexpr int bytes = N * (int)sizeof(T), part = bytes > 16 ? 16 : bytes, parts = bytes / part;
@@ -115,6 +125,14 @@ template <class T, int N, bool LOOSE = false> struct Vec {
 #endif
     }
     __device__ __forceinline__ void zero() { memset(w, 0, sizeof(w)); }
+    // the elements move down by `n`, zeros behind them (a vector of 4 bytes)
+    __device__ __forceinline__ void drop(int n) {
+        static_assert(bytes == 4, "one word");
+        uint32_t u;
+        memcpy(&u, w, 4);
+        u >>= 8 * sizeof(T) * n;
+        memcpy(w, &u, 4);
+    }
     // unpack from here on (else the compiler keeps the floats of an earlier or a later get, twice the registers where elements have 16 bits)
     __device__ __forceinline__ void forget() {
 #if !defined(PLB_HOST_EMUL)

@@ -84,12 +84,13 @@ __device__ __forceinline__ Gates gates(float r, float i, float k2) {
 // which of the S steps from t on are resets: a bit each (uniform over the wave)
 template <int S> __device__ __forceinline__ unsigned reset_bits(const ScanArgs& A, int64_t b, int64_t t, int left) {
     const int lane = threadIdx.x & 63;
-    const int hit = lane < S && lane < left ? A.reset[b * A.T + t + lane] != 0 : 0;
+    const int hit = A.reset && lane < S && lane < left ? A.reset[b * A.T + t + lane] != 0 : 0;
     return (unsigned)__ballot(hit);
 }
 
 // S steps from t on, `stride` elements apart: whole, or the first `left` of them (those behind load the last one again)
-template <bool WHOLE, class T, int VEC, int S> __device__ __forceinline__ void load_steps(const void* base, int64_t stride, int left, unsigned offset, Vec<T, VEC> (&raw)[S]) {
+template <bool WHOLE, class T, int VEC, bool LOOSE, int S>
+__device__ __forceinline__ void load_steps(const void* base, int64_t stride, int left, unsigned offset, Vec<T, VEC, LOOSE> (&raw)[S]) {
     T* row = (T*)base;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
@@ -99,8 +100,39 @@ template <bool WHOLE, class T, int VEC, int S> __device__ __forceinline__ void l
 }
 template <int VEC> __device__ __forceinline__ void load_k2(const ScanArgs& A, int d, float (&k2)[VEC]) {
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) k2[v] = A.k2 ? A.k2[d + v] : -A.c * kLog2e * softplus(A.decay[d + v]);
+    for (int v = 0; v < VEC; ++v) {
+        const int at = VEC == 1 || d + v < A.D ? d + v : d;
+        k2[v] = A.k2 ? A.k2[at] : -A.c * kLog2e * softplus(A.decay[at]);
+    }
 }
+// a lane's channels of a row.  LOOSE: rows at any element's address, and the last lane may have one channel only (`tail`): it loads the two that the
+// row ends with and drops the first, and stores one.
+template <class T, int VEC, bool LOOSE> struct Channels {
+    int d0;
+    bool live, tail;
+    unsigned in, out;                   // byte offsets
+    __device__ __forceinline__ Channels(int first, int D) {
+        d0 = first + (int)(threadIdx.x & 63) * VEC;
+        live = d0 < D;
+        tail = LOOSE && live && d0 + VEC > D;
+        out = (unsigned)(live ? d0 : 0) * (unsigned)sizeof(T);
+        in = out - (tail ? (unsigned)sizeof(T) : 0u);
+    }
+    __device__ __forceinline__ void loaded(Vec<T, VEC, LOOSE>& v) const {
+        if constexpr (LOOSE) v.drop(tail ? 1 : 0);
+    }
+    // `past`: past the caches (the empty asm keeps the compiler from making one ordinary store of the two)
+    __device__ __forceinline__ void store(const Vec<T, VEC, LOOSE>& v, T* row, bool past) const {
+        if (LOOSE && tail) {
+            Vec<T, 1> one;
+            memcpy(one.w, v.w, sizeof(T));
+            one.store(at_offset(row, out));
+        } else if (past) {
+            v.store_past(at_offset(row, out));
+            asm volatile("");
+        } else v.store(at_offset(row, out));
+    }
+};
 __device__ __forceinline__ int steps_left(int64_t T, int64_t t, int most) {
     const int64_t n = T - t;
     return n < most ? (n < 0 ? 0 : (int)n) : most;
@@ -168,7 +200,7 @@ template <int NCH> __device__ __forceinline__ Place place(const ScanArgs& A, uns
     return {(int64_t)b, (int)pos, (int)(rest - b * (unsigned)A.cblks) * NCH};
 }
 
-template <class T, int VEC, int S, int W, bool RESET>
+template <class T, int VEC, int S, int W, bool RESET, bool LOOSE>
 __global__ __launch_bounds__(W * 64) void k_scan_forward(ScanArgs A) {
     constexpr int NCH = 64 * VEC;
     __shared__ float sA[W][NCH], sH[W][NCH];
@@ -177,13 +209,12 @@ __global__ __launch_bounds__(W * 64) void k_scan_forward(ScanArgs A) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const Place at = place<NCH>(A, &ticket);
     const int64_t b = at.b;
-    const int first = at.first, d0 = first + lane * VEC;
-    const bool live = d0 < A.D;                          // VEC divides the width: a lane's channels are all there or none is
-    const int dl = live ? d0 : 0;
+    const int first = at.first;
+    const Channels<T, VEC, LOOSE> mine(first, A.D);
     const int64_t t0 = (int64_t)at.pos * (S * W) + wave * S;
     const int left = __builtin_amdgcn_readfirstlane(steps_left(A.T, t0, S));
     const int64_t from = left ? t0 : A.T - 1;            // (a wave whole behind the end loads the last step)
-    const unsigned offset = (unsigned)dl * (unsigned)sizeof(T), cut = RESET ? reset_bits<S>(A, b, t0, left) : 0u;
+    const unsigned cut = RESET ? reset_bits<S>(A, b, t0, left) : 0u;
     float k2[VEC], a[S][VEC], u[S][VEC], PA[VEC], PH[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
@@ -192,13 +223,15 @@ __global__ __launch_bounds__(W * 64) void k_scan_forward(ScanArgs A) {
     }
     const auto walk = [&](auto whole) {
         constexpr bool WHOLE = decltype(whole)::value;
-        Vec<T, VEC> raw[3][S];
+        Vec<T, VEC, LOOSE> raw[3][S];
 #pragma unroll
-        for (int k = 0; k < 3; ++k) load_steps<WHOLE>((const T*)A.in[k] + b * A.sb[k] + from * A.st[k], A.st[k], left, offset, raw[k]);
-        load_k2<VEC>(A, dl, k2);
+        for (int k = 0; k < 3; ++k) load_steps<WHOLE>((const T*)A.in[k] + b * A.sb[k] + from * A.st[k], A.st[k], left, mine.in, raw[k]);
+        load_k2<VEC>(A, mine.live ? mine.d0 : 0, k2);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             float x[VEC], r[VEC], i[VEC];
+#pragma unroll
+            for (int k = 0; k < 3; ++k) mine.loaded(raw[k][s]);
             raw[0][s].get(x);
             raw[1][s].get(r);
             raw[2][s].get(i);
@@ -233,12 +266,12 @@ __global__ __launch_bounds__(W * 64) void k_scan_forward(ScanArgs A) {
                 th = forgets(pa) ? ph : fmaf(pa, th, ph);
                 ta = forgets(pa) ? -0.0f : ta * pa;
             }
-            Word* mine = A.words + (int64_t)at.pos * stride + col;
+            Word* own = A.words + (int64_t)at.pos * stride + col;
             if (at.pos > 0) {
-                if (at.pos < A.tiles - 1) publish(mine, word_of(ta, th));
+                if (at.pos < A.tiles - 1) publish(own, word_of(ta, th));
                 c = state_before<NCH>(A.words + col, stride, at.pos, &path[0][ch]);
             }
-            if (at.pos < A.tiles - 1) publish(mine, state_word(forgets(ta) ? th : fmaf(ta, c, th)));
+            if (at.pos < A.tiles - 1) publish(own, state_word(forgets(ta) ? th : fmaf(ta, c, th)));
         }
         for (int w = 0; w < waves; ++w) {
             const float pa = sA[w][ch], ph = sH[w][ch];
@@ -253,16 +286,19 @@ __global__ __launch_bounds__(W * 64) void k_scan_forward(ScanArgs A) {
     float now[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) now[v] = sA[wave][lane * VEC + v];
-    if (!live) return;
+    // (without it the compiler waits before every store below, in case one of the loads above is still out, and so for the store before it:
+    // 8 x 2047 x 2048 77 us instead of 70)
+    wait_for_memory();
+    if (!mine.live) return;
     T* out = (T*)A.h + (b * A.T + t0) * A.D;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
         if (s >= left) continue;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) now[v] = RESET && (cut >> s & 1) ? u[s][v] : fmaf(a[s][v], now[v], u[s][v]);
-        Vec<T, VEC> o;
+        Vec<T, VEC, LOOSE> o;
         o.set(now);
-        o.store(at_offset(out + (int64_t)s * A.D, (unsigned)d0 * (unsigned)sizeof(T)));
+        mine.store(o, out + (int64_t)s * A.D, false);
     }
 }
 
@@ -309,7 +345,7 @@ __global__ __launch_bounds__(256) void k_scan_step(ScanArgs A) {
 // h_{t-1} in 32 bits, and backward) go through one exchange; tiles are handed out from the last to the first.
 //   dx = g m s_i   di = g m x s_i (1 - s_i)   dla = g (a h_{t-1} - s_i x a^2 / m)   dr = dla la (1 - s_r)
 // For la -> 0 the product la a^2 / m goes to 0 (m ~ sqrt(-2 la)): where m is 0 that term is left out.
-template <class T, int VEC, int S, int W, bool RESET>
+template <class T, int VEC, int S, int W, bool LOOSE>
 __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
     static_assert(S * W % kCheckpoint == 0, "a tile starts at a checkpoint");
     constexpr int NCH = 64 * VEC;
@@ -320,16 +356,17 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
     const Place at = place<NCH>(A, &ticket);
     const int tile = A.tiles - 1 - at.pos;
     const int64_t b = at.b;
-    const int first = at.first, d0 = first + lane * VEC;
-    const bool live = d0 < A.D;
-    const int dl = live ? d0 : 0;
+    const int first = at.first;
+    const Channels<T, VEC, LOOSE> mine(first, A.D);
     const int64_t t0 = (int64_t)tile * (S * W) + wave * S;
     const int left = __builtin_amdgcn_readfirstlane(steps_left(A.T, t0, S));
     const int64_t from = left ? t0 : A.T - 1;
-    const unsigned offset = (unsigned)dl * (unsigned)sizeof(T), cut = RESET ? reset_bits<S>(A, b, t0, left) : 0u;
-    // Kept for the second walk: x and dh as they came, a, m and the gates.  What can be had from those in a few operations is not (a register more
-    // here is one spilled to memory: with m s_i and s_i x a^2 / m held in m's place, 29 of them, 8 x 2047 x 2048 took 154 us instead of 131).
-    Vec<T, VEC> rawx[S], rawg[S];
+    const unsigned cut = reset_bits<S>(A, b, t0, left);
+    // Kept for the second walk: x and dh as they came, a, m and the gates.  What can be had from those in a few operations is not: a register more
+    // here is one spilled to memory.  (8 x 2047 x 2048: with m s_i and s_i x a^2 / m held in m's place, 29 of them, 154 us instead of 131.  The
+    // compiler would do the same by itself, hence forget and anew: calls in bf16 and fp16 without resets 165 and 171 us, with the 16 and 32
+    // registers that it keeps otherwise 185 and 196.  A kernel without the resets' selects kept more of them and was the slower one.)
+    Vec<T, VEC, LOOSE> rawx[S], rawg[S];
     float k2[VEC], a[S][VEC], sr[S][VEC], si[S][VEC], m[S][VEC], PA[VEC], PH[VEC], PE[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
@@ -338,17 +375,23 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
     }
     const auto walk = [&](auto whole) {
         constexpr bool WHOLE = decltype(whole)::value;
-        Vec<T, VEC> rawr[S], rawi[S];
-        load_steps<WHOLE>((const T*)A.in[1] + b * A.sb[1] + from * A.st[1], A.st[1], left, offset, rawr);
-        load_steps<WHOLE>((const T*)A.in[2] + b * A.sb[2] + from * A.st[2], A.st[2], left, offset, rawi);
-        load_steps<WHOLE>((const T*)A.in[0] + b * A.sb[0] + from * A.st[0], A.st[0], left, offset, rawx);
-        if (A.dh) load_steps<WHOLE>((const T*)A.dh + (b * A.T + from) * A.D, (int64_t)A.D, left, offset, rawg);
+        Vec<T, VEC, LOOSE> rawr[S], rawi[S];
+        load_steps<WHOLE>((const T*)A.in[1] + b * A.sb[1] + from * A.st[1], A.st[1], left, mine.in, rawr);
+        load_steps<WHOLE>((const T*)A.in[2] + b * A.sb[2] + from * A.st[2], A.st[2], left, mine.in, rawi);
+        load_steps<WHOLE>((const T*)A.in[0] + b * A.sb[0] + from * A.st[0], A.st[0], left, mine.in, rawx);
+        if (A.dh) load_steps<WHOLE>((const T*)A.dh + (b * A.T + from) * A.D, (int64_t)A.D, left, mine.in, rawg);
 #pragma unroll
         for (int s = 0; s < S; ++s) if (!A.dh || !(WHOLE || s < left)) rawg[s].zero();
-        load_k2<VEC>(A, dl, k2);
+        load_k2<VEC>(A, mine.live ? mine.d0 : 0, k2);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             float x[VEC], r[VEC], i[VEC];
+            mine.loaded(rawx[s]);
+            mine.loaded(rawr[s]);
+            mine.loaded(rawi[s]);
+            mine.loaded(rawg[s]);
+            rawx[s].forget();
+            rawg[s].forget();
             rawx[s].get(x);
             rawr[s].get(r);
             rawi[s].get(i);
@@ -358,7 +401,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
                 const Gates g = gates(r[v], i[v], k2[v]);
                 sr[s][v] = there ? g.sr : 0.0f;
                 si[s][v] = g.si;
-                if (RESET && (cut >> s & 1)) {
+                if ((cut >> s & 1)) {
                     a[s][v] = 0.0f;
                     m[s][v] = 1.0f;
                     PH[v] = g.si * x[v];
@@ -370,6 +413,8 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
                 }
             }
         }
+#pragma unroll
+        for (int s = 0; s < S; ++s) { rawx[s].forget(); rawg[s].forget(); }
     };
     if (left == S) walk(std::true_type());
     else walk(std::false_type());
@@ -378,11 +423,11 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
         float g[VEC];
         rawg[s].get(g);
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) PE[v] = RESET && (cut >> s & 1) ? 0.0f : a[s][v] * (g[v] + PE[v]);
+        for (int v = 0; v < VEC; ++v) PE[v] = (cut >> s & 1) ? 0.0f : a[s][v] * (g[v] + PE[v]);
     }
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-        sA[wave][lane * VEC + v] = RESET && cut ? -0.0f : PA[v];
+        sA[wave][lane * VEC + v] = cut ? -0.0f : PA[v];
         sH[wave][lane * VEC + v] = PH[v];
         sE[wave][lane * VEC + v] = PE[v];
     }
@@ -398,12 +443,12 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
                 te = forgets(pa) ? pe : fmaf(pa, te, pe);
                 ta = forgets(pa) ? -0.0f : ta * pa;
             }
-            Word* mine = A.words + (int64_t)at.pos * stride + col;
+            Word* own = A.words + (int64_t)at.pos * stride + col;
             if (at.pos > 0) {
-                if (at.pos < A.tiles - 1) publish(mine, word_of(ta, te));
+                if (at.pos < A.tiles - 1) publish(own, word_of(ta, te));
                 e = state_before<NCH>(A.words + col, stride, at.pos, &path[0][ch]);
             }
-            if (at.pos < A.tiles - 1) publish(mine, state_word(forgets(ta) ? te : fmaf(ta, e, te)));
+            if (at.pos < A.tiles - 1) publish(own, state_word(forgets(ta) ? te : fmaf(ta, e, te)));
         }
         for (int w = waves - 1; w >= 0; --w) {
             const float pa = sA[w][ch], pe = sE[w][ch];
@@ -419,7 +464,17 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
     }
     __syncthreads();
 #pragma unroll
-    for (int s = 0; s < S; ++s) { rawx[s].forget(); rawg[s].forget(); }
+    for (int s = 0; s < S; ++s) {
+        rawx[s].forget();
+        rawg[s].forget();
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            anew(m[s][v]);
+            anew(si[s][v]);
+            anew(a[s][v]);
+            anew(sr[s][v]);
+        }
+    }
     float now[VEC], e[VEC], sum[VEC], pull[S][VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
@@ -433,7 +488,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
         rawx[s].get(x);
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            const bool reset = RESET && (cut >> s & 1);
+            const bool reset = (cut >> s & 1);
             const float sx = si[s][v] * x[v], u = m[s][v] * sx, inv = m[s][v] == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(m[s][v]);
             pull[s][v] = reset ? 0.0f : a[s][v] * fmaf(-sx * inv, a[s][v], now[v]);        // dla / g
             now[v] = reset ? u : fmaf(a[s][v], now[v], u);
@@ -446,7 +501,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
         rawg[s].get(g);
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            const bool reset = RESET && (cut >> s & 1);
+            const bool reset = (cut >> s & 1);
             g[v] += e[v];
             e[v] = reset ? 0.0f : a[s][v] * g[v];
             dx[v] = g[v] * m[s][v] * si[s][v];
@@ -456,14 +511,12 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
             dr[v] = q * (k2[v] * kLn2) * (1.0f - sr[s][v]);
             sum[v] += q;
         }
-        if (live && s < left) {
+        if (mine.live && s < left) {
             const int64_t to = (b * A.T + t0 + s) * A.D;
-            Vec<T, VEC> o;
             const auto put = [&](int k, const float* d) {
+                Vec<T, VEC, LOOSE> o;
                 o.set(d);
-                // (an address each: with one the compiler makes one ordinary store of the two)
-                if (A.past) o.store_past(at_offset((T*)A.out[k] + to, offset));
-                else o.store(at_offset((T*)A.out[k] + to, offset));
+                mine.store(o, (T*)A.out[k] + to, A.past);
             };
             put(0, dx);
             put(1, dr);
@@ -508,7 +561,7 @@ __global__ __launch_bounds__(1024) void k_decay_grad(const float* part, const fl
 
 // Steps a wave and waves a workgroup of the two kernels.  Measured at 65537 steps x 1024 channels (forward) and 8 x 2047 x 2048 (both), bf16, us:
 // forward 16 x 8 135 / 75, 8 x 8 155 / 73, 8 x 16 162 / 83, 16 x 4 149 / 81; backward 8 x 8 at 136 registers 171, held to 128 (two workgroups a
-// CU, for some twenty spilled registers) 142; 4 x 16 167, 8 x 16 180, 16 x 4 202.
+// CU, for some twenty spilled registers) 142, without those 128; 4 x 16 167, 8 x 16 180, 16 x 4 202.
 constexpr int kForwardSteps = 16, kForwardWaves = 8, kBackwardSteps = 8, kBackwardWaves = 8;
 // Gradients of more bytes than this go past the caches: the first of them would be gone from the 256 MB cache when the last is written, and x, r, i and
 // dh stay in it.  The backward kernel and a copy that reads its gradients, us: 25 MB 25.5 + 19.9 (past the caches 23.0 + 25.4), 75 MB 55.0 + 58.6
@@ -528,19 +581,16 @@ unsigned threads_of(int64_t steps, bool backward) {
     const int S = backward ? kBackwardSteps : kForwardSteps, W = backward ? kBackwardWaves : kForwardWaves;
     return 64u * (unsigned)std::min<int64_t>((steps + S - 1) / S, W);
 }
-template <class T, int VEC, bool RESET> void launch(const ScanArgs& A, bool backward, hipStream_t st) {
+template <class T, int VEC, bool LOOSE> void launch(const ScanArgs& A, bool backward, hipStream_t st) {
     const dim3 grid((unsigned)(A.B * A.cblks * A.tiles)), block(threads_of(A.T, backward));
-    if (backward) hipLaunchKernelGGL((k_scan_backward<T, VEC, kBackwardSteps, kBackwardWaves, RESET>), grid, block, 0, st, A);
-    else hipLaunchKernelGGL((k_scan_forward<T, VEC, kForwardSteps, kForwardWaves, RESET>), grid, block, 0, st, A);
+    if (backward) hipLaunchKernelGGL((k_scan_backward<T, VEC, kBackwardSteps, kBackwardWaves, LOOSE>), grid, block, 0, st, A);
+    else if (A.reset) hipLaunchKernelGGL((k_scan_forward<T, VEC, kForwardSteps, kForwardWaves, true, LOOSE>), grid, block, 0, st, A);
+    else hipLaunchKernelGGL((k_scan_forward<T, VEC, kForwardSteps, kForwardWaves, false, LOOSE>), grid, block, 0, st, A);
 }
-template <class T, int VEC> void launch(const ScanArgs& A, bool backward, hipStream_t st) {
-    if (A.reset) launch<T, VEC, true>(A, backward, st);
-    else launch<T, VEC, false>(A, backward, st);
-}
-template <class T> void launch(const ScanArgs& A, int vec, bool backward, hipStream_t st) {
+template <class T> void launch(const ScanArgs& A, int vec, bool loose, bool backward, hipStream_t st) {
     if constexpr (sizeof(T) == 2)
-        if (vec == 2) return launch<T, 2>(A, backward, st);
-    launch<T, 1>(A, backward, st);
+        if (vec == 2) return loose ? launch<T, 2, true>(A, backward, st) : launch<T, 2, false>(A, backward, st);
+    launch<T, 1, false>(A, backward, st);
 }
 
 // one step: four channels a lane where everything keeps to them
@@ -555,17 +605,20 @@ template <class T> void launch_step(const ScanArgs& A, hipStream_t st) {
     else hipLaunchKernelGGL((k_scan_step<T, 1>), grid, dim3(256), 0, st, A);
 }
 
-// Channels a lane: 4 bytes' worth, so that a wave's rows are 256 bytes -- 2 channels of 16 bits where rows and pointers keep to it and at least half
-// of a wave's 128 channels are there, else 1.  (16 bits, 8 x 2047 x 2048, forward and backward: 2 channels 70 + 141 us, 1 channel 80 + 158, 4
-// channels 72 + 202; 32 bits, 16 x 50 x 256: 1 channel 7.2 + 9.0 us, 2 channels 8.1 + 11.9.)
-int vector_of(const plmpm_scan* s, bool backward) {
+// Channels a lane: 4 bytes' worth, so that a wave's rows are 256 bytes -- 2 channels of 16 bits where at least half of a wave's 128 channels are
+// there, else 1.  (16 bits, 8 x 2047 x 2048, forward and backward: 2 channels 70 + 141 us, 1 channel 80 + 158, 4 channels 72 + 202; 32 bits,
+// 16 x 50 x 256: 1 channel 7.2 + 9.0 us, 2 channels 8.1 + 11.9.)
+int vector_of(const plmpm_scan* s) { return dtype_size(s->dtype) == 2 && s->width >= 64 ? 2 : 1; }
+// Whether such a row may begin between two words: an odd width, odd strides or pointers.  (16 bits, calls at
+// 8 x 2047 x 2047, forward and backward: 77 + 185 us; with 1 channel a lane 98 + 215.)
+bool loose(const plmpm_scan* s, bool backward) {
     const int size = dtype_size(s->dtype);
     int bytes = 16;
     const void* in[3] = {s->x, s->r, s->i};
     for (int k = 0; k < 3; ++k) bytes = std::min(bytes, std::min(aligned_to(in[k], s->stride_b[k], size), aligned_to(in[k], s->stride_t[k], size)));
     if (backward) for (const void* p : {(const void*)s->dh, (const void*)s->dx, (const void*)s->dr, (const void*)s->di}) bytes = std::min(bytes, aligned_to(p, s->width, size));
     else bytes = std::min(bytes, aligned_to(s->h, s->width, size));
-    return size == 2 && s->width % 2 == 0 && s->width >= 64 && bytes >= 4 ? 2 : 1;
+    return bytes < 4;
 }
 
 int check(const plmpm_scan* s, bool backward, bool pointers) {
@@ -611,7 +664,8 @@ int run(const plmpm_scan* s, bool backward, hipStream_t st) {
         NN_LAUNCHED("scan forward");
         return 0;
     }
-    const int vec = vector_of(s, backward);
+    const int vec = vector_of(s);
+    const bool between = vec == 2 && loose(s, backward);
     A.cblks = (A.D + 64 * vec - 1) / (64 * vec);
     A.tiles = (int)tiles_of(s, backward);
     A.past = 3.0 * dtype_size(s->dtype) * s->batch * s->steps * s->width > kPastCaches;
@@ -625,9 +679,9 @@ int run(const plmpm_scan* s, bool backward, hipStream_t st) {
         const int64_t n = (int64_t)(words / sizeof(Word)), groups = (n + 1023) / 1024;
         hipLaunchKernelGGL(k_prepare, dim3((unsigned)(groups < 2048 ? groups : 2048)), dim3(256), 0, st, (Word*)s->workspace, n, A.k2, A.decay, A.D, A.c);
     }
-    if (s->dtype == PLMPM_NN_F32) launch<float>(A, vec, backward, st);
-    else if (s->dtype == PLMPM_NN_BF16) launch<bf16>(A, vec, backward, st);
-    else launch<f16>(A, vec, backward, st);
+    if (s->dtype == PLMPM_NN_F32) launch<float>(A, vec, between, backward, st);
+    else if (s->dtype == PLMPM_NN_BF16) launch<bf16>(A, vec, between, backward, st);
+    else launch<f16>(A, vec, between, backward, st);
     if (backward)
         hipLaunchKernelGGL(k_decay_grad, dim3((unsigned)((A.D + 63) / 64)), dim3(1024), 0, st, (const float*)A.part, A.decay, s->ddecay, (int64_t)A.tiles * A.B, A.D, A.c);
     NN_LAUNCHED(backward ? "scan backward" : "scan forward");

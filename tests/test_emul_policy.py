@@ -51,6 +51,13 @@ def test_scan(interpreter, B, T, D, dtype, layout, resets):
     cases.run_scan(interpreter, 11, B, T, D, dtype, layout, resets=resets, with_h0=T != 20)
 
 
+@pytest.mark.parametrize("B,T,D,dtype,layout,resets", [
+    (2, 70, 65, "bf16", "plain", 0.1), (1, 200, 193, "f16", "odd", 0.05), (2, 130, 129, "bf16", "packed", 0.0), (2, 20, 128, "f16", "odd", 0.0), (1, 65, 127, "bf16", "time_major", 0.2),
+    (1, 2, 255, "bf16", "plain", 0.0)])
+def test_scan_of_16_bits_between_words(interpreter, B, T, D, dtype, layout, resets):
+    cases.run_scan(interpreter, 12, B, T, D, dtype, layout, resets=resets, with_h0=T != 20)
+
+
 @pytest.mark.parametrize("use", [("h",), ("last",)])
 def test_scan_with_one_gradient(interpreter, use):
     cases.run_scan(interpreter, 5, 2, 70, 16, "f32", use=use)
