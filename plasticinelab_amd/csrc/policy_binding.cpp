@@ -85,6 +85,11 @@ bool tracked(std::initializer_list<const Maybe*> ts) {
     for (const Maybe* t : ts) if (*t && (*t)->requires_grad()) return true;
     return false;
 }
+// A forward-mode tangent that comes with a tensor would be lost: nothing here makes one for what a kernel writes.
+void no_tangents(std::initializer_list<const Maybe*> ts, const char* name) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Maybe* t : ts) REFUSE_IF(*t && (*t)->defined() && (*t)->_fw_grad(0).defined(), name, " has no forward-mode derivative: a tensor with a tangent came in");
+}
 // a tensor was changed in place: a graph that saved it has to notice (tensors of inference mode are in none)
 void written(const Tensor& t) { if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version(); }
 // gradients of a backward pass that was asked for its own graph: they have none, and say so when it is used
@@ -158,6 +163,8 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &r = saved[1], &i = saved[2], &decay = saved[3], &checkpoint = saved[5];
+        const Maybe arrived[2] = {maybe(grads[0]), maybe(grads[1])};
+        no_tangents({&arrived[0], &arrived[1]}, "gated_scan's backward pass");
         Tensor dx, dr, di, ddecay, dh0;
         {
             at::AutoDispatchBelowADInplaceOrView below;
@@ -219,6 +226,7 @@ std::tuple<Tensor, Tensor> gated_scan(Tensor x, Tensor r, Tensor i, const Tensor
     r = rows_of(r);
     i = rows_of(i);
     const Maybe mx(x), mr(r), mi(i), md(decay);
+    no_tangents({&mx, &mr, &mi, &md, &h0}, "gated_scan");
     if (tracked({&mx, &mr, &mi, &md, &h0})) {
         auto o = GatedScan::apply(x, r, i, decay, h0, reset, c);
         return {o[0], o[1]};
@@ -232,6 +240,7 @@ Tensor gated_scan_step(Tensor x, Tensor r, Tensor i, const Tensor& decay, const 
     same_device(x, state, "state");
     REFUSE_IF(state.sizes() != x.sizes() || state.scalar_type() != at::kFloat || !state.is_contiguous(), "state has to be a contiguous float32 tensor of ", x.sizes());
     const Maybe mx(x), mr(r), mi(i), md(decay), ms(state);
+    no_tangents({&mx, &mr, &mi, &md, &ms}, "gated_scan_step");
     REFUSE_IF(tracked({&mx, &mr, &mi, &md, &ms}), "gated_scan_step has no gradients: call it under torch.no_grad(), or gated_scan with one step");
     x = rows_of(x);
     r = rows_of(r);
@@ -320,6 +329,8 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
         const Tensor& x = saved[0];
         const Maybe u = maybe(saved[1]), gate = maybe(saved[2]), scale = maybe(saved[3]), post = maybe(saved[4]), pre = maybe(saved[5]);
         const Tensor dy = u ? grads[0] : Tensor(), dz = pre ? grads.back() : Tensor();
+        const Maybe arrived[2] = {maybe(dy), maybe(dz)};
+        no_tangents({&arrived[0], &arrived[1]}, "block_norm's backward pass");
         variable_list d(9);
         if (!dy.defined() && !dz.defined()) return d;
         {
@@ -376,6 +387,7 @@ std::tuple<Maybe, Maybe> block_norm(const Tensor& x, const Maybe& u, const Maybe
     }
     Tensor y, z;
     const Maybe mx(x);
+    no_tangents({&mx, &u, &gate, &scale, &post, &pre}, "block_norm");
     if (tracked({&mx, &u, &gate, &scale, &post, &pre})) {
         auto o = BlockNorm::apply(x, u, gate, scale, post, pre, (int64_t)u_type, eps, fn);
         if (u) y = o[0];
@@ -417,6 +429,8 @@ Maybe adamw_step(const std::vector<Tensor>& params, const std::vector<Maybe>& gr
         Tensor g = *grads[k];
         const int64_t n = p.numel();
         const int code = code_of(p.scalar_type());
+        const Maybe mp(p);
+        no_tangents({&mp, &grads[k]}, "adamw_step");
         REFUSE_IF(code < 0 || !p.is_contiguous() || p.device() != step.device(), "parameter ", k, " has to be a contiguous float32, bfloat16 or float16 tensor on ", step.device());
         REFUSE_IF(g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes() || g.device() != step.device(),
                   "gradient ", k, " has to match its parameter: ", p.sizes(), " ", name_of(p.scalar_type()), " on ", step.device());

@@ -171,3 +171,26 @@ def test_only_the_gradients_that_are_asked_for(interpreter):
 
 def test_norm_of_rows_far_apart(interpreter):
     cases.run_norm_of_rows_far_apart(interpreter)
+
+
+# ---- what torch carries beside a tensor's values, or records of a call, and a kernel does not see
+def test_forward_mode_tangents_are_refused(interpreter):
+    import torch.autograd.forward_ad as forward_ad
+    x, r, i, decay, h0 = (t.detach() for t in leaves((2, 7, 8), (2, 7, 8), (2, 7, 8), (8,), (2, 8)))
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))                                     # noqa: E731
+        for call in (lambda: P.gated_scan(dual(x), r, i, decay), lambda: P.gated_scan(x, r, i, dual(decay)), lambda: P.gated_scan(x, r, i, decay, dual(h0)),
+                     lambda: P.gated_scan_step(dual(x[:, 0]), r[:, 0], i[:, 0], decay, h0), lambda: P.gated_scan_step(x[:, 0], r[:, 0], i[:, 0], decay, dual(h0)),
+                     lambda: P.block_norm(dual(x), pre=decay), lambda: P.block_norm(x, dual(r)), lambda: P.block_norm(x, r, pre=dual(decay)),
+                     lambda: adamw_step([dual(decay)], [decay.clone()], [torch.zeros(8)], [torch.zeros(8)], torch.zeros(2, dtype=torch.int64)),
+                     lambda: adamw_step([decay], [dual(decay.clone())], [torch.zeros(8)], [torch.zeros(8)], torch.zeros(2, dtype=torch.int64))):
+            with pytest.raises(ValueError, match="no forward-mode derivative"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="no forward-mode derivative"):      # (tangents are carried there too)
+                call()
+        leaf = x.clone().requires_grad_()                    # a tangent that only the gradient has: through a weight behind the operator
+        for out in (P.gated_scan(leaf, r, i, decay)[0], P.gated_scan(leaf, r, i, decay)[1], P.block_norm(leaf, r)[0], P.block_norm(leaf, r, pre=decay)[1]):
+            with pytest.raises((ValueError, RuntimeError), match="no forward-mode derivative"):
+                torch.autograd.grad((out * dual(torch.ones_like(out))).sum(), leaf)
+        with forward_ad._set_fwd_grad_enabled(False):        # where torch itself leaves tangents out
+            assert torch.equal(P.gated_scan(dual(x), r, i, decay)[0], P.gated_scan(x, r, i, decay)[0])
