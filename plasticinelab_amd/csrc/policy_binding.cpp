@@ -4,8 +4,10 @@
 // (1, 128) 5.5 us, with the same checks in Python 10.7; forward and backward of (16, 50, 256) 94 us, 159 in Python (torch's own product and its
 // backward, nothing else: 49); an update of 20 tensors 14 us, 48 in Python.
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -56,12 +58,22 @@ std::string name_of(at::ScalarType t) {
 }
 int code_of(at::ScalarType t) { return t == at::kFloat ? PLMPM_NN_F32 : t == at::kBFloat16 ? PLMPM_NN_BF16 : t == at::kHalf ? PLMPM_NN_F16 : -1; }
 
+// What records the operations of a program sees a call's allocations and not its kernels: the recorded program would return memory that nothing wrote to.
+void not_recorded() {
+    if (torch::jit::tracer::isTracing()) throw EngineError("policy operators cannot be traced (torch.jit.trace): their kernels would be missing from the graph");
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    using Key = c10::impl::TorchDispatchModeKey;
+    bool found = c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
+    if (Modes::any_modes_set()) for (const Key key : {Key::PROXY, Key::FAKE, Key::FUNCTIONAL}) found = found || Modes::get_mode(key).has_value();
+    if (found) throw EngineError("policy operators cannot be traced (make_fx, fake or functional tensors): their kernels would be missing from the graph");
+}
 // the device that a call's kernels go to, made current, and its current stream
 struct Site {
     c10::OptionalDeviceGuard guard;
     void* stream = nullptr;
     explicit Site(const Tensor& t) {
         if (!lib.last_error) throw EngineError("the library is not loaded");
+        not_recorded();
         if (lib.host && t.is_cpu()) return;
         if (!t.is_cuda())
             throw EngineError("policy operators run on a ROCm device, got a tensor on " + t.device().str() + ": there is no CPU path");

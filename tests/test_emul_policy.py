@@ -194,3 +194,25 @@ def test_forward_mode_tangents_are_refused(interpreter):
                 torch.autograd.grad((out * dual(torch.ones_like(out))).sum(), leaf)
         with forward_ad._set_fwd_grad_enabled(False):        # where torch itself leaves tangents out
             assert torch.equal(P.gated_scan(dual(x), r, i, decay)[0], P.gated_scan(x, r, i, decay)[0])
+
+
+def test_recorders_of_programs_are_refused(interpreter):
+    """A traced program would hold the calls' allocations without their kernels and hand out what happens to lie in that memory."""
+    from torch._subclasses import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, r, i, decay = leaves((2, 7, 8), (2, 7, 8), (2, 7, 8), (8,))
+    plain = [t.detach() for t in (x, r, i, decay)]
+    first, second, step = [torch.zeros(8)], [torch.zeros(8)], torch.zeros(2, dtype=torch.int64)
+    h = P.gated_scan(x, r, i, decay)[0]
+    calls = (lambda t: P.gated_scan(t, *plain[1:])[0], lambda t: P.gated_scan_step(t[:, 0], plain[1][:, 0], plain[2][:, 0], plain[3], torch.zeros(2, 8)), lambda t: P.block_norm(t, plain[1])[0],
+             lambda t: P.block_norm(t, pre=plain[3])[1], lambda t: P.gated_scan(t.detach().requires_grad_(), *plain[1:])[0], lambda t: torch.autograd.grad(h, x, t, retain_graph=True)[0],
+             lambda t: adamw_step([t[0, 0]], [plain[3]], first, second, step) or t + 1)
+    for call in calls:
+        for record in (lambda f, t: torch.jit.trace(f, (t,), check_trace=False), lambda f, t: make_fx(f)(t), lambda f, t: make_fx(f, pre_dispatch=True)(t)):
+            with pytest.raises(RuntimeError, match="cannot be traced|Cannot insert a Tensor that requires grad"):      # (the second: torch's own, of a backward pass)
+                record(call, plain[0].clone())
+    with FakeTensorMode() as mode, pytest.raises(_lib.EngineError, match="cannot be traced"):
+        P.block_norm(mode.from_tensor(plain[0]), mode.from_tensor(plain[1]))
+    from torch.utils.flop_counter import FlopCounterMode           # a mode that only looks on
+    with FlopCounterMode(display=False):
+        assert torch.equal(P.gated_scan(*plain)[0], h)
