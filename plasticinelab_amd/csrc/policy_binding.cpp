@@ -82,8 +82,24 @@ struct Site {
     }
 };
 
-const void* ptr(const Maybe& t) { return t ? t->data_ptr() : nullptr; }
-template <class T = void> T* out(const Tensor& t) { return t.defined() ? (T*)t.data_ptr() : nullptr; }
+// Kernels read memory.  What torch has only noted beside it is applied first: a sign (x.conj().imag and gradients of complex products are such views), zeros
+// that were never stored.  What is written in place has to be without.
+void settle(Tensor& t) {
+    if (t.is_neg()) t = t.resolve_neg();
+    if (t._is_zerotensor()) t = at::zeros(t.sizes(), t.options()).add(t);
+}
+void settle(Maybe& t) { if (t) settle(*t); }
+void settled(const Tensor& t, const char* name) {
+    REFUSE_IF(t.is_neg() || t._is_zerotensor(), name, " is written in place: it cannot be a negative view or a tensor of zeros without memory");
+}
+// where a tensor's values lie; a null pointer would be read as a tensor that was not given
+void* memory(const Tensor& t) {
+    void* p = t.data_ptr();
+    if (!p && t.numel()) throw EngineError("a tensor came in that holds no memory (a wrapper of one of torch's transforms)");
+    return p;
+}
+const void* ptr(const Maybe& t) { return t ? memory(*t) : nullptr; }
+template <class T = void> T* out(const Tensor& t) { return t.defined() ? (T*)memory(t) : nullptr; }
 Tensor workspace(const Tensor& like, size_t bytes) { return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor(); }
 Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); }
 
@@ -130,10 +146,10 @@ plmpm_scan scan_of(const Tensor& x, const Tensor& r, const Tensor& i, const Tens
     const Tensor* in[3] = {&x, &r, &i};
     for (int k = 0; k < 3; ++k) { s.stride_b[k] = in[k]->stride(0); s.stride_t[k] = in[k]->stride(1); }
     s.c = c;
-    s.x = x.data_ptr();
-    s.r = r.data_ptr();
-    s.i = i.data_ptr();
-    s.decay = (const float*)decay.data_ptr();
+    s.x = memory(x);
+    s.r = memory(r);
+    s.i = memory(i);
+    s.decay = out<float>(decay);
     s.reset = (const uint8_t*)ptr(reset);
     return s;
 }
@@ -186,7 +202,12 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
             di = at::empty({B, T, D}, x.options());
             ddecay = at::empty({D}, decay.options());
             if (ctx->saved_data["h0"].toBool()) dh0 = at::empty({B, D}, decay.options());
-            const Tensor dh = grads[0].defined() ? grads[0].contiguous() : Tensor(), dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
+            Tensor dh, dlast;
+            for (const auto& [to, k] : {std::pair(&dh, 0), std::pair(&dlast, 1)})
+                if (grads[k].defined()) {
+                    settle(grads[k]);
+                    *to = grads[k].contiguous();
+                }
             if (B && T && D) {
                 plmpm_scan s = scan_of(x, r, i, decay, maybe(saved[4]), ctx->saved_data["c"].toDouble());
                 s.checkpoint = out<float>(checkpoint);
@@ -220,12 +241,13 @@ void check_scan(const Tensor& x, const Tensor& r, const Tensor& i, const Tensor&
     REFUSE_IF(!(c > 0.0 && c < 1e30), "c has to be positive and finite, got ", c);
 }
 
-std::tuple<Tensor, Tensor> gated_scan(Tensor x, Tensor r, Tensor i, const Tensor& decay, Maybe h0, Maybe reset, double c) {
+std::tuple<Tensor, Tensor> gated_scan(Tensor x, Tensor r, Tensor i, Tensor decay, Maybe h0, Maybe reset, double c) {
     check_scan(x, r, i, decay, c, 3);
     if (h0) {
         same_device(x, *h0, "h0");
         REFUSE_IF(h0->dim() != 2 || h0->size(0) != x.size(0) || h0->size(1) != x.size(2) || h0->scalar_type() != at::kFloat,
                   "h0 has to be float32 (", x.size(0), ", ", x.size(2), "), got ", h0->sizes(), " ", name_of(h0->scalar_type()));
+        settle(h0);
         h0 = h0->contiguous();
     }
     if (reset) {
@@ -234,9 +256,11 @@ std::tuple<Tensor, Tensor> gated_scan(Tensor x, Tensor r, Tensor i, const Tensor
                   "reset has to be bool (", x.size(0), ", ", x.size(1), "), got ", reset->sizes(), " ", name_of(reset->scalar_type()));
         reset = reset->contiguous();
     }
-    x = rows_of(x);
-    r = rows_of(r);
-    i = rows_of(i);
+    for (Tensor* t : {&x, &r, &i}) {
+        settle(*t);
+        *t = rows_of(*t);
+    }
+    settle(decay);
     const Maybe mx(x), mr(r), mi(i), md(decay);
     no_tangents({&mx, &mr, &mi, &md, &h0}, "gated_scan");
     if (tracked({&mx, &mr, &mi, &md, &h0})) {
@@ -247,16 +271,19 @@ std::tuple<Tensor, Tensor> gated_scan(Tensor x, Tensor r, Tensor i, const Tensor
     return {h, last};
 }
 
-Tensor gated_scan_step(Tensor x, Tensor r, Tensor i, const Tensor& decay, const Tensor& state, double c) {
+Tensor gated_scan_step(Tensor x, Tensor r, Tensor i, Tensor decay, const Tensor& state, double c) {
     check_scan(x, r, i, decay, c, 2);
     same_device(x, state, "state");
+    settled(state, "state");
     REFUSE_IF(state.sizes() != x.sizes() || state.scalar_type() != at::kFloat || !state.is_contiguous(), "state has to be a contiguous float32 tensor of ", x.sizes());
     const Maybe mx(x), mr(r), mi(i), md(decay), ms(state);
     no_tangents({&mx, &mr, &mi, &md, &ms}, "gated_scan_step");
     REFUSE_IF(tracked({&mx, &mr, &mi, &md, &ms}), "gated_scan_step has no gradients: call it under torch.no_grad(), or gated_scan with one step");
-    x = rows_of(x);
-    r = rows_of(r);
-    i = rows_of(i);
+    for (Tensor* t : {&x, &r, &i}) {
+        settle(*t);
+        *t = rows_of(*t);
+    }
+    settle(decay);
     const Tensor h = at::empty({x.size(0), x.size(1)}, x.options());
     if (h.numel()) {
         plmpm_scan s{};
@@ -268,10 +295,10 @@ Tensor gated_scan_step(Tensor x, Tensor r, Tensor i, const Tensor& decay, const 
         s.stride_b[1] = r.stride(0);
         s.stride_b[2] = i.stride(0);
         s.c = c;
-        s.x = x.data_ptr();
-        s.r = r.data_ptr();
-        s.i = i.data_ptr();
-        s.decay = (const float*)decay.data_ptr();
+        s.x = memory(x);
+        s.r = memory(r);
+        s.i = memory(i);
+        s.decay = out<float>(decay);
         s.h0 = out<float>(state);
         s.h = out(h);
         s.h_last = out<float>(state);
@@ -307,7 +334,7 @@ struct NormCall {
         k = rows_of(t.dim() == 2 ? t : t.reshape({-1, n.width}));
         if (k.size(0) > 1 && k.stride(0) >= kFarRows) k = k.contiguous();
         stride = k.size(0) > 1 ? k.stride(0) : n.width;
-        return k.data_ptr();
+        return memory(k);
     }
 };
 std::tuple<Tensor, Tensor> norm_forward(const Tensor& x, const Maybe& u, const Maybe& gate, const Maybe& scale, const Maybe& post, const Maybe& pre, at::ScalarType u_type, double eps, int64_t fn) {
@@ -340,13 +367,14 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
         const auto saved = ctx->get_saved_variables();
         const Tensor& x = saved[0];
         const Maybe u = maybe(saved[1]), gate = maybe(saved[2]), scale = maybe(saved[3]), post = maybe(saved[4]), pre = maybe(saved[5]);
-        const Tensor dy = u ? grads[0] : Tensor(), dz = pre ? grads.back() : Tensor();
+        Tensor dy = u ? grads[0] : Tensor(), dz = pre ? grads.back() : Tensor();
         const Maybe arrived[2] = {maybe(dy), maybe(dz)};
         no_tangents({&arrived[0], &arrived[1]}, "block_norm's backward pass");
         variable_list d(9);
         if (!dy.defined() && !dz.defined()) return d;
         {
             at::AutoDispatchBelowADInplaceOrView below;
+            for (Tensor* t : {&dy, &dz}) if (t->defined()) settle(*t);
             for (int k = 0; k < 6; ++k) if (saved[k].defined()) d[k] = at::empty(saved[k].sizes(), saved[k].options());
             if (x.numel()) {
                 const Site site(x);
@@ -373,7 +401,8 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
     }
 };
 
-std::tuple<Maybe, Maybe> block_norm(const Tensor& x, const Maybe& u, const Maybe& gate, const Maybe& scale, const Maybe& post, const Maybe& pre, double eps, int64_t fn, std::optional<at::ScalarType> dtype) {
+std::tuple<Maybe, Maybe> block_norm(const Tensor& given, Maybe u, Maybe gate, Maybe scale, Maybe post, Maybe pre, double eps, int64_t fn, std::optional<at::ScalarType> dtype) {
+    Tensor x = given;
     REFUSE_IF(x.dim() < 1, "x has to be a tensor with at least one dimension");
     const std::pair<const Maybe*, const char*> others[5] = {{&u, "u"}, {&gate, "gate"}, {&scale, "scale"}, {&post, "post"}, {&pre, "pre"}};
     for (const auto& [t, name] : others) if (*t) same_device(x, **t, name);
@@ -397,6 +426,8 @@ std::tuple<Maybe, Maybe> block_norm(const Tensor& x, const Maybe& u, const Maybe
         REFUSE_IF(w->dim() != 1 || w->size(0) != D || !w->is_contiguous() || w->scalar_type() != (*first)->scalar_type() || code_of(w->scalar_type()) < 0,
                   others[k].second, " has to be a contiguous tensor of ", D, " values, of one floating type with the other weights");
     }
+    settle(x);
+    for (Maybe* t : {&u, &gate, &scale, &post, &pre}) settle(*t);
     Tensor y, z;
     const Maybe mx(x);
     no_tangents({&mx, &u, &gate, &scale, &post, &pre}, "block_norm");
@@ -406,19 +437,21 @@ std::tuple<Maybe, Maybe> block_norm(const Tensor& x, const Maybe& u, const Maybe
         if (pre) z = o.back();
     } else
         std::tie(y, z) = norm_forward(x, u, gate, scale, post, pre, u_type, eps, fn);
-    return {u ? Maybe(y) : Maybe(x), maybe(z)};
+    return {u ? y : given, maybe(z)};
 }
 
 // ---------------------------------------------------------------------------------------------- AdamW
 float* plain(const Tensor& t, int64_t n, const Tensor& step, const char* name, size_t k) {
     REFUSE_IF(t.scalar_type() != at::kFloat || t.numel() != n || !t.is_contiguous() || t.device() != step.device(),
               name, " ", k, " has to be ", n, " contiguous float32 values on the parameters' device");
-    return (float*)t.data_ptr();
+    settled(t, name);
+    return out<float>(t);
 }
 void* codes_of(const Tensor& t, int64_t n, const Tensor& step, at::ScalarType type, const char* name, size_t k) {
     REFUSE_IF(t.scalar_type() != type || t.numel() != n || !t.is_contiguous() || t.device() != step.device(),
               name, " ", k, ": codes have to be ", n, " contiguous ", name_of(type), " values on the parameters' device");
-    return t.data_ptr();
+    settled(t, name);
+    return memory(t);
 }
 int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }
 
@@ -429,6 +462,7 @@ Maybe adamw_step(const std::vector<Tensor>& params, const std::vector<Maybe>& gr
     REFUSE_IF(grads.size() != count || first.size() != count || second.size() != count || (!masters.empty() && masters.size() != count),
               "params, grads, first, second and masters have to be of one length");
     REFUSE_IF(step.dim() != 1 || step.size(0) != 2 || step.scalar_type() != at::kLong || !step.is_contiguous(), "step has to be an int64 tensor of two values");
+    settled(step, "step");
     std::vector<plmpm_adamw_tensor> table;
     std::vector<Tensor> keep;
     std::vector<size_t> touched;
@@ -446,13 +480,13 @@ Maybe adamw_step(const std::vector<Tensor>& params, const std::vector<Maybe>& gr
         REFUSE_IF(code < 0 || !p.is_contiguous() || p.device() != step.device(), "parameter ", k, " has to be a contiguous float32, bfloat16 or float16 tensor on ", step.device());
         REFUSE_IF(g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes() || g.device() != step.device(),
                   "gradient ", k, " has to match its parameter: ", p.sizes(), " ", name_of(p.scalar_type()), " on ", step.device());
-        if (!g.is_contiguous()) {
-            g = g.contiguous();
-            keep.push_back(g);
-        }
+        settled(p, "a parameter");
+        settle(g);
+        g = g.contiguous();
+        if (!g.is_same(*grads[k])) keep.push_back(g);
         plmpm_adamw_tensor t{};
-        t.p = p.data_ptr();
-        t.g = g.data_ptr();
+        t.p = memory(p);
+        t.g = memory(g);
         t.n = n;
         t.dtype = code;
         if (bits == 8) {
@@ -493,8 +527,8 @@ Maybe adamw_step(const std::vector<Tensor>& params, const std::vector<Maybe>& gr
     a.max_norm = max_norm;
     a.lo = lo;
     a.hi = hi;
-    a.step = (int64_t*)step.data_ptr();
-    a.grad_norm = norm ? (float*)norm->data_ptr() : nullptr;
+    a.step = out<int64_t>(step);
+    a.grad_norm = norm ? out<float>(*norm) : nullptr;
     size_t need = 0;
     check(lib.adamw_workspace(&a, table.data(), (int)table.size(), &need));
     const Tensor work = workspace(step, need);

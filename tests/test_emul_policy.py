@@ -216,3 +216,57 @@ def test_recorders_of_programs_are_refused(interpreter):
     from torch.utils.flop_counter import FlopCounterMode           # a mode that only looks on
     with FlopCounterMode(display=False):
         assert torch.equal(P.gated_scan(*plain)[0], h)
+
+
+@pytest.mark.parametrize("how", ["imag", "view"])
+def test_negative_views_and_zeros_without_memory(interpreter, how):
+    """x.conj().imag and the gradients of complex products are views with a sign that torch only notes: the operators see the values."""
+    B, T, D = 2, 7, 8
+    noted = lambda t: torch.complex(torch.zeros_like(t), t).conj().imag if how == "imag" and t.dim() > 1 else torch._neg_view(t)                  # noqa: E731
+    args = leaves((B, T, D), (B, T, D), (B, T, D), (D,), (B, D))
+    minus = [noted(t) for t in args]
+    assert all(t.is_neg() for t in minus)
+    for one, other in ((P.gated_scan(*minus), P.gated_scan(*[-t for t in args])), (P.gated_scan(*[t.detach() for t in minus]), P.gated_scan(*[-t for t in args]))):
+        assert all(torch.equal(a, b) for a, b in zip(one, other))
+    x, r, i, decay, h0 = args
+    weights = [noted(t) for t in leaves((D,), (D,), (D,))]
+    for a, b in zip(P.block_norm(minus[0], minus[1], minus[2], *weights), P.block_norm(-x, -r, -i, *[w.clone() for w in weights])):
+        assert torch.equal(a, b)
+    y, z = P.block_norm(minus[0], pre=weights[0])
+    assert y is minus[0] and torch.equal(z, P.block_norm(-x, pre=weights[0].clone())[1])
+    out = P.gated_scan_step(*[t.detach()[:, 0] for t in minus[:3]], minus[3].detach(), h0.detach().clone())
+    assert torch.equal(out, P.gated_scan_step(*[-t.detach()[:, 0] for t in args[:3]], -decay.detach(), h0.detach().clone()))
+    # gradients of the inputs, and incoming ones
+    for call in (lambda s: P.gated_scan(s[0], s[1], s[2], s[3], s[4])[0], lambda s: P.gated_scan(s[0], s[1], s[2], s[3], s[4])[1], lambda s: P.block_norm(s[0], s[1], s[2], s[3], s[3], s[3])[0],
+                 lambda s: P.block_norm(s[0], s[1], s[2], s[3], s[3], s[3])[1]):
+        got = torch.autograd.grad(call([noted(t) for t in args]).square().sum(), args, allow_unused=True)
+        want = torch.autograd.grad(call([-t for t in args]).square().sum(), args, allow_unused=True)
+        assert all((a is None and b is None) or torch.equal(a, b) for a, b in zip(got, want))
+        value = call(args)
+        got = torch.autograd.grad(value, args, torch._neg_view(torch.ones_like(value)), allow_unused=True, retain_graph=True)
+        want = torch.autograd.grad(value, args, -torch.ones_like(value), allow_unused=True, retain_graph=True)
+        assert all((a is None and b is None) or torch.equal(a, b) for a, b in zip(got, want))
+        got = torch.autograd.grad(value, args, torch._efficientzerotensor(value.shape), allow_unused=True)
+        assert all(a is None or float(a.abs().sum()) == 0 for a in got)
+    zeros = torch._efficientzerotensor((B, T, D))
+    assert torch.equal(P.block_norm(x, zeros, pre=weights[0])[0], x) and torch.equal(P.gated_scan(zeros, r, i, decay)[1], torch.zeros(B, D))
+    # an update: the gradient's values; nothing that it writes to
+    p, one, two = (torch.ones(D) for _ in range(3))
+    new = lambda: [torch.zeros(D)]                                                                       # noqa: E731
+    count = lambda: torch.zeros(2, dtype=torch.int64)                                                    # noqa: E731
+    adamw_step([one], [noted(decay).detach()], new(), new(), count())
+    adamw_step([two], [-decay.detach()], new(), new(), count())
+    assert torch.equal(one, two)
+    for args in (([torch._neg_view(p)], [p.clone()], new(), new(), count()), ([p], [p.clone()], [torch._neg_view(p.clone())], new(), count()),
+                 ([p], [p.clone()], new(), new(), torch._neg_view(count())), ([p.half()], [p.half()], new(), new(), count(), [torch._neg_view(p.clone())])):
+        masters = {"masters": args[5]} if len(args) > 5 else {}
+        with pytest.raises(ValueError, match="written in place"):
+            adamw_step(*args[:5], **masters)
+    with pytest.raises(ValueError, match="written in place"):
+        P.gated_scan_step(*[t.detach()[:, 0] for t in (x, r, i)], decay.detach(), torch._neg_view(h0.detach()))
+
+
+def test_wrappers_without_memory_are_refused(interpreter):
+    x, r = (t.detach() for t in leaves((4, 8), (4, 8)))
+    with pytest.raises(_lib.EngineError, match="holds no memory"):
+        torch.func.functionalize(lambda u: P.block_norm(x, u)[0])(r)
