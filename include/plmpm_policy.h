@@ -80,7 +80,8 @@ int plmpm_norm_backward(const plmpm_norm* n, void* hip_stream);
  *   w = clip(w - lr weight_decay w - lr / (1 - beta_1^t) m / (sqrt(v / (1 - beta_2^t)) + epsilon), lo, hi)
  * w is the float master where one is given (the 16-bit parameter is then its rounding), else the parameter itself.
  * State of 32 bits: float m, v.  State of 8 bits: blocks of 256 elements with a float scale s, the block's largest magnitude:
- * m = s sign(c) (c / 127)^2 with int8 c, v = s (c / 255)^4 with uint8 c, where a v above zero keeps a code above zero. */
+ * m = s sign(c) (c / 127)^2 with int8 c, v = s (c / 255)^4 with uint8 c, where a v above zero keeps a code above zero.
+ * What a call writes may not overlap anything else of the call, except that a gradient may be its parameter itself. */
 typedef struct plmpm_adamw_tensor {
     void* p;
     const void* g;                          /* of the parameter's type */

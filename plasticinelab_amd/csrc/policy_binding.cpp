@@ -454,6 +454,25 @@ void* codes_of(const Tensor& t, int64_t n, const Tensor& step, at::ScalarType ty
     return memory(t);
 }
 int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }
+// The memory that a call touches through its lists of tensors: what it writes it may touch through one of them only, or two updates would race.
+struct Touched {
+    struct Range {
+        uintptr_t from, to;
+        bool written;
+    };
+    std::vector<Range> ranges;
+    void add(const void* p, int64_t bytes, bool written) { if (p && bytes) ranges.push_back({(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, written}); }
+    bool races() {
+        std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.from < b.from; });
+        uintptr_t end[2] = {0, 0};      // of what was read or written so far; of what was written
+        for (const Range& r : ranges) {
+            if (r.from < end[r.written ? 0 : 1]) return true;
+            end[0] = std::max(end[0], r.to);
+            if (r.written) end[1] = std::max(end[1], r.to);
+        }
+        return false;
+    }
+};
 
 Maybe adamw_step(const std::vector<Tensor>& params, const std::vector<Maybe>& grads, const std::vector<Tensor>& first, const std::vector<Tensor>& second,
                  const std::vector<Tensor>& first_scales, const std::vector<Tensor>& second_scales, const std::vector<Maybe>& masters, const Tensor& step, int64_t bits,
@@ -466,9 +485,10 @@ Maybe adamw_step(const std::vector<Tensor>& params, const std::vector<Maybe>& gr
     std::vector<plmpm_adamw_tensor> table;
     std::vector<Tensor> keep;
     std::vector<size_t> touched;
-    std::vector<const void*> written_to;
+    Touched memory_of;
     table.reserve(count);
-    written_to.reserve(6 * count);
+    memory_of.ranges.reserve(5 * count + 1);
+    memory_of.add(memory(step), 2 * sizeof(int64_t), true);
     for (size_t k = 0; k < count; ++k) {
         if (!grads[k]) continue;
         const Tensor& p = params[k];
@@ -503,13 +523,18 @@ Maybe adamw_step(const std::vector<Tensor>& params, const std::vector<Maybe>& gr
             t.master = plain(*masters[k], n, step, "master", k);
         }
         if (!n) continue;
-        for (const void* p : {(const void*)t.p, (const void*)t.m, (const void*)t.v, (const void*)t.m_scale, (const void*)t.v_scale, (const void*)t.master}) if (p) written_to.push_back(p);
+        const int64_t size = p.element_size(), moment = n * (bits == 8 ? 1 : sizeof(float));
+        memory_of.add(t.p, n * size, true);
+        if (t.g != t.p) memory_of.add(t.g, n * size, false);       // (the parameter itself as its gradient: each element is read before it is written)
+        memory_of.add(t.m, moment, true);
+        memory_of.add(t.v, moment, true);
+        memory_of.add(t.m_scale, blocks_of(n) * sizeof(float), true);
+        memory_of.add(t.v_scale, blocks_of(n) * sizeof(float), true);
+        memory_of.add(t.master, n * sizeof(float), true);
         table.push_back(t);
         touched.push_back(k);
     }
-    std::sort(written_to.begin(), written_to.end());
-    REFUSE_IF(std::adjacent_find(written_to.begin(), written_to.end()) != written_to.end(),
-              "a parameter, a moment of it or its master is in the list twice: the updates would race");
+    REFUSE_IF(memory_of.races(), "a parameter, a moment of it, its master or step is in the list twice, or overlaps another tensor of the call: the updates would race");
     Maybe norm;
     if (max_norm > 0) norm = at::empty({}, step.options().dtype(at::kFloat));
     if (table.empty()) {
@@ -548,6 +573,7 @@ void adamw_values(const std::vector<Tensor>& codes, const std::vector<Tensor>& s
     std::vector<float*> o;
     std::vector<int64_t> sizes;
     std::vector<int32_t> which;
+    Touched memory_of;
     for (size_t k = 0; k < count; ++k) {
         const int64_t n = codes[k].numel();
         const at::ScalarType type = codes[k].scalar_type();
@@ -557,7 +583,11 @@ void adamw_values(const std::vector<Tensor>& codes, const std::vector<Tensor>& s
         o.push_back(plain(values[k], n, codes[0], "out", k));
         sizes.push_back(n);
         which.push_back(type == at::kByte);
+        memory_of.add(c.back(), n, false);
+        memory_of.add(s.back(), blocks_of(n) * sizeof(float), false);
+        memory_of.add(o.back(), n * sizeof(float), true);
     }
+    REFUSE_IF(memory_of.races(), "a tensor of out is in the list twice, or overlaps another tensor of the call");
     const Site site(codes[0]);
     check(lib.adamw_values(c.data(), s.data(), o.data(), sizes.data(), which.data(), (int)count, site.stream));
     for (const Tensor& t : values) written(t);

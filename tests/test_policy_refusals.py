@@ -130,3 +130,34 @@ def test_c_entries_check_before_they_launch():
     t[0].n = 0
     assert lib.plmpm_adamw_step(_lib.AdamWStep(**ok), t, 1, None) == 0
     assert lib.plmpm_adamw_values(None, None, None, None, None, 1, None) != 0 and "null" in error()
+
+
+def test_adamw_refuses_tensors_that_share_memory():
+    """Whatever an update writes: the other tensor begins before it, behind its start, or is what another parameter reads."""
+    n, step = 300, torch.zeros(2, dtype=torch.int64)
+    z = lambda dt=torch.float32: torch.zeros(n, dtype=dt)                                                # noqa: E731
+    wide = torch.zeros(2 * n)
+    halves, shifted = [wide[:n], wide[n:]], [wide[:n], wide[n - 1:2 * n - 1]]
+    eight = lambda: ((z(torch.int8), torch.zeros(2)), (z(torch.uint8), torch.zeros(2)))                  # noqa: E731
+    a, b = eight(), eight()
+    scales = torch.zeros(3)
+    two = lambda: [z(), z()]                                                                             # noqa: E731
+    words = torch.zeros(n, dtype=torch.int64)
+    for args, kw in (((shifted, two(), two(), two(), step), {}), ((shifted[::-1], two(), two(), two(), step), {}), ((two(), two(), shifted, two(), step), {}), ((two(), two(), two(), shifted, step), {}),
+                     (([z()], [wide[:n]], [wide[n - 1:2 * n - 1]], [z()], step), {}), ((halves, [wide[1:n + 1], z()], two(), two(), step), {}), ((halves, [z(), wide[:n]], two(), two(), step), {}),
+                     (([z(torch.float16)], [z(torch.float16)], [wide[:n]], [z()], step), {"masters": [wide[1:n + 1]]}),
+                     (([words.view(torch.float32)[:n]], [z()], [z()], [z()], words[1:3]), {}),
+                     ((two(), two(), [(a[0][0], scales[:2]), (b[0][0], scales[1:])], [a[1], b[1]], step), {}), ((two(), two(), [a[0], b[0]], [(a[1][0], scales[:2]), (b[1][0], scales[1:])], step), {})):
+        with pytest.raises(ValueError, match="overlaps"):
+            adamw_step(*args, **kw)
+    g = z()                                                  # side by side, a gradient for two, a gradient that is its parameter: on to the check of the device
+    for args in ((halves, [g, g], two(), two(), step), ([g], [g], [z()], [z()], step)):
+        with pytest.raises(_lib.EngineError, match="no CPU path"):
+            adamw_step(*args)
+    codes = lambda: (z(torch.int8), torch.zeros(2))                                                      # noqa: E731
+    for moments, out in (([codes(), codes()], shifted), ([(wide.view(torch.int8)[4:4 + n], torch.zeros(2))], [wide[:n]]), ([(z(torch.int8), wide[n - 1:n + 1])], [wide[:n]])):
+        with pytest.raises(ValueError, match="overlaps"):
+            adamw_values(moments, out=out)
+    one = codes()
+    with pytest.raises(_lib.EngineError, match="no CPU path"):
+        adamw_values([one, one], out=halves)
