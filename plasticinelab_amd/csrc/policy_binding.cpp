@@ -560,7 +560,12 @@ Maybe adamw_step(const std::vector<Tensor>& params, const std::vector<Maybe>& gr
     a.workspace = out(work);
     a.workspace_bytes = need;
     check(lib.adamw_step(&a, table.data(), (int)table.size(), site.stream));
-    for (size_t k : touched) written(params[k]);
+    written(step);
+    for (size_t k : touched) {
+        for (const Tensor* t : {&params[k], &first[k], &second[k]}) written(*t);
+        if (bits == 8) for (const Tensor* t : {&first_scales[k], &second_scales[k]}) written(*t);
+        if (!masters.empty() && masters[k]) written(*masters[k]);
+    }
     return norm;
 }
 

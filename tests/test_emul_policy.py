@@ -270,3 +270,28 @@ def test_wrappers_without_memory_are_refused(interpreter):
     x, r = (t.detach() for t in leaves((4, 8), (4, 8)))
     with pytest.raises(_lib.EngineError, match="holds no memory"):
         torch.func.functionalize(lambda u: P.block_norm(x, u)[0])(r)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_graph_notices_whatever_an_update_changed(interpreter, bits):
+    """Moments, their scales, masters and the count are written in place like the parameters: a graph that saved one of them has to say so."""
+    n = 300
+    z = lambda dt=torch.float32, size=n: torch.zeros(size, dtype=dt)                                     # noqa: E731
+    p, master, step = z(torch.bfloat16), z(), z(torch.int64, 2)
+    first, second = ([z()], [z()]) if bits == 32 else ([(z(torch.int8), z(size=2))], [(z(torch.uint8), z(size=2))])
+    changed = [p, master, step] + [t for m in (first[0], second[0]) for t in (m if bits == 8 else [m])]
+    leaf = torch.ones((), requires_grad=True)
+    graphs = [(leaf * t).sum() for t in changed]
+    versions = [t._version for t in changed]
+    g = torch.ones(n, dtype=torch.bfloat16)
+    kept = (leaf * g).sum()
+    adamw_step([p], [g], first, second, step, masters=[master])
+    assert all(t._version > v for t, v in zip(changed, versions))
+    for loss in graphs:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    kept.backward()                                          # the gradient was only read
+    idle = z()
+    before = idle._version
+    adamw_step([idle], [None], [z()], [z()], step)
+    assert idle._version == before
