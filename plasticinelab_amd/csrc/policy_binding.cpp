@@ -271,6 +271,16 @@ std::tuple<Tensor, Tensor> gated_scan(Tensor x, Tensor r, Tensor i, Tensor decay
     return {h, last};
 }
 
+// whether two tensors' memory meets anywhere between the first and the last element of each
+bool meet(const Tensor& a, const Tensor& b) {
+    const auto end = [](const Tensor& t) {
+        int64_t last = 0;
+        for (int64_t k = 0; k < t.dim(); ++k) last += (t.size(k) - 1) * t.stride(k);
+        return (uintptr_t)memory(t) + (uintptr_t)((last + 1) * t.element_size());
+    };
+    return a.numel() && b.numel() && (uintptr_t)memory(a) < end(b) && (uintptr_t)memory(b) < end(a);
+}
+
 Tensor gated_scan_step(Tensor x, Tensor r, Tensor i, Tensor decay, const Tensor& state, double c) {
     check_scan(x, r, i, decay, c, 2);
     same_device(x, state, "state");
@@ -284,6 +294,9 @@ Tensor gated_scan_step(Tensor x, Tensor r, Tensor i, Tensor decay, const Tensor&
         *t = rows_of(*t);
     }
     settle(decay);
+    // an input that lies in the state would be read after another thread moved it on, unless each element is its own
+    for (Tensor* t : {&x, &r, &i}) if (meet(*t, state) && !(t->data_ptr() == state.data_ptr() && t->is_contiguous())) *t = t->clone(at::MemoryFormat::Contiguous);
+    if (meet(decay, state)) decay = decay.clone();
     const Tensor h = at::empty({x.size(0), x.size(1)}, x.options());
     if (h.numel()) {
         plmpm_scan s{};

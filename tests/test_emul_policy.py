@@ -295,3 +295,20 @@ def test_a_graph_notices_whatever_an_update_changed(interpreter, bits):
     before = idle._version
     adamw_step([idle], [None], [z()], [z()], step)
     assert idle._version == before
+
+
+def test_a_step_whose_inputs_lie_in_its_state(interpreter):
+    """A row of the state for every row's input, the state itself, a part of it as the decays: as with copies of them."""
+    B, D = 9, 130
+    x, r, i, decay, state = (t.detach() for t in leaves((B, D), (B, D), (B, D), (D,), (B, D)))
+    halves = torch.empty(2 * B * D - D)                      # the state, and an input that begins in its last row
+    for pick in (lambda s: (s[:1].expand(B, D), r, i, decay), lambda s: (x, s[2:3].expand(B, D), i, decay), lambda s: (x, r, s[-1:].expand(B, D), decay), lambda s: (s, s, s, decay),
+                 lambda s: (x, r, i, s[0]), lambda s: (x, r, i, s[B - 1]), lambda s: (s[0].view(D)[:1].expand(B, D), r, i, decay), lambda s: (halves[(B - 1) * D:].view(B, D), r, i, decay)):
+        halves.copy_(torch.linspace(-1, 1, halves.numel()))
+        mine = halves[:B * D].view(B, D)
+        mine.copy_(state)
+        args = pick(mine)
+        other = mine.clone()
+        want = P.gated_scan_step(*[t.clone().contiguous() for t in args], other)
+        got = P.gated_scan_step(*args, mine)
+        assert torch.equal(got, want) and torch.equal(mine, other)
