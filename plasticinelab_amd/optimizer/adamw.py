@@ -88,7 +88,8 @@ class AdamW(Optimizer):
     """``AdamW(parameters, cfg, **kw)``: parameters a list of tensors on one GPU; ``step(grads)`` (default: their ``.grad``) updates them in place
     and returns them.  Config keys beside Adam's: ``weight_decay``, ``state_bits`` (32 or 8), ``max_norm`` (of all gradients together, before the
     update; 0: no clipping).  16-bit parameters get a float32 master copy, which is made anew from a parameter that was written to between two
-    updates (torch's version counter says so; writes through ``.data`` go unnoticed).  ``grad_norm`` is the last norm (on the GPU)."""
+    updates (torch's version counter says so; writes through ``.data`` go unnoticed; before a capture ``renew_masters`` has to do it, since the copy would
+    be part of the graph and each replay would lose what the master holds beyond the parameter).  ``grad_norm`` is the last norm (on the GPU)."""
     extra_keys = {"lr": 1e-3, "bounds": (-np.inf, np.inf), "beta_1": 0.9, "beta_2": 0.999, "epsilon": 1e-8, "weight_decay": 0.01, "state_bits": 32, "max_norm": 0.0}
 
     def __init__(self, parameters, cfg=None, **kwargs):
@@ -137,12 +138,20 @@ class AdamW(Optimizer):
         return self._values("second")
 
     @torch.no_grad()
+    def renew_masters(self):
+        """Make the masters of parameters that were written to since the last update anew (``step`` does it by itself, outside a capture)."""
+        stale = [k for k, (p, w, seen) in enumerate(zip(self.parameters, self.masters, self._seen)) if w is not None and p._version != seen]
+        if stale and torch.cuda.is_current_stream_capturing():
+            raise P.L.EngineError(f"parameter {stale[0]} was written to since the last update: call renew_masters() before the capture")
+        for k in stale:
+            self.masters[k].copy_(self.parameters[k])
+            self._seen[k] = self.parameters[k]._version
+
+    @torch.no_grad()
     def step(self, grads=None):
         c = self.cfg
         grads = [p.grad for p in self.parameters] if grads is None else list(grads)
-        for p, w, seen in zip(self.parameters, self.masters, self._seen):
-            if w is not None and p._version != seen:
-                w.copy_(p)
+        self.renew_masters()
         self.grad_norm = adamw_step(self.parameters, grads, self.state["first"], self.state["second"], self._count, lr=self.lr, beta_1=c.beta_1, beta_2=c.beta_2,
                                     epsilon=c.epsilon, weight_decay=c.weight_decay, max_norm=c.max_norm, bounds=self.bounds, masters=self.masters)
         self._seen = [p._version for p in self.parameters]

@@ -10,7 +10,7 @@ import torch
 
 from plasticinelab_amd import _lib
 from plasticinelab_amd import policy as P
-from plasticinelab_amd.optimizer import adamw_step
+from plasticinelab_amd.optimizer import AdamW, adamw_step
 from tests import policy_cases as cases
 from tests.util import ROOT
 
@@ -312,3 +312,20 @@ def test_a_step_whose_inputs_lie_in_its_state(interpreter):
         want = P.gated_scan_step(*[t.clone().contiguous() for t in args], other)
         got = P.gated_scan_step(*args, mine)
         assert torch.equal(got, want) and torch.equal(mine, other)
+
+
+def test_a_master_is_not_made_anew_inside_a_capture(interpreter, monkeypatch):
+    p, g = torch.zeros(40, dtype=torch.bfloat16), torch.ones(40, dtype=torch.bfloat16)
+    opt = AdamW([p], lr=1e-3)
+    p.fill_(1.0)
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(_lib.EngineError, match="renew_masters"):
+            opt.step([g])
+        assert float(p[0]) == 1.0 and opt.iter == 0
+    opt.renew_masters()
+    assert float(opt.masters[0][0]) == 1.0
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        opt.step([g])
+    assert opt.iter == 1 and float(opt.masters[0][0]) != float(p[0])

@@ -3,6 +3,7 @@ bounds from a running error analysis (tests/policy_oracle.py), and how they beha
 import pytest
 import torch
 
+from plasticinelab_amd import _lib as L
 from plasticinelab_amd import policy as P
 from plasticinelab_amd.optimizer import AdamW, adamw_step
 from tests import policy_cases as cases
@@ -395,3 +396,29 @@ def test_out_of_memory_is_torchs_own_error():
     x = torch.zeros(1, 1, 1024, dtype=torch.bfloat16, device=DEV).expand(1, 1 << 29, 1024)          # a terabyte of outputs, 2 KB of inputs
     with pytest.raises(torch.OutOfMemoryError):
         P.gated_scan(x, x, x, torch.zeros(1024, device=DEV))
+
+
+def test_adamw_object_captured():
+    """Updates as a graph: a parameter that was set before it has its master renewed outside; one that was not is refused, since every replay would
+    round the master back to the parameter."""
+    torch.manual_seed(5)
+    start, g = torch.randn(3000, device=DEV).bfloat16(), torch.randn(3000, device=DEV).bfloat16()
+    grad = torch.empty_like(g)
+    graphed, eager = (AdamW([torch.zeros(3000, device=DEV, dtype=torch.bfloat16)], lr=1e-4) for _ in range(2))
+    for opt in (graphed, eager):
+        opt.parameters[0].copy_(start)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(L.EngineError, match="renew_masters"):
+            graphed.step([grad])
+        grad.copy_(g)
+    graphed.renew_masters()
+    with torch.cuda.graph(graph):
+        graphed.step([grad])
+    for k in range(5):
+        grad.copy_(g * (k + 1))
+        graph.replay()
+        eager.step([g * (k + 1)])
+        torch.cuda.synchronize()
+        assert torch.equal(graphed.parameters[0], eager.parameters[0]) and torch.equal(graphed.masters[0], eager.masters[0]), k
+    assert not torch.equal(eager.masters[0], eager.parameters[0].float())
