@@ -137,11 +137,15 @@ class AdamW(Optimizer):
     def v_buffer(self):
         return self._values("second")
 
+    def _capturing(self):
+        with torch.cuda.device_of(self._count):              # (the stream asked about is the current one of the parameters' device)
+            return self._count.is_cuda and torch.cuda.is_current_stream_capturing()
+
     @torch.no_grad()
     def renew_masters(self):
         """Make the masters of parameters that were written to since the last update anew (``step`` does it by itself, outside a capture)."""
         stale = [k for k, (p, w, seen) in enumerate(zip(self.parameters, self.masters, self._seen)) if w is not None and p._version != seen]
-        if stale and torch.cuda.is_current_stream_capturing():
+        if stale and self._capturing():
             raise P.L.EngineError(f"parameter {stale[0]} was written to since the last update: call renew_masters() before the capture")
         for k in stale:
             self.masters[k].copy_(self.parameters[k])

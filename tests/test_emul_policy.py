@@ -319,13 +319,13 @@ def test_a_master_is_not_made_anew_inside_a_capture(interpreter, monkeypatch):
     opt = AdamW([p], lr=1e-3)
     p.fill_(1.0)
     with monkeypatch.context() as m:
-        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        m.setattr(AdamW, "_capturing", lambda self: True)
         with pytest.raises(_lib.EngineError, match="renew_masters"):
             opt.step([g])
         assert float(p[0]) == 1.0 and opt.iter == 0
     opt.renew_masters()
     assert float(opt.masters[0][0]) == 1.0
     with monkeypatch.context() as m:
-        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        m.setattr(AdamW, "_capturing", lambda self: True)
         opt.step([g])
     assert opt.iter == 1 and float(opt.masters[0][0]) != float(p[0])
