@@ -50,7 +50,8 @@ def adamw_step(params, grads, first, second, step, *, lr=1e-3, beta_1=0.9, beta_
     a 16-bit parameter is itself updated in float32 and rounded, and loses updates below its last bit.  step: int64 (2,) on the GPU, zeros at the
     start: the updates done, and those begun.  lr and the other numbers are fixed in a captured graph; the count is not.
     No tensor that the update writes may be in the call twice or share memory with another one of it (but for a gradient that is its parameter itself).  A call without any gradient does nothing.
-    A gradient that is not finite makes its element's moments and weight not finite (moments of 8 bits: its 256's; with max_norm: all of them).
+    A gradient that is not finite makes its element's moments and weight not finite (moments of 8 bits: its 256's).  With max_norm a NaN does so to all of
+    them; an infinity makes k zero, so all other elements move as with a gradient of zero.
     """
     bits, first_scales, second_scales = 32, [], []
     if len(first) and isinstance(first[0], (tuple, list)):

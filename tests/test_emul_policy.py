@@ -10,7 +10,7 @@ import torch
 
 from plasticinelab_amd import _lib
 from plasticinelab_amd import policy as P
-from plasticinelab_amd.optimizer import AdamW, adamw_step
+from plasticinelab_amd.optimizer import AdamW, adamw_step, adamw_values
 from tests import policy_cases as cases
 from tests.util import ROOT
 
@@ -329,3 +329,33 @@ def test_a_master_is_not_made_anew_inside_a_capture(interpreter, monkeypatch):
         m.setattr(AdamW, "_capturing", lambda self: True)
         opt.step([g])
     assert opt.iter == 1 and float(opt.masters[0][0]) != float(p[0])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_adamw_gradients_that_are_not_finite(interpreter, bits, value):
+    """What becomes of an element, of its block of 256 and of the rest, with and without clipping."""
+    n = 1000
+    z = lambda dt=torch.float32, size=n: torch.zeros(size, dtype=dt)                                     # noqa: E731
+    g = torch.linspace(-1, 1, n)
+    g[700] = value
+    for max_norm in (0.0, 1.0):
+        results = []
+        for grad in (g, torch.where(torch.isfinite(g), g, torch.zeros(()))):
+            p = torch.ones(n)
+            first, second = ([z()], [z()]) if bits == 32 else ([(z(torch.int8), z(size=4))], [(z(torch.uint8), z(size=4))])
+            norm = adamw_step([p], [grad * 0 if max_norm and grad is not g else grad], first, second, z(torch.int64, 2), max_norm=max_norm)
+            m, v = ((first[0], second[0]) if bits == 32 else adamw_values([first[0], second[0]]))
+            results.append((p, m, v, norm))
+        (p, m, v, norm), (rest_p, rest_m, rest_v, _) = results
+        touched = torch.zeros(n, dtype=torch.bool)
+        touched[700] = True
+        if max_norm and value != value:
+            assert not torch.isfinite(p).any() and not torch.isfinite(m).any() and not torch.isfinite(norm)
+            continue
+        assert not torch.isfinite(p[700])
+        moments = touched if bits == 32 else (torch.arange(n) // 256 == 700 // 256)
+        assert not torch.isfinite(m[moments]).any() and not torch.isfinite(v[moments]).any()
+        assert torch.equal(p[~touched], rest_p[~touched]) and torch.equal(m[~moments], rest_m[~moments]) and torch.equal(v[~moments], rest_v[~moments])
+        if max_norm:
+            assert float(norm) == float("inf")
