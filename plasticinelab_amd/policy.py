@@ -142,6 +142,10 @@ class RecurrentPolicy(torch.nn.Module):
         """The state before the first observation: float32 (depth, batch, width), zeros."""
         return torch.zeros(self.depth, batch, self.width, device=self.decay[0].device)
 
+    def _check_state(self, state):
+        if len(state) != self.depth:
+            _refuse(f"state has to be of {self.depth} blocks, got {len(state)}")
+
     def _run(self, obs, memory):
         """obs (..., obs_dim) -> actions; ``memory(k, x, r, i)`` is block k's recurrence."""
         dtype = self.embed.weight.dtype
@@ -158,6 +162,8 @@ class RecurrentPolicy(torch.nn.Module):
         episode begins."""
         if obs.dim() != 3:
             _refuse(f"obs has to be (batch, steps, obs_dim), got {tuple(obs.shape)}")
+        if state is not None:
+            self._check_state(state)
         states = []
 
         def memory(k, x, r, i):
@@ -180,4 +186,5 @@ class RecurrentPolicy(torch.nn.Module):
         """``step`` without gradients: -> actions; ``state`` moves on in place."""
         if obs.dim() != 2:
             _refuse(f"obs has to be (batch, obs_dim), got {tuple(obs.shape)}")
+        self._check_state(state)
         return self._run(obs, lambda k, x, r, i: gated_scan_step(x, r, i, self.decay[k], state[k], c=self.c))

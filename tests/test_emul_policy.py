@@ -359,3 +359,17 @@ def test_adamw_gradients_that_are_not_finite(interpreter, bits, value):
         assert torch.equal(p[~touched], rest_p[~touched]) and torch.equal(m[~moments], rest_m[~moments]) and torch.equal(v[~moments], rest_v[~moments])
         if max_norm:
             assert float(norm) == float("inf")
+
+
+def test_a_state_of_another_policy_is_refused(interpreter):
+    """Before anything moves: too few blocks ended in an IndexError with the first ones moved on, too many went unnoticed."""
+    policy, obs = P.RecurrentPolicy(5, 2, width=8, depth=2, device="cpu"), torch.randn(3, 5)
+    for blocks in (1, 3):
+        state = torch.zeros(blocks, 3, 8)
+        for call in (lambda: policy.act(obs, state), lambda: policy.step(obs, state), lambda: policy(obs[:, None], state)):
+            with pytest.raises(ValueError, match="of 2 blocks"):
+                call()
+        assert float(state.abs().sum()) == 0
+    state = policy.initial_state(3)
+    action, after = policy.step(obs, state)
+    assert torch.allclose(policy.act(obs, state), action.detach()) and torch.allclose(state, after)
