@@ -17,6 +17,8 @@ A policy on the CPU runs in float64.  A policy on a GPU keeps its own type and p
 """
 from __future__ import annotations
 
+import inspect
+
 import numpy as np
 import torch
 
@@ -184,19 +186,50 @@ class SolverNN:
             env.step(a)
         return np.stack(seen)
 
+    def _whole_sequences(self, obs, reset):
+        """The policy's actions over sequences (B, H, obs.dim).  A policy with a memory whose ``forward`` takes ``reset`` gets them at once and answers
+        (actions, state); any other one goes through ``initial_state`` and ``step``, row by row where there are resets (which part of a state is a
+        row's is the policy's business).  A policy without a memory has nothing to reset."""
+        if not hasattr(self.policy, "initial_state"):
+            return self.policy(obs)
+        if "reset" in inspect.signature(self.policy.forward).parameters:
+            out = self.policy(obs, reset=reset)
+            if not isinstance(out, (tuple, list)) or len(out) != 2:
+                raise ValueError(f"a policy whose forward takes reset has to answer (actions, state), got {type(out).__name__}")
+            return out[0]
+
+        def walk(rows, begins):
+            state, answers = self.policy.initial_state(rows.shape[0]), []
+            for t in range(rows.shape[1]):
+                if begins[t]:
+                    state = self.policy.initial_state(rows.shape[0])
+                answer, state = self.policy.step(rows[:, t], state)
+                answers.append(answer)
+            return torch.stack(answers, 1)
+
+        if reset is None:
+            return walk(obs, [False] * obs.shape[1])
+        return torch.cat([walk(row[None], begins) for row, begins in zip(obs, reset.tolist())])
+
     def imitate(self, observations, actions, n_iters=100, reset=None):
         """Fit the policy to recorded sequences by least squares: observations (B, H, obs.dim), actions (B, H, action_dim); ``reset`` (B, H) marks steps
-        that begin an episode (sequences of several).  Whole sequences go through the policy at once; AdamW with this solver's optimiser settings
-        updates it.  -> the mean squared errors, one an iteration."""
+        that begin an episode (sequences of several).  Whole sequences go through the policy at once (one with a memory whose ``forward`` takes no
+        ``reset`` goes through its ``step``); AdamW with this solver's optimiser settings updates it.  -> the mean squared errors, one an iteration."""
         obs, target = (torch.as_tensor(np.asarray(a)).to(**self.place) for a in (observations, actions))
+        if hasattr(self.policy, "initial_state") and obs.dim() != 3:
+            raise ValueError(f"observations of a policy with a memory have to be (B, H, obs.dim), got {tuple(obs.shape)}")
         if reset is not None:
             reset = torch.as_tensor(np.asarray(reset, bool)).to(self.place["device"])
+            if reset.shape != obs.shape[:-1]:
+                raise ValueError(f"reset has to be {tuple(obs.shape[:-1])}, got {tuple(reset.shape)}")
         optim = AdamW(list(self.policy.parameters()), self.cfg.optim)
         losses = []
         for _ in range(int(n_iters)):
             for p in self.policy.parameters():
                 p.grad = None
-            out = self.policy(obs, reset=reset)[0] if hasattr(self.policy, "initial_state") else self.policy(obs)
+            out = self._whole_sequences(obs, reset)
+            if out.shape != target.shape:
+                raise ValueError(f"the policy answers {tuple(out.shape)} to these observations, actions are {tuple(target.shape)}")
             loss = torch.nn.functional.mse_loss(out.float(), target.float())
             loss.backward()
             optim.step()

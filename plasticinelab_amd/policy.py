@@ -159,7 +159,7 @@ class RecurrentPolicy(torch.nn.Module):
 
     def forward(self, obs, state=None, reset=None):
         """obs (batch, steps, obs_dim) -> (actions (batch, steps, action_dim), state behind the last step).  ``reset``: (batch, steps) bool, where a new
-        episode begins."""
+        episode begins (its first input then enters with a gain of 1, as ``gated_scan``'s reset has it; behind a state of zeros it is sqrt(1 - a^2))."""
         if obs.dim() != 3:
             _refuse(f"obs has to be (batch, steps, obs_dim), got {tuple(obs.shape)}")
         if state is not None:

@@ -373,3 +373,85 @@ def test_a_state_of_another_policy_is_refused(interpreter):
     state = policy.initial_state(3)
     action, after = policy.step(obs, state)
     assert torch.allclose(policy.act(obs, state), action.detach()) and torch.allclose(state, after)
+
+
+class Sums(torch.nn.Module):
+    """A policy with a memory of the documented kind: ``initial_state`` and ``step``, its ``forward`` for one observation."""
+
+    def __init__(self):
+        super().__init__()
+        self.lin = torch.nn.Linear(4, 2)
+
+    def initial_state(self, batch):
+        return [torch.zeros(batch, 4)]
+
+    def step(self, obs, state):
+        state = [0.5 * state[0] + obs]
+        return self.lin(state[0]), state
+
+    def forward(self, obs):
+        return self.lin(obs)
+
+
+def imitation(policy):
+    from plasticinelab_amd.config import CfgNode
+    from plasticinelab_amd.optimizer.solver_nn import SolverNN
+    solver = SolverNN.__new__(SolverNN)                      # (a simulator needs a GPU; imitation does without one)
+    solver.policy, solver.place = policy, {"dtype": torch.float32, "device": "cpu"}
+    solver.cfg = CfgNode({"optim": {"lr": 1e-3, "bounds": (-float("inf"), float("inf")), "type": "Adam"}})
+    return solver
+
+
+def test_imitation_by_policies_of_every_kind(interpreter):
+    B, H = 3, 6
+    gen = torch.Generator().manual_seed(8)
+    obs, target = torch.randn(B, H, 4, generator=gen), torch.randn(B, H, 2, generator=gen)
+    reset = torch.rand(B, H, generator=gen) < 0.3
+    assert reset.any()
+
+    def expected(policy, reset):
+        if reset is not None and isinstance(policy, P.RecurrentPolicy):          # (there a reset is a = 0 with a gain of 1, not a state of zeros)
+            return float(((policy(obs, reset=reset)[0] - target).detach() ** 2).mean())
+        out = []
+        for b in range(B):
+            state = policy.initial_state(1)
+            for t in range(H):
+                if reset is not None and reset[b, t]:
+                    state = policy.initial_state(1)
+                a, state = policy.step(obs[b:b + 1, t], state)
+                out.append(a)
+        return float(((torch.cat(out).view(B, H, 2) - target).detach() ** 2).mean())
+
+    for make in (Sums, lambda: P.RecurrentPolicy(4, 2, width=8, depth=2, device="cpu")):
+        for cuts in (None, reset):
+            torch.manual_seed(9)
+            policy = make()
+            want = expected(policy, cuts)
+            before = [p.detach().clone() for p in policy.parameters()]
+            losses = imitation(policy).imitate(obs, target, n_iters=3, reset=cuts)
+            assert len(losses) == 3 and abs(losses[0] - want) <= 1e-5 * want
+            assert not any(torch.equal(a, b) for a, b in zip(policy.parameters(), before))
+            want = expected(policy, cuts)                    # (of the policy as the updates left it)
+            assert abs(imitation(policy).imitate(obs, target, n_iters=1, reset=cuts)[0] - want) <= 1e-5 * want
+
+    linear = torch.nn.Linear(4, 2)                           # without a memory: nothing to reset
+    want = float(((linear(obs) - target).detach() ** 2).mean())
+    for cuts in (None, reset):
+        fresh = torch.nn.Linear(4, 2)
+        fresh.load_state_dict(linear.state_dict())
+        assert abs(imitation(fresh).imitate(obs, target, n_iters=1, reset=cuts)[0] - want) <= 1e-5 * want
+
+
+def test_imitation_refuses_what_does_not_fit(interpreter):
+    class Odd(Sums):
+        def forward(self, obs, reset=None):
+            return self.lin(obs)
+
+    obs, target = torch.zeros(3, 6, 4), torch.zeros(3, 6, 2)
+    for policy, args, kw, text in ((Odd(), (obs, target), {}, "answer \\(actions, state\\)"), (Sums(), (obs, target[:, :, :1]), {}, "actions are"), (Sums(), (obs, target[0]), {}, "actions are"),
+                                   (torch.nn.Linear(4, 2), (obs, target[0]), {}, "actions are"), (Sums(), (obs[0], target[0]), {}, "B, H, obs.dim"),
+                                   (Sums(), (obs, target), {"reset": torch.zeros(3, 5)}, "reset has to be"), (P.RecurrentPolicy(4, 2, width=8, device="cpu"), (obs, target[0]), {}, "actions are")):
+        before = [p.detach().clone() for p in policy.parameters()]
+        with pytest.raises(ValueError, match=text):
+            imitation(policy).imitate(*args, n_iters=1, **kw)
+        assert all(torch.equal(a, b) for a, b in zip(policy.parameters(), before))
