@@ -28,7 +28,7 @@ enum plmpm_nn_dtype { PLMPM_NN_F32 = 0, PLMPM_NN_BF16 = 1, PLMPM_NN_F16 = 2 };
  * x, r, i: [batch][steps][width], unit stride over the width, element strides over batch and steps as given (slices of one
  * projection are read in place).  h and every gradient: contiguous.  decay, h0, h_last, dh0, dlast, ddecay: float.
  * checkpoint: float [ceil(steps / 64)][batch][width], the state each run of 64 steps starts from: written by the forward call
- * if not null, read by the backward call.  h0, reset, h_last, dh, dlast, dh0 may be null. */
+ * if not null, read by the backward call (and a forward call that is given it is refused where that would be).  h0, reset, h_last, dh, dlast, dh0 may be null. */
 typedef struct plmpm_scan {
     int32_t dtype, reserved;
     int64_t batch, steps, width;

@@ -621,6 +621,12 @@ bool loose(const plmpm_scan* s, bool backward) {
     return bytes < 4;
 }
 
+// a launch takes less than 2^32 threads
+int blocks_across(const plmpm_scan* s) { return (int)((s->width + 64 * vector_of(s) - 1) / (64 * vector_of(s))); }
+bool fits_a_launch(const plmpm_scan* s, bool backward) {
+    return (uint64_t)s->batch * blocks_across(s) * tiles_of(s, backward) * threads_of(s->steps, backward) < ((uint64_t)1 << 32);
+}
+
 int check(const plmpm_scan* s, bool backward, bool pointers) {
     NN_REQUIRE(s, "scan: null argument");
     NN_REQUIRE(s->dtype >= PLMPM_NN_F32 && s->dtype <= PLMPM_NN_F16, "scan: unknown dtype %d", s->dtype);
@@ -657,6 +663,8 @@ int run(const plmpm_scan* s, bool backward, hipStream_t st) {
     A.dh = s->dh; A.dlast = s->dlast; A.out[0] = s->dx; A.out[1] = s->dr; A.out[2] = s->di;
     A.dh0 = s->dh0;
     A.B = s->batch; A.T = s->steps; A.D = (int)s->width; A.c = (float)s->c;
+    // (a forward call that keeps checkpoints is refused where its backward call would be)
+    NN_REQUIRE(((!backward && s->steps == 1) || fits_a_launch(s, backward)) && (backward || !s->checkpoint || fits_a_launch(s, true)), "scan: batch x width x steps is too large for one launch");
     if (!backward && s->steps == 1) {
         if (s->dtype == PLMPM_NN_F32) launch_step<float>(A, st);
         else if (s->dtype == PLMPM_NN_BF16) launch_step<bf16>(A, st);
@@ -666,10 +674,9 @@ int run(const plmpm_scan* s, bool backward, hipStream_t st) {
     }
     const int vec = vector_of(s);
     const bool between = vec == 2 && loose(s, backward);
-    A.cblks = (A.D + 64 * vec - 1) / (64 * vec);
+    A.cblks = blocks_across(s);
     A.tiles = (int)tiles_of(s, backward);
     A.past = 3.0 * dtype_size(s->dtype) * s->batch * s->steps * s->width > kPastCaches;
-    NN_REQUIRE((uint64_t)A.B * A.cblks * A.tiles * threads_of(A.T, backward) < ((uint64_t)1 << 32), "scan: batch x width x steps is too large for one launch");
     const size_t words = word_bytes(s, backward);
     A.part = (float*)((char*)s->workspace + words + k2_bytes(s, backward));
     if (words) {

@@ -161,3 +161,12 @@ def test_adamw_refuses_tensors_that_share_memory():
     one = codes()
     with pytest.raises(_lib.EngineError, match="no CPU path"):
         adamw_values([one, one], out=halves)
+
+
+def test_a_forward_call_is_refused_where_its_backward_call_would_be():
+    """10^7 rows of 50 steps of one channel: the forward launch takes them, the backward one, whose waves hold half the steps, does not."""
+    lib = _lib.load_policy()
+    some = 1 << 20
+    for steps, batch in ((50, 10 ** 7), (1, 1 << 27)):
+        s = _lib.Scan(dtype=0, batch=batch, steps=steps, width=1, c=8.0, x=some, r=some, i=some, decay=some, h=some, checkpoint=some, workspace=some, workspace_bytes=1 << 60)
+        assert lib.plmpm_scan_forward(s, None) != 0 and "one launch" in lib.plmpm_last_error().decode()
