@@ -50,6 +50,7 @@ inline void from_f(float f, f16& o) {
     o.v = (uint16_t)(s | ((r - (112u << 23)) >> 13));
 }
 inline float exp2_fast(float x) { return exp2f(x); }
+inline float fract_below_one(float x) { const float f = x - std::floor(x); return f > 0.999999940395355224609375f ? 0.999999940395355224609375f : f; }
 inline void sleep_a_little() { __builtin_amdgcn_s_sleep(1); }
 inline void wait_for_memory() {}
 #else
@@ -58,6 +59,7 @@ __device__ __forceinline__ float to_f(f16 x) { _Float16 h; memcpy(&h, &x, 2); re
 __device__ __forceinline__ void from_f(float f, bf16& o) { const __bf16 h = (__bf16)f; memcpy(&o, &h, 2); }
 __device__ __forceinline__ void from_f(float f, f16& o) { const _Float16 h = (_Float16)f; memcpy(&o, &h, 2); }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }       // v_exp_f32: within 1 ulp; exponents below -126 give 0
+__device__ __forceinline__ float fract_below_one(float x) { return __builtin_amdgcn_fractf(x); }        // v_fract_f32: at most the last float below 1
 __device__ __forceinline__ void sleep_a_little() { __builtin_amdgcn_s_sleep(8); }        // 8 x 64 cycles
 __device__ __forceinline__ void wait_for_memory() { __builtin_amdgcn_s_waitcnt(0x0f70); }       // vmcnt(0)
 #endif
@@ -73,6 +75,15 @@ __device__ __forceinline__ void anew(float& f) {
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 // 1 / (1 + e^-x): both ends come out right by themselves (e^-x = inf -> 0, 0 -> 1)
 __device__ __forceinline__ float sigmoid_fast(float x) { return __builtin_amdgcn_rcpf(1.0f + exp2_fast(-kLog2e * x)); }
+// A sigmoid s and 1 - s in one number, each to its own last bits: the smaller of the two, q e with e = e^-|x| and q = 1 / (1 + e), with the sign of x.  (From a
+// rounded s near 1 the difference cancels: 23 % off at x = 15.7, nothing left above 17.)  s is then what is left of its negative above a whole number,
+// one instruction, and s (1 - s) one more.  The smaller side is never 0, whose negative has nothing left: 2^-126 is added where it is multiplied.
+__device__ __forceinline__ float both_sides(float x) {
+    const float e = exp2_fast(-kLog2e * fabsf(x)), q = __builtin_amdgcn_rcpf(1.0f + e);
+    return copysignf(fmaf(e, q, 1.1754943508222875e-38f), x);
+}
+__device__ __forceinline__ float side_of(float both) { return fract_below_one(-both); }
+__device__ __forceinline__ float product_of(float both) { const float t = fabsf(both); return fmaf(-t, t, t); }
 
 // N neighbouring elements as one access of the widest type their bytes allow (up to 16; more: several).  LOOSE: at any element's address -- global
 // memory takes accesses of 16 bytes at every alignment, and the compiler makes one of a packed type

@@ -69,11 +69,19 @@ __device__ __forceinline__ float softplus(float x) {
 // sigmoid(r), sigmoid(i), log2 a, a and 1 - a^2.  1 - a^2 = -expm1(2 ln2 l2) cancels for a near 1: above l2 = -0.18 (a^2 > 0.78) it
 // comes from a cubic for -expm1(2 ln2 l) / l, the polynomial through its values at the Chebyshev points (relative error 2.7e-7, half
 // of that in the root); below, 1 - a a is off by at most 2^-24 / 0.22.
-struct Gates { float sr, si, l2, a, m2; };
-__device__ __forceinline__ Gates gates(float r, float i, float k2) {
+// BOTH (backward): the sigmoids also as both_sides has them, and taken from there, so that the walks that come back to them see the same numbers.
+struct Gates { float sr, si, l2, a, m2, both_r, both_i; };
+template <bool BOTH = false> __device__ __forceinline__ Gates gates(float r, float i, float k2) {
     Gates g;
-    g.sr = sigmoid_fast(r);
-    g.si = sigmoid_fast(i);
+    if (BOTH) {
+        g.both_r = both_sides(r);
+        g.both_i = both_sides(i);
+        g.sr = side_of(g.both_r);
+        g.si = side_of(g.both_i);
+    } else {
+        g.sr = sigmoid_fast(r);
+        g.si = sigmoid_fast(i);
+    }
     g.l2 = k2 * g.sr;
     g.a = exp2_fast(g.l2);
     const float q = fmaf(fmaf(fmaf(-0.13934674859046936f, g.l2, -0.4424225986003876f), g.l2, -0.960848331451416f), g.l2, -1.3862940073013306f);
@@ -345,6 +353,7 @@ __global__ __launch_bounds__(256) void k_scan_step(ScanArgs A) {
 // h_{t-1} in 32 bits, and backward) go through one exchange; tiles are handed out from the last to the first.
 //   dx = g m s_i   di = g m x s_i (1 - s_i)   dla = g (a h_{t-1} - s_i x a^2 / m)   dr = dla la (1 - s_r)
 // For la -> 0 the product la a^2 / m goes to 0 (m ~ sqrt(-2 la)): where m is 0 that term is left out.
+// s (1 - s) comes from the smaller side (both_sides): 3 % more time at 8 x 2047 x 2048 than with 1 - s from s, whose gradients are wrong far out.
 template <class T, int VEC, int S, int W, bool LOOSE>
 __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
     static_assert(S * W % kCheckpoint == 0, "a tile starts at a checkpoint");
@@ -362,8 +371,8 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
     const int left = __builtin_amdgcn_readfirstlane(steps_left(A.T, t0, S));
     const int64_t from = left ? t0 : A.T - 1;
     const unsigned cut = reset_bits<S>(A, b, t0, left);
-    // Kept for the second walk: x and dh as they came, a, m and the gates.  What can be had from those in a few operations is not: a register more
-    // here is one spilled to memory.  (8 x 2047 x 2048: with m s_i and s_i x a^2 / m held in m's place, 29 of them, 154 us instead of 131.  The
+    // Kept for the second walk: x and dh as they came, a, m and both sides of the gates (sr, si).  What can be had from those in a few operations is
+    // not: a register more here is one spilled to memory.  (8 x 2047 x 2048: with m s_i and s_i x a^2 / m held in m's place, 29 of them, 154 us instead of 131.  The
     // compiler would do the same by itself, hence forget and anew: calls in bf16 and fp16 without resets 165 and 171 us, with the 16 and 32
     // registers that it keeps otherwise 185 and 196.  A kernel without the resets' selects kept more of them and was the slower one.)
     Vec<T, VEC, LOOSE> rawx[S], rawg[S];
@@ -398,9 +407,9 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
             const bool there = WHOLE || s < left;
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                const Gates g = gates(r[v], i[v], k2[v]);
-                sr[s][v] = there ? g.sr : 0.0f;
-                si[s][v] = g.si;
+                const Gates g = gates<true>(r[v], i[v], k2[v]);
+                sr[s][v] = there ? g.both_r : 0.0f;
+                si[s][v] = g.both_i;
                 if ((cut >> s & 1)) {
                     a[s][v] = 0.0f;
                     m[s][v] = 1.0f;
@@ -489,7 +498,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             const bool reset = (cut >> s & 1);
-            const float sx = si[s][v] * x[v], u = m[s][v] * sx, inv = m[s][v] == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(m[s][v]);
+            const float sx = side_of(si[s][v]) * x[v], u = m[s][v] * sx, inv = m[s][v] == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(m[s][v]);
             pull[s][v] = reset ? 0.0f : a[s][v] * fmaf(-sx * inv, a[s][v], now[v]);        // dla / g
             now[v] = reset ? u : fmaf(a[s][v], now[v], u);
         }
@@ -502,14 +511,14 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             const bool reset = (cut >> s & 1);
+            anew(si[s][v]);
             g[v] += e[v];
             e[v] = reset ? 0.0f : a[s][v] * g[v];
-            dx[v] = g[v] * m[s][v] * si[s][v];
-            const float gu = dx[v] * x[v];
-            di[v] = fmaf(-gu, si[s][v], gu);
-            const float q = reset || s >= left ? 0.0f : g[v] * pull[s][v] * sr[s][v];        // (behind the end: 0 times a state that may be infinite)
-            dr[v] = q * (k2[v] * kLn2) * (1.0f - sr[s][v]);
-            sum[v] += q;
+            dx[v] = g[v] * m[s][v] * side_of(si[s][v]);
+            di[v] = g[v] * m[s][v] * x[v] * product_of(si[s][v]);
+            const float q = reset || s >= left ? 0.0f : g[v] * pull[s][v];         // (behind the end: 0 times a state that may be infinite)
+            dr[v] = q * (k2[v] * kLn2) * product_of(sr[s][v]);
+            sum[v] = fmaf(q, reset ? 0.0f : side_of(sr[s][v]), sum[v]);            // (a gate that is no number counts for nothing where its step begins anew)
         }
         if (mine.live && s < left) {
             const int64_t to = (b * A.T + t0 + s) * A.D;

@@ -225,3 +225,31 @@ def run_norm_of_rows_far_apart(dev):
     pre = torch.ones(8, dtype=torch.float16, device=dev)
     for a, b in zip(P.block_norm(x, u, pre=pre), P.block_norm(x.contiguous(), u.contiguous(), pre=pre)):
         assert torch.equal(a, b)
+
+
+def run_gates_far_out(dev, dtype):
+    """Gradients of gates up to +-30, each within its own last bits: 1 - sigmoid must not come from a rounded sigmoid.  u = 2^-24.  e^-x of a rounded product and
+    constant: (1.3 |x| + 2) u; the sum 1, rcp 2, e^-x sigmoid 1 and the other side's sum 1 more: S(x) = (1.3 |x| + 8) u for each side.  One step from zero:
+    di = dh m x s(i) (1 - s(i)) with m = sqrt(1 - a^2), whose la is off by S(r) + 8 u, half of it through the root, the cubic or 1 - a a and the root 16 u more
+    (as tests/policy_oracle.py has it): S(r) + 24 u, and five products; dr = -dh s(i) x a^2 / m la (1 - s(r)), a^2 off by 2 |la| (S(r) + 8 u) + 6 u.  Where every
+    step begins anew, a = 0, m = 1 and nothing is handed on: di = dh x s(i) (1 - s(i))."""
+    U, dt, D = R.U, DTYPES[dtype], 257
+    S = lambda t: (1.3 * t.abs() + 8) * U                                                                # noqa: E731
+    for T, cut in ((1, False), (70, True)):
+        i = torch.linspace(-30, 30, D).expand(1, T, D).to(dt)
+        r = torch.linspace(-30, 30, D)[torch.randperm(D, generator=torch.Generator().manual_seed(1))].expand(1, T, D).to(dt)
+        x, dh = (normal(k, 1, T, D, dtype=dt).abs() + 0.1 for k in (2, 3))
+        x, dh = x.to(dt), dh.to(dt)
+        decay = torch.full((D,), -4.0)
+        reset = torch.ones(1, T, dtype=torch.bool) if cut else None
+        leaves = [t.contiguous().to(dev).requires_grad_() for t in (x, r, i)]
+        h, _ = P.gated_scan(*leaves, decay.to(dev), None, None if reset is None else reset.to(dev))
+        got = torch.autograd.grad(h, leaves, dh.to(dev))
+        X, Rr, I, G = (t.double() for t in (x, r, i, dh))
+        si, oi, sr, orr = torch.sigmoid(I), torch.sigmoid(-I), torch.sigmoid(Rr), torch.sigmoid(-Rr)
+        la = -8.0 * torch.nn.functional.softplus(decay.double()) * sr
+        m = torch.ones_like(la) if cut else torch.sqrt(-torch.expm1(2 * la))
+        em = torch.zeros_like(la) if cut else S(Rr) + 24 * U
+        ref = {"dx": G * m * si, "di": G * m * X * si * oi, "dr": torch.zeros_like(la) if cut else -G * si * X * torch.exp(2 * la) / m * la * orr}
+        tol = {"dx": em + S(I) + 3 * U, "di": em + 2 * S(I) + 5 * U, "dr": S(I) + 2 * la.abs() * (S(Rr) + 8 * U) + 6 * U + em + 2 * S(Rr) + 8 * U + 10 * U}
+        check(dict(zip(("dx", "dr", "di"), got)), ref, {k: tol[k] * ref[k].abs() + R.rounding(ref[k], dt) for k in ref})

@@ -455,3 +455,8 @@ def test_imitation_refuses_what_does_not_fit(interpreter):
         with pytest.raises(ValueError, match=text):
             imitation(policy).imitate(*args, n_iters=1, **kw)
         assert all(torch.equal(a, b) for a, b in zip(policy.parameters(), before))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_scan_gradients_of_gates_far_out(interpreter, dtype):
+    cases.run_gates_far_out(interpreter, dtype)

@@ -422,3 +422,8 @@ def test_adamw_object_captured():
         torch.cuda.synchronize()
         assert torch.equal(graphed.parameters[0], eager.parameters[0]) and torch.equal(graphed.masters[0], eager.masters[0]), k
     assert not torch.equal(eager.masters[0], eager.parameters[0].float())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_scan_gradients_of_gates_far_out(dtype):
+    cases.run_gates_far_out(DEV, dtype)
