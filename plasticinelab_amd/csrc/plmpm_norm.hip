@@ -55,7 +55,7 @@ template <int VW> __device__ __forceinline__ void gates_of(int fn, float (&g)[VW
         for (int k = 0; k < VW; ++k) df[k] = 1.0f;
     } else if (fn == PLMPM_GATE_SIGMOID) {
 #pragma unroll
-        for (int k = 0; k < VW; ++k) { g[k] = sigmoid_fast(g[k]); df[k] = g[k] * (1.0f - g[k]); }
+        for (int k = 0; k < VW; ++k) { const float both = both_sides(g[k]); g[k] = side_of(both); df[k] = product_of(both); }
     } else {
 #pragma unroll
         for (int k = 0; k < VW; ++k) { const float s = sigmoid_fast(g[k]); df[k] = s * fmaf(g[k], 1.0f - s, 1.0f); g[k] *= s; }

@@ -253,3 +253,20 @@ def run_gates_far_out(dev, dtype):
         ref = {"dx": G * m * si, "di": G * m * X * si * oi, "dr": torch.zeros_like(la) if cut else -G * si * X * torch.exp(2 * la) / m * la * orr}
         tol = {"dx": em + S(I) + 3 * U, "di": em + 2 * S(I) + 5 * U, "dr": S(I) + 2 * la.abs() * (S(Rr) + 8 * U) + 6 * U + em + 2 * S(Rr) + 8 * U + 10 * U}
         check(dict(zip(("dx", "dr", "di"), got)), ref, {k: tol[k] * ref[k].abs() + R.rounding(ref[k], dt) for k in ref})
+
+
+def run_norm_gates_far_out(dev, tx, tu):
+    """The gradient of a sigmoid gate up to +-30, each element within its own last bits: dy scale post uh s (1 - s), the sides as in run_gates_far_out, uh 15 u
+    (tests/policy_oracle.py), five products."""
+    U, D = R.U, 520
+    x, u, _, scale, post, _ = norm_inputs(31, (9, D), tx, tu)
+    gate = torch.linspace(-30, 30, D).expand(9, D).to(DTYPES[tu])
+    dy = (normal(32, 9, D).abs() + 0.1).to(x.dtype)
+    leaf = gate.contiguous().to(dev).requires_grad_()
+    y, _ = P.block_norm(x.to(dev), u.to(dev), leaf, scale.to(dev), post.to(dev))
+    got, = torch.autograd.grad(y, leaf, dy.to(dev))
+    X, G, (scale, post, DY) = u.double(), gate.double(), (t.double() for t in (scale, post, dy))
+    uh = X / torch.sqrt((X * X).mean(1, keepdim=True) + 1e-6)
+    ref = DY * scale * post * uh * torch.sigmoid(G) * torch.sigmoid(-G)
+    tol = (2 * (1.3 * G.abs() + 8) + 15 + 6) * U
+    check({"dgate": got}, {"dgate": ref}, {"dgate": tol * ref.abs() + R.rounding(ref, DTYPES[tu])})

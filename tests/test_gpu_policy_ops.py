@@ -407,12 +407,12 @@ def test_adamw_object_captured():
     graphed, eager = (AdamW([torch.zeros(3000, device=DEV, dtype=torch.bfloat16)], lr=1e-4) for _ in range(2))
     for opt in (graphed, eager):
         opt.parameters[0].copy_(start)
-    graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
         with pytest.raises(L.EngineError, match="renew_masters"):
             graphed.step([grad])
         grad.copy_(g)
     graphed.renew_masters()
+    graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         graphed.step([grad])
     for k in range(5):
@@ -427,3 +427,8 @@ def test_adamw_object_captured():
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 def test_scan_gradients_of_gates_far_out(dtype):
     cases.run_gates_far_out(DEV, dtype)
+
+
+@pytest.mark.parametrize("tx,tu", [("f32", "f32"), ("f32", "bf16"), ("f16", "f16")])
+def test_norm_gradients_of_gates_far_out(tx, tu):
+    cases.run_norm_gates_far_out(DEV, tx, tu)
