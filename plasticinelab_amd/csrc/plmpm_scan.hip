@@ -552,11 +552,11 @@ __global__ __launch_bounds__(256) void k_prepare(Word* p, int64_t n, float* k2, 
 }
 
 // d decay[d] = -c sigmoid(decay[d]) * (sum of column d of part[rows][D]): 64 columns and 16 strips of rows a workgroup, strips joined in a
-// fixed order
+// fixed order, all in 64 bits: a row is a tile of one sequence, and there can be hundreds of thousands of them
 __global__ __launch_bounds__(1024) void k_decay_grad(const float* part, const float* decay, float* out, int64_t rows, int D, float c) {
-    __shared__ float strip[16][64];
+    __shared__ double strip[16][64];
     const int col = threadIdx.x & 63, s = threadIdx.x >> 6, d = blockIdx.x * 64 + col;
-    float sum = 0.0f;
+    double sum = 0.0;
     if (d < D)
 #pragma unroll 8
         for (int64_t r = s; r < rows; r += 16) sum += part[r * D + d];
@@ -564,7 +564,7 @@ __global__ __launch_bounds__(1024) void k_decay_grad(const float* part, const fl
     __syncthreads();
     if (s == 0 && d < D) {
         for (int k = 1; k < 16; ++k) sum += strip[k][col];
-        out[d] = -c * sigmoid_fast(decay[d]) * sum;
+        out[d] = (float)(-c * sigmoid_fast(decay[d]) * sum);
     }
 }
 

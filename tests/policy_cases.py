@@ -270,3 +270,17 @@ def run_norm_gates_far_out(dev, tx, tu):
     ref = DY * scale * post * uh * torch.sigmoid(G) * torch.sigmoid(-G)
     tol = (2 * (1.3 * G.abs() + 8) + 15 + 6) * U
     check({"dgate": got}, {"dgate": ref}, {"dgate": tol * ref.abs() + R.rounding(ref, DTYPES[tu])})
+
+
+def run_decay_gradient_of_many_rows(dev, B):
+    """Rows that are all alike: the decays' gradient is that of one row, times their number.  A row's part is the same number in both; its sum over the rows is made
+    in 64 bits (2^-53 an addition), and both results are rounded once: 2 x 2^-24, and 2^-24 for the quotient."""
+    x, r, i, decay, _, _ = scan_inputs(41, 1, 3, 5, "f32", with_h0=False)
+
+    def gradient(rows):
+        ins = [t.expand(rows, 3, 5).to(dev) for t in (x, r, i)]
+        leaf = decay.to(dev).requires_grad_()
+        return torch.autograd.grad(P.gated_scan(*ins, leaf)[1].sum(), leaf)[0].cpu()
+
+    one, many = gradient(1), gradient(B) / B
+    assert float(((many - one).abs() / one.abs()).max()) <= 3.01 * R.U

@@ -470,3 +470,7 @@ def test_scan_gradients_of_gates_far_out(interpreter, dtype):
 @pytest.mark.parametrize("tx,tu", [("f32", "f32"), ("f32", "bf16"), ("f16", "f16")])
 def test_norm_gradients_of_gates_far_out(interpreter, tx, tu):
     cases.run_norm_gates_far_out(interpreter, tx, tu)
+
+
+def test_decay_gradient_of_many_rows(interpreter):
+    cases.run_decay_gradient_of_many_rows(interpreter, 4099)

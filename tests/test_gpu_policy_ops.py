@@ -432,3 +432,7 @@ def test_scan_gradients_of_gates_far_out(dtype):
 @pytest.mark.parametrize("tx,tu", [("f32", "f32"), ("f32", "bf16"), ("f16", "f16")])
 def test_norm_gradients_of_gates_far_out(tx, tu):
     cases.run_norm_gates_far_out(DEV, tx, tu)
+
+
+def test_decay_gradient_of_many_rows():
+    cases.run_decay_gradient_of_many_rows(DEV, 300007)
