@@ -5,7 +5,7 @@ import torch
 
 from plasticinelab_amd import _lib as L
 from plasticinelab_amd import policy as P
-from plasticinelab_amd.optimizer import AdamW, adamw_step
+from plasticinelab_amd.optimizer import AdamW, adamw_step, adamw_values
 from tests import policy_cases as cases
 from tests import policy_oracle as R
 
@@ -436,3 +436,88 @@ def test_norm_gradients_of_gates_far_out(tx, tu):
 
 def test_decay_gradient_of_many_rows():
     cases.run_decay_gradient_of_many_rows(DEV, 300007)
+
+
+@pytest.mark.parametrize("use,grads", [(("pre",), ("dz",)), (("u",), ("dy",)), (("u", "pre"), ("dz",)), (("u", "gate", "post"), ("dy",)), (("u", "gate", "pre"), ("dy",)), (("u", "pre"), ("dy", "dz"))])
+@pytest.mark.parametrize("tx,tu", [("f32", "f32"), ("f32", "bf16"), ("f32", "f16"), ("bf16", "bf16"), ("f16", "f16")])
+def test_norm_parts_of_wide_rows(use, grads, tx, tu):
+    """A workgroup of 1024 threads a row, with something left out: whole rows of 8192, and rows that threads do not divide."""
+    cases.run_norm(DEV, 25, (300, 8192), tx, tu, use=use, grads=grads)
+    cases.run_norm(DEV, 26, (7, 5003), tx, tu, "silu", use=use, grads=grads)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [2048, 2047])
+def test_scan_gradients_past_the_caches(D, dtype):
+    """More than 128 MB of gradients go past the caches, in 4 bytes a lane, between words too, and in 2 at the end of an odd row: the bits of the same sequences alone."""
+    torch.manual_seed(6)
+    B, T = 8, 1500
+    assert 3 * 2 * B * T * D > 128 << 20 > 3 * 2 * T * D
+    x, r, i = (torch.randn(B, T, D, device=DEV).to(dtype).requires_grad_() for _ in range(3))
+    decay, dh = torch.full((D,), -4.0, device=DEV), torch.randn(B, T, D, device=DEV).to(dtype)
+    whole = torch.autograd.grad(P.gated_scan(x, r, i, decay)[0], (x, r, i), dh)
+    for b in range(B):
+        one = [t.detach()[b:b + 1].requires_grad_() for t in (x, r, i)]
+        for got, want in zip(whole, torch.autograd.grad(P.gated_scan(*one, decay)[0], one, dh[b:b + 1])):
+            assert torch.equal(got[b], want[0])
+
+
+def test_scan_backward_beyond_32_bits_of_elements():
+    """2.2e9 elements of each gradient, the inputs rows that all batches share (stride 0): every batch's are what a batch of one gives, bit for bit."""
+    T, D, B = 65600, 1024, 33
+    torch.manual_seed(7)
+    one = [torch.randn(1, T, D, device=DEV, dtype=torch.bfloat16).requires_grad_() for _ in range(3)]
+    decay, dh = torch.full((D,), -5.0, device=DEV), torch.randn(1, T, D, device=DEV, dtype=torch.bfloat16)
+    want = torch.autograd.grad(P.gated_scan(*one, decay)[0], one, dh)
+    wide = [t.expand(B, T, D) for t in one]
+    got = torch.autograd.grad(P.gated_scan(*wide, decay)[0], wide, dh.expand(B, T, D))
+    for a, b in zip(got, want):
+        assert a.numel() > 2 ** 31 and torch.equal(a[-1], b[0]) and torch.equal(a[B // 2], b[0]) and torch.equal(a[0], b[0])
+
+
+def test_norm_backward_beyond_32_bits_of_elements():
+    D, rows = 4096, 540000
+    torch.manual_seed(8)
+    x = torch.zeros(rows, D, device=DEV, dtype=torch.bfloat16)
+    x[-3:] = torch.randn(3, D, device=DEV, dtype=torch.bfloat16)
+    u, pre = torch.randn(1, D, device=DEV, dtype=torch.bfloat16).expand(rows, D), torch.ones(D, device=DEV)
+    dy, dz = (torch.randn(1, D, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+
+    def gradients(x, u):
+        x, u = x.detach().requires_grad_(), u.detach().requires_grad_()
+        return torch.autograd.grad(P.block_norm(x, u, pre=pre), (x, u), (dy.expand_as(x), dz.expand_as(x)))
+
+    whole = gradients(x, u)
+    for got, want in zip(whole, gradients(x[-3:], u[-3:])):
+        assert got.numel() > 2 ** 31 and torch.equal(got[-3:], want)
+
+
+@pytest.mark.parametrize("bits,dtype", [(32, torch.float32), (8, torch.bfloat16)])
+def test_adamw_beyond_32_bits_of_elements(bits, dtype):
+    """A tensor of 2^31 + 5000 elements, and its last 5000 updated alone (they begin a chunk and a block of 256)."""
+    far, tail = 2 ** 31, 5000
+    n = far + tail
+    torch.manual_seed(9)
+
+    def moments(size):
+        if bits == 32:
+            return [torch.zeros(size, device=DEV)], [torch.zeros(size, device=DEV)]
+        blocks = -(-size // 256)
+        return ([(torch.zeros(size, dtype=torch.int8, device=DEV), torch.zeros(blocks, device=DEV))], [(torch.zeros(size, dtype=torch.uint8, device=DEV), torch.zeros(blocks, device=DEV))])
+
+    p, g = torch.zeros(n, dtype=dtype, device=DEV), torch.zeros(n, dtype=dtype, device=DEV)
+    p[far:], g[far:] = torch.randn(tail, device=DEV).to(dtype), torch.randn(tail, device=DEV).to(dtype)
+    g[5] = 1.0
+    q = p[far:].clone()
+    whole, part = moments(n), moments(tail)
+    steps = [torch.zeros(2, dtype=torch.int64, device=DEV) for _ in range(2)]
+    for _ in range(2):
+        adamw_step([p], [g], *whole, steps[0], lr=0.1)
+        adamw_step([q], [g[far:].clone()], *part, steps[1], lr=0.1)
+    assert torch.equal(p[far:], q) and float(p[5]) != 0 and float(p[6]) == 0
+    for a, b in zip(whole, part):
+        for s, t in zip(*[(k[0],) if bits == 32 else k[0] for k in (a, b)]):
+            assert torch.equal(s[-t.numel():], t)
+        if bits == 8:
+            wide, narrow = adamw_values(a)[0], adamw_values(b)[0]
+            assert torch.equal(wide[far:], narrow)
