@@ -178,12 +178,15 @@ class SolverNN:
 
     # ---- a warm start from action sequences that another solver found
     def record(self, sim_state, actions):
-        """Run ``actions`` (H, action_dim) from ``sim_state``: -> the observations (H, obs.dim) a policy would have seen before each of them."""
+        """Run ``actions`` (H, action_dim) from ``sim_state``: -> the observations (H, obs.dim) a policy would have seen before each of them.  No
+        frames are kept, so H is not bound by ``max_steps``; the environment is left at ``sim_state``."""
         env, seen = self.env, []
-        env.set_state(sim_state, self.cfg.softness, False)
+        softness, is_copy = env.primitives.get_softness(), env._is_copy
+        env.set_state(sim_state, self.cfg.softness, True)
         for a in actions:
             seen.append(self.obs.read(env.simulator.cur))
             env.step(a)
+        env.set_state(sim_state, softness, is_copy)
         return np.stack(seen)
 
     def _whole_sequences(self, obs, reset):
