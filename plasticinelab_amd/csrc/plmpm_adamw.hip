@@ -143,7 +143,7 @@ __device__ __forceinline__ float value_second(int code, float scale) {
 // the hardware's approximations (each within one unit in the last place: at most 4 units, 5e-7 relative, from the rounded ones): they give the
 // same code unless they come that near to the border of two, and only then is it computed in full -- for 4 % of the waves where the codes
 // lie evenly.  (With one distance for all codes, that of the largest, it was 40 %: 55 M elements 221 us, so 210.)
-// ordinary: the scale lies where its reciprocal and the quotient are ordinary numbers.
+// ordinary: the scale is a number and lies where its reciprocal and the quotient are ordinary numbers.
 __device__ __forceinline__ bool ordinary(float scale) { return scale > 1e-30f && scale < 1e30f; }
 __device__ __forceinline__ bool near_border(float q) { return fmaf(q, 6e-7f, fabsf(q - rintf(q))) > 0.5f; }
 __device__ __forceinline__ float exact_first(float m, float safe) { return sqrtf(fabsf(m) / safe) * 127.0f; }
@@ -161,8 +161,8 @@ __device__ __forceinline__ void codes_of(const float (&m)[4], const float (&v)[4
     if (again)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            qm[e] = exact_first(m[e], safe_m);
-            qv[e] = exact_second(v[e], safe_v);
+            qm[e] = fminf(exact_first(m[e], safe_m), 127.0f);      // (a block whose scale is infinite or no number comes here: a NaN has no integer)
+            qv[e] = fminf(exact_second(v[e], safe_v), 255.0f);
         }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -279,7 +279,7 @@ template <class T, int BITS, bool VECTOR> __device__ __forceinline__ void chunk_
                     tv = max(tv, as_u(v[e]) & 0x7fffffffu);
                 }
                 const float top_m = as_f(wave_max(tm)), top_v = as_f(wave_max(tv));
-                codes_of(m, v, top_m > 0.0f ? top_m : 1.0f, top_v > 0.0f ? top_v : 1.0f, cm[r], cv[r]);
+                codes_of(m, v, top_m == 0.0f ? 1.0f : top_m, top_v == 0.0f ? 1.0f : top_v, cm[r], cv[r]);
                 store4<int8_t, VECTOR>((int8_t*)t.m, from + e0, left, cm[r]);
                 store4<uint8_t, VECTOR>((uint8_t*)t.v, from + e0, left, cv[r]);
                 if ((VECTOR || left + lane4 > 0) && lane4 == 0) {
