@@ -7,7 +7,6 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -59,12 +58,15 @@ std::string name_of(at::ScalarType t) {
 int code_of(at::ScalarType t) { return t == at::kFloat ? PLMPM_NN_F32 : t == at::kBFloat16 ? PLMPM_NN_BF16 : t == at::kHalf ? PLMPM_NN_F16 : -1; }
 
 // What records the operations of a program sees a call's allocations and not its kernels: the recorded program would return memory that nothing wrote to.
+// (One look at the thread's dispatch keys: a recorder has one of these in there.)
 void not_recorded() {
-    if (torch::jit::tracer::isTracing()) throw EngineError("policy operators cannot be traced (torch.jit.trace): their kernels would be missing from the graph");
+    const c10::DispatchKeySet keys = c10::impl::tls_local_dispatch_key_set().included_;
+    if (!keys.has_any(c10::DispatchKeySet({c10::DispatchKey::Tracer, c10::DispatchKey::Python, c10::DispatchKey::PreDispatch}))) return;
+    if (keys.has(c10::DispatchKey::Tracer)) throw EngineError("policy operators cannot be traced (torch.jit.trace): their kernels would be missing from the graph");
     using Modes = c10::impl::TorchDispatchModeTLS;
     using Key = c10::impl::TorchDispatchModeKey;
-    bool found = c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
-    if (Modes::any_modes_set()) for (const Key key : {Key::PROXY, Key::FAKE, Key::FUNCTIONAL}) found = found || Modes::get_mode(key).has_value();
+    bool found = keys.has(c10::DispatchKey::PreDispatch);
+    for (const Key key : {Key::PROXY, Key::FAKE, Key::FUNCTIONAL}) found = found || Modes::get_mode(key).has_value();
     if (found) throw EngineError("policy operators cannot be traced (make_fx, fake or functional tensors): their kernels would be missing from the graph");
 }
 // the device that a call's kernels go to, made current, and its current stream
@@ -114,9 +116,12 @@ bool tracked(std::initializer_list<const Maybe*> ts) {
     return false;
 }
 // A forward-mode tangent that comes with a tensor would be lost: nothing here makes one for what a kernel writes.
+void no_tangent(const Tensor& t, const char* name) {
+    REFUSE_IF(t.unsafeGetTensorImpl()->autograd_meta() && t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode(),
+              name, " has no forward-mode derivative: a tensor with a tangent came in");
+}
 void no_tangents(std::initializer_list<const Maybe*> ts, const char* name) {
-    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
-    for (const Maybe* t : ts) REFUSE_IF(*t && (*t)->defined() && (*t)->_fw_grad(0).defined(), name, " has no forward-mode derivative: a tensor with a tangent came in");
+    for (const Maybe* t : ts) if (*t) no_tangent(**t, name);
 }
 // a tensor was changed in place: a graph that saved it has to notice (tensors of inference mode are in none)
 void written(const Tensor& t) { if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version(); }
@@ -271,14 +276,11 @@ std::tuple<Tensor, Tensor> gated_scan(Tensor x, Tensor r, Tensor i, Tensor decay
     return {h, last};
 }
 
-// whether two tensors' memory meets anywhere between the first and the last element of each
-bool meet(const Tensor& a, const Tensor& b) {
-    const auto end = [](const Tensor& t) {
-        int64_t last = 0;
-        for (int64_t k = 0; k < t.dim(); ++k) last += (t.size(k) - 1) * t.stride(k);
-        return (uintptr_t)memory(t) + (uintptr_t)((last + 1) * t.element_size());
-    };
-    return a.numel() && b.numel() && (uintptr_t)memory(a) < end(b) && (uintptr_t)memory(b) < end(a);
+// behind the last element of a tensor's memory
+uintptr_t end_of(const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t k = 0; k < t.dim(); ++k) last += (t.size(k) - 1) * t.stride(k);
+    return (uintptr_t)memory(t) + (uintptr_t)((last + 1) * (int64_t)t.element_size());
 }
 
 Tensor gated_scan_step(Tensor x, Tensor r, Tensor i, Tensor decay, const Tensor& state, double c) {
@@ -295,8 +297,12 @@ Tensor gated_scan_step(Tensor x, Tensor r, Tensor i, Tensor decay, const Tensor&
     }
     settle(decay);
     // an input that lies in the state would be read after another thread moved it on, unless each element is its own
-    for (Tensor* t : {&x, &r, &i}) if (meet(*t, state) && !(t->data_ptr() == state.data_ptr() && t->is_contiguous())) *t = t->clone(at::MemoryFormat::Contiguous);
-    if (meet(decay, state)) decay = decay.clone();
+    if (x.numel()) {
+        const uintptr_t from = (uintptr_t)memory(state), to = end_of(state);
+        const auto meets = [&](const Tensor& t) { return (uintptr_t)memory(t) < to && end_of(t) > from; };
+        for (Tensor* t : {&x, &r, &i}) if (meets(*t) && !((uintptr_t)memory(*t) == from && t->is_contiguous())) *t = t->clone(at::MemoryFormat::Contiguous);
+        if (meets(decay)) decay = decay.clone();
+    }
     const Tensor h = at::empty({x.size(0), x.size(1)}, x.options());
     if (h.numel()) {
         plmpm_scan s{};
@@ -470,19 +476,23 @@ int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }
 // The memory that a call touches through its lists of tensors: what it writes it may touch through one of them only, or two updates would race.
 struct Touched {
     struct Range {
-        uintptr_t from, to;
-        bool written;
+        uintptr_t from;
+        int64_t bytes;                  // below zero: only read
     };
     std::vector<Range> ranges;
-    void add(const void* p, int64_t bytes, bool written) { if (p && bytes) ranges.push_back({(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, written}); }
+    void reads(const void* p, int64_t bytes) { ranges.push_back({(uintptr_t)p, -bytes}); }
+    void writes(const void* p, int64_t bytes) { ranges.push_back({(uintptr_t)p, bytes}); }
     bool races() {
         std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.from < b.from; });
-        uintptr_t end[2] = {0, 0};      // of what was read or written so far; of what was written
-        for (const Range& r : ranges) {
-            if (r.from < end[r.written ? 0 : 1]) return true;
-            end[0] = std::max(end[0], r.to);
-            if (r.written) end[1] = std::max(end[1], r.to);
-        }
+        uintptr_t read = 0, written = 0;        // where what was read or written so far ends
+        for (const Range& r : ranges)
+            if (r.bytes > 0) {
+                if (r.from < std::max(read, written)) return true;
+                written = r.from + (uintptr_t)r.bytes;
+            } else {
+                if (r.from < written) return true;
+                read = std::max(read, r.from + (uintptr_t)-r.bytes);
+            }
         return false;
     }
 };
@@ -501,21 +511,21 @@ Maybe adamw_step(const std::vector<Tensor>& params, const std::vector<Maybe>& gr
     Touched memory_of;
     table.reserve(count);
     memory_of.ranges.reserve(5 * count + 1);
-    memory_of.add(memory(step), 2 * sizeof(int64_t), true);
+    memory_of.writes(memory(step), 2 * sizeof(int64_t));
     for (size_t k = 0; k < count; ++k) {
         if (!grads[k]) continue;
         const Tensor& p = params[k];
         Tensor g = *grads[k];
         const int64_t n = p.numel();
         const int code = code_of(p.scalar_type());
-        const Maybe mp(p);
-        no_tangents({&mp, &grads[k]}, "adamw_step");
+        no_tangent(p, "adamw_step");
+        no_tangent(g, "adamw_step");
         REFUSE_IF(code < 0 || !p.is_contiguous() || p.device() != step.device(), "parameter ", k, " has to be a contiguous float32, bfloat16 or float16 tensor on ", step.device());
         REFUSE_IF(g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes() || g.device() != step.device(),
                   "gradient ", k, " has to match its parameter: ", p.sizes(), " ", name_of(p.scalar_type()), " on ", step.device());
         settled(p, "a parameter");
         settle(g);
-        g = g.contiguous();
+        if (!g.is_contiguous()) g = g.contiguous();
         if (!g.is_same(*grads[k])) keep.push_back(g);
         plmpm_adamw_tensor t{};
         t.p = memory(p);
@@ -536,14 +546,14 @@ Maybe adamw_step(const std::vector<Tensor>& params, const std::vector<Maybe>& gr
             t.master = plain(*masters[k], n, step, "master", k);
         }
         if (!n) continue;
-        const int64_t size = p.element_size(), moment = n * (bits == 8 ? 1 : sizeof(float));
-        memory_of.add(t.p, n * size, true);
-        if (t.g != t.p) memory_of.add(t.g, n * size, false);       // (the parameter itself as its gradient: each element is read before it is written)
-        memory_of.add(t.m, moment, true);
-        memory_of.add(t.v, moment, true);
-        memory_of.add(t.m_scale, blocks_of(n) * sizeof(float), true);
-        memory_of.add(t.v_scale, blocks_of(n) * sizeof(float), true);
-        memory_of.add(t.master, n * sizeof(float), true);
+        const int64_t size = n * (code == PLMPM_NN_F32 ? 4 : 2), moment = bits == 8 ? n : 4 * n, scales = 4 * blocks_of(n);
+        memory_of.writes(t.p, size);
+        if (t.g != t.p) memory_of.reads(t.g, size);               // (the parameter itself as its gradient: each element is read before it is written)
+        memory_of.writes(t.m, moment);
+        memory_of.writes(t.v, moment);
+        if (t.m_scale) memory_of.writes(t.m_scale, scales);
+        if (t.v_scale) memory_of.writes(t.v_scale, scales);
+        if (t.master) memory_of.writes(t.master, 4 * n);
         table.push_back(t);
         touched.push_back(k);
     }
@@ -601,9 +611,10 @@ void adamw_values(const std::vector<Tensor>& codes, const std::vector<Tensor>& s
         o.push_back(plain(values[k], n, codes[0], "out", k));
         sizes.push_back(n);
         which.push_back(type == at::kByte);
-        memory_of.add(c.back(), n, false);
-        memory_of.add(s.back(), blocks_of(n) * sizeof(float), false);
-        memory_of.add(o.back(), n * sizeof(float), true);
+        if (!n) continue;
+        memory_of.reads(c.back(), n);
+        memory_of.reads(s.back(), 4 * blocks_of(n));
+        memory_of.writes(o.back(), 4 * n);
     }
     REFUSE_IF(memory_of.races(), "a tensor of out is in the list twice, or overlaps another tensor of the call");
     const Site site(codes[0]);
