@@ -183,10 +183,12 @@ class SolverNN:
         env, seen = self.env, []
         softness, is_copy = env.primitives.get_softness(), env._is_copy
         env.set_state(sim_state, self.cfg.softness, True)
-        for a in actions:
-            seen.append(self.obs.read(env.simulator.cur))
-            env.step(a)
-        env.set_state(sim_state, softness, is_copy)
+        try:
+            for a in actions:
+                seen.append(self.obs.read(env.simulator.cur))
+                env.step(a)
+        finally:
+            env.set_state(sim_state, softness, is_copy)
         return np.stack(seen)
 
     def _whole_sequences(self, obs, reset):

@@ -276,3 +276,23 @@ def test_recording_longer_than_the_frames_and_what_it_leaves():
     solver.record(state, actions[:2])
     solver.solve(callbacks=[lambda s, optim, loss, grad: losses.append(loss)])        # straight on, as imitation's warm start ends
     assert len(losses) == 1 and np.isfinite(losses[0])
+
+
+def test_a_recording_that_fails_leaves_the_environment_where_it_began(monkeypatch):
+    from plasticinelab_amd.optimizer.solver_nn import SolverNN
+    _, env, obs_dim = make_env(1000, 40)
+    solver = SolverNN(env, torch.nn.Linear(obs_dim, env.primitives.action_dim), horizon=2, n_observed_particles=40)
+    state, softness, copying = env.get_state()["state"], env.primitives.get_softness(), env._is_copy
+    step, steps = env.step, []
+
+    def failing(action):
+        if len(steps) == 2:
+            raise RuntimeError("stopped")
+        steps.append(action)
+        step(action)
+
+    monkeypatch.setattr(env, "step", failing)
+    with pytest.raises(RuntimeError, match="stopped"):
+        solver.record(state, np.full((4, env.primitives.action_dim), 0.3))
+    assert len(steps) == 2 and env.primitives.get_softness() == softness and env._is_copy == copying
+    assert all(np.array_equal(np.asarray(a), np.asarray(b)) for a, b in zip(env.get_state()["state"], state))
