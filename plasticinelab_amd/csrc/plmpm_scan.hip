@@ -411,7 +411,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
                 sr[s][v] = there ? g.both_r : 0.0f;
                 si[s][v] = g.both_i;
                 if ((cut >> s & 1)) {
-                    a[s][v] = 0.0f;
+                    a[s][v] = sr[s][v] = 0.0f;          // (r has no part in a step that begins anew, whatever it is)
                     m[s][v] = 1.0f;
                     PH[v] = g.si * x[v];
                 } else {
@@ -518,7 +518,7 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
             di[v] = g[v] * m[s][v] * x[v] * product_of(si[s][v]);
             const float q = reset || s >= left ? 0.0f : g[v] * pull[s][v];         // (behind the end: 0 times a state that may be infinite)
             dr[v] = q * (k2[v] * kLn2) * product_of(sr[s][v]);
-            sum[v] = fmaf(q, reset ? 0.0f : side_of(sr[s][v]), sum[v]);            // (a gate that is no number counts for nothing where its step begins anew)
+            sum[v] = fmaf(q, side_of(sr[s][v]), sum[v]);
         }
         if (mine.live && s < left) {
             const int64_t to = (b * A.T + t0 + s) * A.D;

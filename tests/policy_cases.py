@@ -284,3 +284,19 @@ def run_decay_gradient_of_many_rows(dev, B):
 
     one, many = gradient(1), gradient(B) / B
     assert float(((many - one).abs() / one.abs()).max()) <= 3.01 * R.U
+
+
+def run_gate_of_a_reset_that_is_no_number(dev, dtype):
+    """a is 0 where a step begins anew, whatever r is there: outputs and gradients as with any other r, and r's own gradient is 0."""
+    B, T, D = 2, 130, 70
+    x, r, i, decay, h0, reset = scan_inputs(42, B, T, D, dtype, resets=0.1)
+    assert reset.any()
+    for value in (float("nan"), float("inf"), float("-inf")):
+        results = []
+        for other in (value, 0.25):
+            leaves = [t.to(dev).requires_grad_() for t in (x, torch.where(reset[..., None], torch.full((), other, dtype=r.dtype), r), i, decay, h0)]
+            h, last = P.gated_scan(*leaves, reset.to(dev))
+            results.append([h, last, *torch.autograd.grad((h, last), leaves, (torch.ones_like(h), torch.ones_like(last)))])
+        for a, b in zip(*results):
+            assert torch.equal(a, b)
+        assert float(results[0][3].cpu()[reset].abs().sum()) == 0

@@ -474,3 +474,8 @@ def test_norm_gradients_of_gates_far_out(interpreter, tx, tu):
 
 def test_decay_gradient_of_many_rows(interpreter):
     cases.run_decay_gradient_of_many_rows(interpreter, 4099)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_gate_of_a_reset_that_is_no_number(interpreter, dtype):
+    cases.run_gate_of_a_reset_that_is_no_number(interpreter, dtype)

@@ -521,3 +521,8 @@ def test_adamw_beyond_32_bits_of_elements(bits, dtype):
         if bits == 8:
             wide, narrow = adamw_values(a)[0], adamw_values(b)[0]
             assert torch.equal(wide[far:], narrow)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_gate_of_a_reset_that_is_no_number(dtype):
+    cases.run_gate_of_a_reset_that_is_no_number(DEV, dtype)
