@@ -374,7 +374,8 @@ __global__ __launch_bounds__(W * 64, 4) void k_scan_backward(ScanArgs A) {
     // Kept for the second walk: x and dh as they came, a, m and both sides of the gates (sr, si).  What can be had from those in a few operations is
     // not: a register more here is one spilled to memory.  (8 x 2047 x 2048: with m s_i and s_i x a^2 / m held in m's place, 29 of them, 154 us instead of 131.  The
     // compiler would do the same by itself, hence forget and anew: calls in bf16 and fp16 without resets 165 and 171 us, with the 16 and 32
-    // registers that it keeps otherwise 185 and 196.  A kernel without the resets' selects kept more of them and was the slower one.)
+    // registers that it keeps otherwise 185 and 196.  A kernel without the resets' selects kept more of them and was the slower one.  These were taken with the
+    // gates themselves held; both sides of them cost 3 %, 14 to 26 spilled registers until they were taken back from one number, here and at the last walk.)
     Vec<T, VEC, LOOSE> rawx[S], rawg[S];
     float k2[VEC], a[S][VEC], sr[S][VEC], si[S][VEC], m[S][VEC], PA[VEC], PH[VEC], PE[VEC];
 #pragma unroll
@@ -570,7 +571,8 @@ __global__ __launch_bounds__(1024) void k_decay_grad(const float* part, const fl
 
 // Steps a wave and waves a workgroup of the two kernels.  Measured at 65537 steps x 1024 channels (forward) and 8 x 2047 x 2048 (both), bf16, us:
 // forward 16 x 8 135 / 75, 8 x 8 155 / 73, 8 x 16 162 / 83, 16 x 4 149 / 81; backward 8 x 8 at 136 registers 171, held to 128 (two workgroups a
-// CU, for some twenty spilled registers) 142, without those 128; 4 x 16 167, 8 x 16 180, 16 x 4 202.
+// CU, for some twenty spilled registers) 142, without those 128; 4 x 16 167, 8 x 16 180, 16 x 4 202.  (8 x 8 with both sides of the gates: 131 to 136.)  32 bits have
+// one channel a lane and 98 registers; 8 x 2047 x 1024 101 us of a floor of 90, so its tiles were not looked for apart.
 constexpr int kForwardSteps = 16, kForwardWaves = 8, kBackwardSteps = 8, kBackwardWaves = 8;
 // Gradients of more bytes than this go past the caches: the first of them would be gone from the 256 MB cache when the last is written, and x, r, i and
 // dh stay in it.  The backward kernel and a copy that reads its gradients, us: 25 MB 25.5 + 19.9 (past the caches 23.0 + 25.4), 75 MB 55.0 + 58.6
@@ -619,7 +621,7 @@ template <class T> void launch_step(const ScanArgs& A, hipStream_t st) {
 // 16 x 50 x 256: 1 channel 7.2 + 9.0 us, 2 channels 8.1 + 11.9.)
 int vector_of(const plmpm_scan* s) { return dtype_size(s->dtype) == 2 && s->width >= 64 ? 2 : 1; }
 // Whether such a row may begin between two words: an odd width, odd strides or pointers.  (16 bits, calls at
-// 8 x 2047 x 2047, forward and backward: 77 + 185 us; with 1 channel a lane 98 + 215.)
+// 8 x 2047 x 2047, forward and backward: 77 + 185 us; with 1 channel a lane 98 + 215.  The kernels alone: 84 + 150.)
 bool loose(const plmpm_scan* s, bool backward) {
     const int size = dtype_size(s->dtype);
     int bytes = 16;

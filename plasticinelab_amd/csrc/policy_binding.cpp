@@ -1,8 +1,8 @@
 // The policy-training operators as torch sees them: argument checks, allocation, autograd and the calls of the C entries (include/plmpm_policy.h),
 // whose addresses plasticinelab_amd/policy.py hands over.  No device code.  In C++ because many of these calls are shorter than what a Python
 // function around them costs, and because the autograd engine's thread would have to wait for the interpreter's lock: one step of
-// (1, 128) 5.5 us, with the same checks in Python 10.7; forward and backward of (16, 50, 256) 94 us, 159 in Python (torch's own product and its
-// backward, nothing else: 49); an update of 20 tensors 14 us, 48 in Python.
+// (1, 128) 5.6 us, with the checks in Python 10.7; forward and backward of (16, 50, 256) 93 us, 159 in Python (torch's own product and its
+// backward, nothing else: 52); an update of 20 tensors 14.5 us, 48 in Python.
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>

@@ -8,7 +8,8 @@ the policy built from them.
 
 Tensors live on one GPU; kernels go to the current stream of that GPU and nothing synchronises, so calls can be captured into a graph (a
 backward pass too, as long as no eager graph of the same leaves is alive: torch would join the two streams, which a capture forbids).
-There is no CPU path.  The reference's counterpart is a per-step MLP (plb/engine/nn/mlp.py:11-183) without a memory.
+There is no CPU path.  Derivatives are first ones in reverse mode; forward-mode tangents, second derivatives and tracing (torch.jit.trace, make_fx) are refused.
+The reference's counterpart is a per-step MLP (plb/engine/nn/mlp.py:11-183) without a memory.
 """
 from __future__ import annotations
 
@@ -76,7 +77,7 @@ def gated_scan(x, r, i, decay, h0=None, reset=None, *, c: float = 8.0):
 
 def gated_scan_step(x, r, i, decay, state, *, c: float = 8.0):
     """One step of ``gated_scan`` for (B, D) inputs: -> h (B, D); ``state`` (B, D) float32 moves on in place.  No gradients (serving and
-    evaluation; a differentiable step is ``gated_scan`` with T = 1)."""
+    evaluation; a differentiable step is ``gated_scan`` with T = 1).  Inputs may lie in the state: they are read as they were before it moves."""
     try:
         return _binding().gated_scan_step(x, r, i, decay, state, c)
     except TypeError:
