@@ -197,7 +197,11 @@ class SolverNN:
         row's is the policy's business).  A policy without a memory has nothing to reset."""
         if not hasattr(self.policy, "initial_state"):
             return self.policy(obs)
-        if "reset" in inspect.signature(self.policy.forward).parameters:
+        try:
+            at_once = "reset" in inspect.signature(self.policy.forward).parameters
+        except (TypeError, ValueError):                    # (a compiled forward has no signature to ask)
+            at_once = False
+        if at_once:
             out = self.policy(obs, reset=reset)
             if not isinstance(out, (tuple, list)) or len(out) != 2:
                 raise ValueError(f"a policy whose forward takes reset has to answer (actions, state), got {type(out).__name__}")

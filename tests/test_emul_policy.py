@@ -479,3 +479,17 @@ def test_decay_gradient_of_many_rows(interpreter):
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_gate_of_a_reset_that_is_no_number(interpreter, dtype):
     cases.run_gate_of_a_reset_that_is_no_number(interpreter, dtype)
+
+
+def test_imitation_by_a_policy_whose_forward_has_no_signature(interpreter):
+    class Compiled:
+        __signature__ = "none"
+
+        def __call__(self, obs):
+            raise AssertionError("not reached")
+
+    torch.manual_seed(10)
+    policy = Sums()
+    policy.forward = Compiled()
+    obs, target = torch.randn(2, 3, 4), torch.randn(2, 3, 2)
+    assert len(imitation(policy).imitate(obs, target, n_iters=1)) == 1
